@@ -38,6 +38,12 @@ class Prepared(Structure):
                 ("codes8", c_void_p), ("scales8", c_void_p), ("mask4", c_void_p)]
 
 
+class LinearWeights(Structure):
+    """struct b200moe_linear_weights"""
+    _fields_ = [("tiles", c_void_p), ("bias", c_void_p), ("rows", c_int64), ("k", c_int64), ("gated", c_int)]
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5, "swiglu_oai": 6}  # from 5 on gated
 LAYER_ROUTER, LAYER_SHARED, LAYER_OWN_SLOTS, LAYER_OWN_SHARED_OUT, LAYER_COMPACT = 1, 2, 4, 8, 16
 
 _P = c_void_p
@@ -107,6 +113,12 @@ SIGNATURES = {
     "b200moe_route_sort_partials": (c_int, [_P, c_int64, c_int64, c_int, _P, c_int64, c_int, c_int, c_float, c_int, _P, _P,
                                             _P, _P, _P, _P, _P, _P]),
     "b200moe_reduce_slots_add_rmsnorm_quant": (c_int, [_P, _P, _P, _P, c_float, c_int64, _P, _P, _P, _P, _P]),
+    "b200moe_add_rmsnorm_quant": (c_int, [_P, c_int64, _P, c_int64, _P, c_float, c_float, c_int64, c_int64, _P, c_int64, _P,
+                                          c_int64, _P, _P, _P]),
+    "b200moe_linear_weight_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "b200moe_preshuffle_linear": (c_int, [_P, _P, c_int64, c_int64, c_int, _P, _P]),
+    "b200moe_quant_mxfp8": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P, _P]),
+    "b200moe_linear": (c_int, [POINTER(LinearWeights), _P, _P, c_int64, c_int, _P, c_int64, _P, c_int64, _P, _P, _P, _P]),
     "b200moe_forward": (c_int, [POINTER(Weights), _P, _P, c_int64, _P, c_size_t, _P, _P, _P, _P]),
     "b200moe_forward_host": (c_int, [POINTER(Weights), _P, _P, c_int64, _P, _P, _P, c_size_t, _P, _P, _P, _P, _P]),
 }

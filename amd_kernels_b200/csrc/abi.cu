@@ -72,6 +72,7 @@ int set_wait_limit_shared_pair(unsigned long long ns);
 int set_wait_limit_pair(unsigned long long ns);
 int set_wait_limit_router(unsigned long long ns);
 int set_wait_limit_ep_sync(unsigned long long ns);
+int set_wait_limit_linear(unsigned long long ns);
 
 constexpr int64_t kSmallTokens = 32;  // up to here routing, sort and gather are one launch
 
@@ -146,6 +147,7 @@ extern "C" int b200moe_set_wait_limit_ns(uint64_t ns) {
   if (!r) r = b200moe::set_wait_limit_pair(ns);
   if (!r) r = b200moe::set_wait_limit_router(ns);
   if (!r) r = b200moe::set_wait_limit_ep_sync(ns);
+  if (!r) r = b200moe::set_wait_limit_linear(ns);
   return r;
 }
 

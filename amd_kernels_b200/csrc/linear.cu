@@ -1,0 +1,241 @@
+// The MXFP8 matrix product with bias, activation and residual in its epilogue: weight layout, row quantiser, entry point.
+#include "linear.cuh"
+#include "tc_host.cuh"
+#include "tc_ptx.cuh"
+
+namespace b200moe {
+
+// ------------------------------------------------------------------------------------------------ weight layout
+// One CTA per (row of a tile, tile): 16-byte pieces of the source row into the swizzled image, its scales into the atoms.
+__global__ void preshuffle_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int k,
+                                         int tiles_k, int gated, uint8_t* __restrict__ out) {
+  const int64_t t = blockIdx.x >> 7;
+  const int r = static_cast<int>(blockIdx.x & 127u);
+  int64_t src = t * 128 + r;
+  bool have = src < rows;
+  if (gated) {
+    const int g = r >> 5;
+    const int64_t half = rows / 2, i = 64 * t + 32 * (g >> 1) + (r & 31);
+    have = i < half;
+    src = (g & 1) ? half + i : i;
+  }
+  uint8_t* tile0 = out + t * tiles_k * kLinearRecordBytes;
+  for (int j = threadIdx.x; j < tiles_k * 8; j += blockDim.x) {
+    const int kt = j >> 3, c = j & 7;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (have && j * 16 < k) v = *reinterpret_cast<const uint4*>(codes + src * k + j * 16);
+    *reinterpret_cast<uint4*>(tile0 + static_cast<int64_t>(kt) * kLinearRecordBytes + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+  }
+  for (int j = threadIdx.x; j < tiles_k * 4; j += blockDim.x)
+    tile0[static_cast<int64_t>(j >> 2) * kLinearRecordBytes + kLinearCodeBytes + atom_offset(r, j & 3)] =
+        have && j * 32 < k ? scales[src * (k / 32) + j] : static_cast<uint8_t>(127);
+}
+
+// ------------------------------------------------------------------------------------------------ row quantiser
+// bf16 rows -> E4M3 codes and E8M0 scales, row-major. Four lanes to a block of 32 values, 16 bytes a lane; vectors of all rows in a row.
+__global__ void __launch_bounds__(256) quant_mxfp8_kernel(const uint4* x, int64_t x_stride, int64_t rows, int vectors, uint2* codes,
+                                                          uint8_t* scales) {
+  pdl_enter(x);
+  const int64_t total = rows * vectors;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const bool in = i < total;
+  const int64_t row = in ? i / vectors : 0;
+  const int c = static_cast<int>(i - row * vectors);
+  float v[8];
+  unpack_bf16x8(in ? __ldcg(x + row * x_stride + c) : make_uint4(0u, 0u, 0u, 0u), v);
+  float amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const int e = linear_scale(amax);
+  const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+  if (!in) return;
+  codes[i] = make_uint2(pack_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                        pack_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+  if ((c & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(e);
+}
+
+// ------------------------------------------------------------------------------------------------ product on CUDA cores
+// 16 tokens x one weight tile per CTA, fp32 FMAs on values decoded into shared memory; sums in rising K.
+__device__ __forceinline__ float e4m3_value(uint32_t c) {
+  const uint32_t m = c & 0x7fu;
+  float v = m < 8u ? static_cast<float>(m) * 0.001953125f : __uint_as_float((m << 20) + (120u << 23));
+  if (m == 0x7fu) v = __uint_as_float(0x7fc00000u);
+  return (c & 0x80u) ? -v : v;
+}
+
+__global__ void __launch_bounds__(256) linear_simt_kernel(const LinearArgs args) {
+  pdl_launch_dependents();
+  pdl_wait();
+  LinearArgs a = args;
+  launder(a.tiles);
+  launder(a.codes);
+  launder(a.scales);
+  launder(a.residual);
+  extern __shared__ float sm[];
+  float* ws = sm;               // [128][129]
+  float* xs = sm + 128 * 129;   // [16][128], later the sums
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16;
+  const int tn = blockIdx.x, r = threadIdx.x & 127, half = threadIdx.x >> 7;
+  float acc[8] = {};
+  for (int kt = 0; kt < a.tiles_k; ++kt) {
+    const uint8_t* rec = a.tiles + (static_cast<int64_t>(tn) * a.tiles_k + kt) * kLinearRecordBytes;
+    for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+      const int rr = i >> 7, c = i & 127;
+      const float s = e8m0_value(__ldcg(rec + kLinearCodeBytes + atom_offset(rr, c >> 5)));
+      ws[rr * 129 + c] = e4m3_value(__ldcg(rec + rr * 128 + (((c >> 4) ^ (rr & 7)) << 4) + (c & 15))) * s;
+    }
+    for (int i = threadIdx.x; i < 16 * 128; i += 256) {
+      const int64_t row = row0 + (i >> 7);
+      const int c = kt * 128 + (i & 127);
+      xs[i] = row < a.m && c < a.k ? e4m3_value(__ldcg(a.codes + row * a.k + c)) * e8m0_value(__ldcg(a.scales + row * (a.k / 32) + c / 32)) : 0.0f;
+    }
+    __syncthreads();
+    for (int c = 0; c < 128; ++c)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) acc[t] = fmaf(ws[r * 129 + c], xs[(half * 8 + t) * 128 + c], acc[t]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) xs[(half * 8 + t) * 128 + r] = acc[t];
+  __syncthreads();
+  const bool gated = linear_gated(a.act);
+  const int groups = gated ? 2 : 4;  // of 32 output columns
+  const int t = threadIdx.x / groups, g = threadIdx.x % groups;
+  const int64_t row = row0 + t;
+  const int col0 = tn * 32 * groups + 32 * g;
+  if (t >= 16 || row >= a.m || col0 >= a.n) return;
+  float y[32], amax = 0.0f;
+  for (int j = 0; j < 32; ++j) {
+    const int c = col0 + j;
+    if (gated) {
+      float p = xs[t * 128 + 64 * g + j], u = xs[t * 128 + 64 * g + 32 + j];
+      if (a.bias != nullptr) p += __ldcg(a.bias + c), u += __ldcg(a.bias + a.n + c);
+      y[j] = activate_gated(p, u, a.act);
+    } else {
+      float p = xs[t * 128 + 32 * g + j];
+      if (a.bias != nullptr && c < a.n) p += __ldcg(a.bias + c);
+      y[j] = activate(p, a.act);
+    }
+    if (a.residual != nullptr && c < a.n) y[j] += __bfloat162float(a.residual[row * a.residual_stride + c]);
+    amax = fmaxf(amax, fabsf(y[j]));
+  }
+  if (a.out != nullptr) {
+    for (int j = 0; j < 32 && col0 + j < a.n; ++j) a.out[row * a.out_stride + col0 + j] = __float2bfloat16_rn(y[j]);
+    return;
+  }
+  const int e = linear_scale(amax);
+  const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+  for (int j = 0; j < 32; ++j) a.out_codes[row * a.n + col0 + j] = static_cast<uint8_t>(cvt_e4m3x2(y[j] * inv, 0.0f));
+  a.out_scales[row * (a.n / 32) + col0 / 32] = static_cast<uint8_t>(e);
+}
+
+static int launch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+  constexpr int kSmem = (128 * 129 + 16 * 128) * 4;
+  static PerDeviceOnce once;
+  const int rc = once.run([] {
+    return static_cast<int>(cudaFuncSetAttribute(linear_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  });
+  if (rc) return rc;
+  B200MOE_LAUNCH(linear_simt_kernel, dim3(a.tiles_n, static_cast<unsigned>((a.m + 15) / 16)), 256, kSmem, stream, a);
+  return 0;
+}
+
+static int64_t linear_row_tiles(int64_t rows) { return (rows + 127) / 128; }  // gated: 64 output columns, 128 rows, as well
+static int64_t linear_k_tiles(int64_t k) { return (k + 127) / 128; }
+
+static bool linear_dims(int64_t rows, int64_t k, int gated) {
+  if (rows < 8 || k < 32 || k % 32 || rows % (gated ? 64 : 8) || rows > B200MOE_LINEAR_MAX_DIM || k > B200MOE_LINEAR_MAX_DIM) return false;
+  // the weights seen as rows of 128 bytes are counted in 32 bits (274 GB)
+  return linear_row_tiles(rows) * linear_k_tiles(k) <= INT32_MAX / 132;
+}
+
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  return a && b && pa < pb + nb && pb < pa + na;
+}
+
+int set_wait_limit_linear(unsigned long long ns) { return set_wait_limit_here(ns); }
+
+}  // namespace b200moe
+
+extern "C" size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated) {
+  using namespace b200moe;
+  if (!linear_dims(rows, k, gated)) return 0;
+  return static_cast<size_t>(linear_row_tiles(rows)) * linear_k_tiles(k) * kLinearRecordBytes;
+}
+
+extern "C" int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated,
+                                         uint8_t* tiles, void* stream) {
+  using namespace b200moe;
+  if (!codes || !scales || !tiles || !linear_dims(rows, k, gated)) return B200MOE_E_ARG;
+  if (misaligned(codes, 16) || misaligned(tiles, 128)) return B200MOE_E_ALIGN;
+  B200MOE_LAUNCH_PLAIN(preshuffle_linear_kernel, dim3(static_cast<unsigned>(linear_row_tiles(rows) * 128)), 128, 0,
+                       static_cast<cudaStream_t>(stream), codes, scales, rows, static_cast<int>(k),
+                       static_cast<int>(linear_k_tiles(k)), gated, tiles);
+  return 0;
+}
+
+extern "C" int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t rows, int64_t k, uint8_t* codes8, uint8_t* scales8,
+                                   void* stream) {
+  using namespace b200moe;
+  if (rows < 0 || rows > B200MOE_LINEAR_MAX_ROWS || k < 32 || k % 32 || k > B200MOE_LINEAR_MAX_DIM) return B200MOE_E_ARG;
+  if (rows == 0) return 0;
+  if (!x_bf16 || !codes8 || !scales8) return B200MOE_E_ARG;
+  if (rows > 1 && x_stride < k && x_stride != 0) return B200MOE_E_ARG;
+  if (misaligned(x_bf16, 16) || misaligned(codes8, 8) || (rows > 1 && (x_stride & 7))) return B200MOE_E_ALIGN;
+  const int64_t grid = (rows * (k / 8) + 255) / 256;
+  if (grid > 0x7fffffff) return B200MOE_E_ARG;
+  B200MOE_LAUNCH(quant_mxfp8_kernel, dim3(static_cast<unsigned>(grid)), 256, 0, static_cast<cudaStream_t>(stream),
+                 static_cast<const uint4*>(x_bf16), x_stride / 8, rows, static_cast<int>(k / 8), reinterpret_cast<uint2*>(codes8),
+                 scales8);
+  return 0;
+}
+
+extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
+                              int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
+                              uint8_t* out_codes8, uint8_t* out_scales8, int32_t* status, void* stream) {
+  using namespace b200moe;
+  if (!w || m < 0 || m > B200MOE_LINEAR_MAX_ROWS) return B200MOE_E_ARG;
+  if (!linear_dims(w->rows, w->k, w->gated) || activation < B200MOE_ACT_NONE || activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
+  if ((w->gated != 0) != (activation >= B200MOE_ACT_SWIGLU)) return B200MOE_E_ARG;
+  if (m == 0) return 0;
+  if (!w->tiles || !codes8 || !scales8 || !status) return B200MOE_E_ARG;
+  if ((out_bf16 != nullptr) == (out_codes8 != nullptr) || (out_codes8 != nullptr) != (out_scales8 != nullptr)) return B200MOE_E_ARG;
+  LinearArgs a;
+  const int64_t n = w->gated ? w->rows / 2 : w->rows;
+  if (out_codes8 && n % 32) return B200MOE_E_ARG;
+  if (m > 1 && ((out_bf16 && out_stride < n) || (residual_bf16 && residual_stride < n && residual_stride != 0))) return B200MOE_E_ARG;
+  if (misaligned(w->tiles, 128) || misaligned(codes8, 16) || misaligned(out_bf16, 16) || misaligned(out_codes8, 16) ||
+      misaligned(residual_bf16, 16) || misaligned(w->bias, 4) || (m > 1 && ((out_bf16 && (out_stride & 7)) || (residual_bf16 && (residual_stride & 7)))))
+    return B200MOE_E_ALIGN;
+  // the rows of out may be those of the residual (a thread stores where it has loaded); any other overlap with an input is refused
+  const void* outs[3] = {out_bf16, out_codes8, out_scales8};
+  const size_t out_bytes[3] = {((m - 1) * static_cast<size_t>(out_stride) + n) * 2, static_cast<size_t>(m) * n, static_cast<size_t>(m) * (n / 32)};
+  const size_t res_bytes = ((m - 1) * static_cast<size_t>(residual_stride) + n) * 2;
+  for (int i = 0; i < 3; ++i) {
+    if (overlap(outs[i], out_bytes[i], codes8, static_cast<size_t>(m) * w->k) || overlap(outs[i], out_bytes[i], scales8, static_cast<size_t>(m) * (w->k / 32)))
+      return B200MOE_E_ARG;
+    const bool same = i == 0 && out_bf16 == residual_bf16 && (m == 1 || out_stride == residual_stride);
+    if (!same && overlap(outs[i], out_bytes[i], residual_bf16, res_bytes)) return B200MOE_E_ARG;
+  }
+  if (overlap(out_codes8, out_bytes[1], out_scales8, out_bytes[2])) return B200MOE_E_ARG;
+  a.tiles = w->tiles;
+  a.bias = w->bias;
+  a.codes = codes8;
+  a.scales = scales8;
+  a.residual = static_cast<const __nv_bfloat16*>(residual_bf16);
+  a.out = static_cast<__nv_bfloat16*>(out_bf16);
+  a.out_codes = out_codes8;
+  a.out_scales = out_scales8;
+  a.m = m;
+  a.residual_stride = residual_stride;
+  a.out_stride = out_stride;
+  a.k = static_cast<int>(w->k);
+  a.n = static_cast<int>(n);
+  a.tiles_n = static_cast<int>(linear_row_tiles(w->rows));
+  a.tiles_k = static_cast<int>(linear_k_tiles(w->k));
+  a.act = activation;
+  return launch_linear(a, status, static_cast<cudaStream_t>(stream));
+}

@@ -8,7 +8,9 @@ from ..mxfp4_h6144_i768_e128_top4 import shared_expert as _shared
 from ..mxfp4_h6144_i768_e128_top4.chain import mxfp4_moe, warm_up_mxfp4_moe, route, mxfp4_moe_experts
 from ..mxfp4_h6144_i768_e128_top4.prepared_input import MoeInput, MoeInputCompact, prepare_mxfp4_moe, gather_mxfp4_moe
 from ..mxfp4_h6144_i768_e128_top4.shared_expert import set_dbo_query
-from ..mxfp4_h6144_i768_e128_top4.tail import slots4_add_rmsnorm_mxfp8
+from ..mxfp4_h6144_i768_e128_top4.tail import TailOutput, slots4_add_rmsnorm_mxfp8
+from ..mxfp4_h6144_i768_e128_top4.add_rmsnorm import add_rmsnorm_mxfp8
+from ..mxfp4_h6144_i768_e128_top4.linear import LinearWeights, mxfp8_linear, mxfp8_quant
 
 H, I, E, TOPK = 6144, 1536, 128, 4  # noqa: E741
 SWIGLU_OAI = (1.702, 7.0, 1.0)  # alpha, limit, beta (up + beta)
@@ -35,4 +37,5 @@ def unsupported_reason(w13, w13_scale, w2, w2_scale, shared_w13, shared_s13, sha
 
 __all__ = ["MoeWeights", "SharedWeights", "mxfp4_moe", "warm_up_mxfp4_moe", "MoeInput", "MoeInputCompact",
            "prepare_mxfp4_moe", "gather_mxfp4_moe", "set_dbo_query", "unsupported_reason", "route", "mxfp4_moe_experts",
-           "slots4_add_rmsnorm_mxfp8", "SHARED_FULL"]
+           "slots4_add_rmsnorm_mxfp8", "TailOutput", "add_rmsnorm_mxfp8", "LinearWeights", "mxfp8_linear", "mxfp8_quant",
+           "SHARED_FULL"]

@@ -1,0 +1,137 @@
+"""The MXFP8 matrix product with bias, activation and residual in its epilogue on B200: the projections around the MoE layer. It reads
+the MXFP8 rows that ``slots4_add_rmsnorm_mxfp8`` and ``add_rmsnorm_mxfp8`` hand out (or quantises bf16 rows itself) and writes bf16
+rows, added to the residual stream if asked, or MXFP8 rows for the next product. E4M3 codes with one E8M0 scale per 32 elements
+on both sides, fp32 accumulation; the shared expert (``SharedWeights``) is two such products of fixed shape."""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+
+import torch
+
+from ... import _lib
+from .add_rmsnorm import _rows, check_mxfp8, launch_on
+from .chain import status_word
+
+MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
+
+
+@dataclass
+class LinearWeights:
+    """A weight [rows, k] in the kernels' layout, built once by ``from_row_major`` before graph capture. ``tiles`` u8 [row tiles, K-tiles,
+    16896]: records of 128 rows x 128 K-elements of E4M3 codes in the 128-byte-swizzled shared-memory image, then the tile's scale
+    atom. ``bias`` fp32 [rows] or None."""
+    tiles: torch.Tensor
+    bias: torch.Tensor | None
+    rows: int
+    k: int
+    gated: bool
+    _abi: object = field(default=None, repr=False, compare=False)
+
+    @property
+    def n(self) -> int:
+        """Output columns."""
+        return self.rows // 2 if self.gated else self.rows
+
+    def abi(self) -> _lib.LinearWeights:
+        """``struct b200moe_linear_weights`` over this object's tensors as they are now."""
+        a, bias = self._abi, None if self.bias is None else self.bias.data_ptr()
+        if a is None or a.tiles != self.tiles.data_ptr() or a.bias != bias:
+            a = self._abi = _lib.LinearWeights(self.tiles.data_ptr(), bias, self.rows, self.k, int(self.gated))
+        return a
+
+    @classmethod
+    def from_row_major(cls, w, scale, bias=None, *, gated: bool = False):
+        """From row-major E4M3 codes [rows, K] and E8M0 scales [rows, K / 32] (one byte an element, any dtype of that size) and a bias
+        [rows] of any floating type. K a multiple of 32, rows a multiple of 8. ``gated``: the first half of the rows are the gate,
+        the second half the up projection (each a multiple of 32); the activation of the call is then a gated one."""
+        if w.ndim != 2 or w.element_size() != 1 or scale.element_size() != 1:
+            raise ValueError("expected codes [rows, K] and scales [rows, K / 32] of one byte each")
+        rows, k = w.shape
+        if not w.is_cuda or scale.device != w.device or (bias is not None and bias.device != w.device):
+            raise ValueError("weights must be CUDA tensors of one device")
+        nbytes = int(_lib.load().b200moe_linear_weight_bytes(rows, k, int(gated)))
+        if nbytes == 0:
+            raise ValueError(f"unsupported weight [{rows}, {k}]: K a multiple of 32, rows a multiple of {64 if gated else 8}, both up to {MAX_DIM}")
+        if scale.shape != (rows, k // 32):
+            raise ValueError(f"scales: needs [{rows}, {k // 32}]")
+        if bias is not None:
+            if bias.shape != (rows,) or not bias.is_floating_point():
+                raise ValueError(f"bias: needs [{rows}] of a floating type")
+            bias = bias.detach().float().contiguous()
+        codes, scales = w.contiguous().view(torch.uint8), scale.contiguous().view(torch.uint8)
+        if codes.data_ptr() & 15:
+            codes = codes.clone()
+        tiles = torch.empty((-(-rows // 128), -(-k // 128), nbytes // (-(-rows // 128) * -(-k // 128))), dtype=torch.uint8, device=w.device)
+        launch_on(w.device, _lib.load().b200moe_preshuffle_linear,
+                  (codes.data_ptr(), scales.data_ptr(), rows, k, int(gated), tiles.data_ptr()), "preshuffle_linear")
+        return cls(tiles, bias, rows, k, bool(gated))
+
+
+def mxfp8_quant(x: torch.Tensor, *, out=None):
+    """bf16 [M, K] -> (E4M3 codes u8 [M, K], E8M0 scales u8 [M, K / 32]): ``shared_quant_rows`` at any width that is a multiple of 32
+    (the same bits at 6144; an infinite value saturates and keeps its block's scale finite). Rows any multiple of 8 elements apart."""
+    if x.ndim != 2:
+        raise ValueError("expected BF16 [M, K]")
+    (m, k), dev = x.shape, x.device
+    if k < 32 or k % 32 or k > MAX_DIM or m > MAX_ROWS:
+        raise ValueError(f"rows of {k} columns (needs a multiple of 32, up to {MAX_DIM}; up to {MAX_ROWS} rows)")
+    stride = _rows("x", x, m, k, dev, shared_row=True)
+    if out is None:
+        out = torch.empty((m, k), dtype=torch.uint8, device=dev), torch.empty((m, k // 32), dtype=torch.uint8, device=dev)
+    else:
+        check_mxfp8("out", *out, m, k, dev)
+    launch_on(dev, _lib.load().b200moe_quant_mxfp8, (x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr()), "quant_mxfp8")
+    return out
+
+
+def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual: torch.Tensor | None = None,
+                 mxfp8_out: bool = False, out=None):
+    """``y = activation(x @ w.T + bias) + residual``, fp32 until one rounding at the end.
+
+    ``x``: MXFP8 rows as a pair (codes [M, K], scales [M, K / 32]), or bf16 [M, K], which ``mxfp8_quant`` quantises first. M may be 0.
+    ``activation``: None, "relu", "silu", "gelu" (exact), "gelu_tanh"; for gated weights "swiglu" (silu(gate) * up) or "swiglu_oai"
+    (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart (or one
+    expanded row). Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.
+    ``out``: where the result goes, a bf16 tensor or a pair (``mxfp8_out`` is then not read); a bf16 ``out`` may be the residual
+    itself. The sums of one call repeat bit for bit; between calls of different M they may be split along K in another way."""
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    if (act >= 5) != w.gated:
+        raise ValueError(f"activation {activation!r} on {'gated' if w.gated else 'plain'} weights")
+    k, n, dev = w.k, w.n, w.tiles.device
+    pair = isinstance(x, (tuple, list))
+    if not pair and not isinstance(x, torch.Tensor):
+        raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
+    rows = x[0] if pair else x
+    if rows.ndim != 2 or rows.shape[1] != k:
+        raise ValueError(f"expected rows of {k} columns")
+    m = rows.shape[0]
+    if m > MAX_ROWS:
+        raise ValueError(f"more than {MAX_ROWS} rows")
+    if rows.device != dev or dev.type != "cuda":
+        raise ValueError(f"x is on {rows.device}, the weights on {dev}: expected one CUDA device")
+    if pair:
+        codes, scales = x
+        check_mxfp8("x", codes, scales, m, k, dev)
+    else:
+        codes, scales = mxfp8_quant(x)
+    rs = 0 if residual is None else _rows("residual", residual, m, n, dev, shared_row=True)
+    os, oc, osc = n, None, None
+    if out is None:
+        if mxfp8_out:
+            out = torch.empty((m, n), dtype=torch.uint8, device=dev), torch.empty((m, n // 32), dtype=torch.uint8, device=dev)
+        else:
+            out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+    if isinstance(out, torch.Tensor):
+        os, y = _rows("out", out, m, n, dev), out.data_ptr()
+    else:
+        if n % 32:
+            raise ValueError(f"MXFP8 output of {n} columns (needs a multiple of 32)")
+        check_mxfp8("out", *out, m, n, dev)
+        y, oc, osc = None, out[0].data_ptr(), out[1].data_ptr()
+    launch_on(dev, _lib.load().b200moe_linear,
+              (ctypes.byref(w.abi()), codes.data_ptr(), scales.data_ptr(), m, act, None if residual is None else residual.data_ptr(), rs,
+               y, os, oc, osc, status_word(dev).data_ptr()), "linear")
+    return out

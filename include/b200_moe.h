@@ -410,6 +410,64 @@ size_t b200moe_workspace_bytes_x(int64_t tokens, int num_experts);
 int b200moe_forward_x(const b200moe_weights* w, const void* x_bf16, int64_t tokens, void* workspace,
                       size_t workspace_bytes, void* slots_bf16, void* out_bf16, int32_t* status, void* stream);
 
+/* Residual addition, RMS norm and MXFP8 / bf16 rows of any width, where there are no slots to sum: the tail's steps behind its sum
+ * (amd_kernels/norm/gemma_add_rmsnorm_h6144/reference.py steps 2-4), the same bits at width 6144 and weight_offset 1.
+ *   s = fp32(x) + fp32(residual) (residual may be null: s = x);  residual_out = bf16(s) (may be null);
+ *   y = (s * rstd) * (weight + weight_offset), rstd = 1/sqrt(sum(s^2)/h + eps);  normed = bf16(y) (may be null);
+ *   codes8 [rows][h] / scales8 [rows][h/32] as the tail's (both may be null). At least one output is given.
+ * x, residual, residual_out and normed are bf16 rows with a stride of their own in elements (a multiple of 8, at least h; a residual
+ * stride of 0 is one row for all), weight bf16 [h]; 16-byte aligned, codes8 8-byte. h: a multiple of 32, up to
+ * B200MOE_NORM_MAX_H. residual_out or normed may be x or residual (the same address and stride); any other overlap of an output is
+ * B200MOE_E_ARG. The bits of a row do not depend on the other rows. rows may be 0. */
+#define B200MOE_NORM_MAX_H 65536
+int b200moe_add_rmsnorm_quant(const void* x_bf16, int64_t x_stride, const void* residual_bf16, int64_t residual_stride,
+                              const void* weight_bf16, float weight_offset, float eps, int64_t rows, int64_t h,
+                              void* residual_out_bf16, int64_t residual_out_stride, void* normed_bf16, int64_t normed_stride,
+                              uint8_t* codes8, uint8_t* scales8, void* stream);
+
+/* The MXFP8 matrix product with its epilogue, any shape: what reads the rows of the tail and of the norm above (the next
+ * projection), and the dense SwiGLU blocks around MoE layers.
+ *   p = x @ w^T + bias;  a = act(p);  y = a + residual;  out = bf16(y), or MXFP8 of the fp32 y
+ * x: E4M3 codes [m][k], E8M0 scales [m][k/32] (any alignment); fp32 accumulators, one rounding at the end. Gated activations: the
+ * weight rows are n gate rows, then n up rows, y has n columns: SWIGLU silu(g) * u; SWIGLU_OAI g = min(g, 7), u = clamp(u, -7, 7),
+ * g * sigmoid(1.702 g) * (u + 1). GELU is the exact form, GELU_TANH the tanh one.
+ * MXFP8 output: scale byte = clamp(ceil(log2(amax / 448)) + 127, 1, 254) per 32 columns, the shared expert's rule.
+ * k: a multiple of 32. Weight rows: a multiple of 8, with MXFP8 output of 32, gated of 64. */
+#define B200MOE_LINEAR_MAX_DIM (1 << 20)
+#define B200MOE_LINEAR_MAX_ROWS (1 << 24)
+#define B200MOE_ACT_NONE 0
+#define B200MOE_ACT_RELU 1
+#define B200MOE_ACT_SILU 2
+#define B200MOE_ACT_GELU 3
+#define B200MOE_ACT_GELU_TANH 4
+#define B200MOE_ACT_SWIGLU 5 /* from here on gated */
+#define B200MOE_ACT_SWIGLU_OAI 6
+
+/* Weights: row-major E4M3 codes [rows][k] (16-byte aligned) and E8M0 scales [rows][k/32] -> tiles, b200moe_linear_weight_bytes bytes
+ * (0: a shape that is not taken), 128-byte aligned. Layout: [row tile of 128][K-tile of 128] records of 16384 bytes of codes in the
+ * 128-byte-swizzled image and one scale atom; what is beyond the matrix is zero; gated rows interleaved [gate 32 | up 32] twice a tile. */
+size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated);
+int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated, uint8_t* tiles,
+                              void* stream);
+
+/* bf16 rows (x_stride elements apart, a multiple of 8, or 0) -> codes8 [rows][k], scales8 [rows][k/32], the rule above. */
+int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t rows, int64_t k, uint8_t* codes8, uint8_t* scales8,
+                        void* stream);
+
+typedef struct b200moe_linear_weights {
+  const uint8_t* tiles; /* b200moe_preshuffle_linear */
+  const float* bias;    /* fp32 [rows], in the order of the checkpoint's rows, or null */
+  int64_t rows, k;
+  int gated;
+} b200moe_linear_weights;
+
+/* codes8 16-byte aligned; residual and out are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a residual stride of
+ * 0 is one row for all). Either out or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the residual (same
+ * address and stride); any other overlap of an output with an input is B200MOE_E_ARG. No workspace, one launch. m may be 0. */
+int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m, int activation,
+                   const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride, uint8_t* out_codes8,
+                   uint8_t* out_scales8, int32_t* status, void* stream);
+
 /* The whole layer in one call, with or without the shared expert (MOE/chain.py:127-197 mxfp4_moe; the shared expert runs
  * beside the routed experts inside the same launches up to 512 tokens; above, its two GEMMs are launches of their own, on
  * side_stream when one is given: they start behind the input's quantisation and are joined before the reduce, or before the call

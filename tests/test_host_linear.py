@@ -1,0 +1,146 @@
+"""Refusals of the norm without slots and of the MXFP8 product, without a GPU: the entry points' own checks and the C ABI's."""
+import ctypes
+
+import pytest
+import torch
+
+from amd_kernels_b200 import _lib
+from amd_kernels_b200.moe import mxfp4_h6144_i768_e128_top4 as P
+from amd_kernels_b200.moe import mxfp4_h6144_i1536_e128_top4 as P2
+from amd_kernels_b200.moe.mxfp4_h6144_i768_e128_top4 import linear as L
+
+BF16, U8 = torch.bfloat16, torch.uint8
+
+
+def at(a):
+    return None if a is None else ctypes.c_void_p(a)
+
+
+def test_both_packages_have_them():
+    for name in ("TailOutput", "add_rmsnorm_mxfp8", "LinearWeights", "mxfp8_linear", "mxfp8_quant"):
+        assert name in P.__all__ and name in P2.__all__ and getattr(P, name) is getattr(P2, name)
+
+
+# ------------------------------------------------------------------------------------------------ the norm
+def norm_call(lib, x=4096, xs=64, r=1 << 20, rs=64, w=256, rows=4, h=64, ro=2 << 20, ros=64, n=3 << 20, ns=64, c=4 << 20, s=5 << 20):
+    return lib.b200moe_add_rmsnorm_quant(at(x), xs, at(r), rs, at(w), 1.0, 1e-6, rows, h, at(ro), ros, at(n), ns, at(c), at(s), None)
+
+
+@pytest.mark.parametrize("inter", [768, 1536])
+def test_c_abi_refuses_norm_arguments(inter):
+    lib = _lib.load(inter)
+    A, L_ = _lib.E_ARG, _lib.E_ALIGN
+    for bad in (dict(x=None), dict(w=None), dict(rows=-1), dict(h=0), dict(h=48), dict(h=65568), dict(c=None), dict(s=None),
+                dict(r=None), dict(ro=None, n=None, c=None, s=None), dict(xs=56), dict(rs=56), dict(ros=0), dict(ns=32), dict(xs=0)):
+        assert norm_call(lib, **bad) == A, bad
+    for bad in (dict(x=4104), dict(r=(1 << 20) + 2), dict(w=264), dict(ro=(2 << 20) + 8), dict(n=(3 << 20) + 8), dict(c=(4 << 20) + 4),
+                dict(xs=68), dict(rs=65), dict(ros=66), dict(ns=70)):
+        assert norm_call(lib, **bad) == L_, bad
+    # overlaps: only the very rows of x or residual may be written
+    for bad in (dict(ro=4096 + 128), dict(n=(1 << 20) + 128), dict(n=2 << 20), dict(c=4096), dict(s=(4 << 20) + 8), dict(ro=4096, ros=72),
+                dict(r=1 << 20, rs=0, ro=1 << 20), dict(n=256 - 128), dict(c=(2 << 20) + 400)):
+        assert norm_call(lib, **bad) == A, bad
+    assert norm_call(lib, rows=0, x=None, r=None, w=None, ro=None, n=None, c=None, s=None) == 0
+
+
+def norm_inputs(m=4, h=64):
+    return torch.zeros((m, h), dtype=BF16), torch.zeros((m, h), dtype=BF16), torch.zeros(h, dtype=BF16)
+
+
+def test_norm_refuses_bad_tensors():
+    x, r, w = norm_inputs()
+    out = lambda **k: P.TailOutput(**{"residual": None, "codes": None, "scales": None, "normed": None, **k})  # noqa: E731
+    for args, kw in [((x.float(), r, w), {}), ((x[0], r, w), {}), ((x, r[:3], w), {}), ((x, r.float(), w), {}), ((x, r, w[:32]), {}),
+                     ((x, r, w.float()), {}), ((x, r, w[None]), {}), ((x[:, :48], r[:, :48], w[:48]), {}),
+                     ((x[:, ::2], r[:, ::2], w[:32]), {}), ((x[:1].expand(4, 64), r, w), {}),
+                     ((torch.zeros((4, 68), dtype=BF16)[:, :64], r, w), {}), ((x, r, w), dict(out=out())),
+                     ((x, None, w), dict(mxfp8=False)), ((x, None, w), dict(out=out(residual=torch.zeros_like(x)))),
+                     ((x, r, w), dict(out=out(codes=torch.zeros((4, 64), dtype=U8)))),
+                     ((x, r, w), dict(out=out(codes=torch.zeros((4, 64), dtype=U8), scales=torch.zeros((4, 3), dtype=U8)))),
+                     ((x, r, w), dict(out=out(codes=torch.zeros((4, 64), dtype=torch.int16), scales=torch.zeros((4, 2), dtype=U8)))),
+                     ((x, r, w), dict(out=out(normed=torch.zeros((4, 64))))),
+                     ((x, r.to("meta"), w), {}), ((x, r, w.to("meta")), {}), ((x, r, w), {})]:  # (the last: host tensors)
+        with pytest.raises(ValueError):
+            P.add_rmsnorm_mxfp8(*args, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ the product
+def weights(rows=64, k=96, gated=False, bias=False):
+    tiles = torch.zeros((1, 1, 16896), dtype=U8)
+    return P.LinearWeights(tiles, torch.zeros(rows) if bias else None, rows, k, gated)
+
+
+def linear_call(lib, rows=64, k=96, gated=0, tiles=256, bias=None, c=1 << 20, s=2 << 20, m=4, act=0, r=None, rs=64, o=3 << 20, os=64,
+                oc=None, osc=None, status=256):
+    w = _lib.LinearWeights(tiles, bias, rows, k, gated)
+    return lib.b200moe_linear(ctypes.byref(w), at(c), at(s), m, act, at(r), rs, at(o), os, at(oc), at(osc), at(status), None)
+
+
+@pytest.mark.parametrize("inter", [768, 1536])
+def test_c_abi_refuses_product_arguments(inter):
+    lib = _lib.load(inter)
+    A, L_ = _lib.E_ARG, _lib.E_ALIGN
+    for bad in (dict(c=None), dict(s=None), dict(o=None), dict(status=None), dict(tiles=None), dict(m=-1), dict(m=(1 << 24) + 1), dict(k=0),
+                dict(k=40), dict(k=(1 << 20) + 32), dict(rows=0), dict(rows=60), dict(rows=(1 << 20) + 8), dict(act=7), dict(act=-1), dict(act=5),
+                dict(gated=1), dict(gated=1, act=3), dict(rows=32, gated=1, act=5), dict(oc=4 << 20), dict(o=None, oc=4 << 20),
+                dict(oc=4 << 20, osc=5 << 20), dict(rows=40, o=None, oc=4 << 20, osc=5 << 20), dict(os=56), dict(r=4 << 20, rs=8),
+                dict(rows=1 << 20, k=1 << 20)):
+        assert linear_call(lib, **bad) == A, bad
+    for bad in (dict(tiles=272), dict(c=(1 << 20) + 8), dict(o=(3 << 20) + 8), dict(os=68), dict(r=(4 << 20) + 8), dict(r=4 << 20, rs=66),
+                dict(o=None, oc=(4 << 20) + 8, osc=5 << 20), dict(bias=258)):
+        assert linear_call(lib, **bad) == L_, bad
+    # overlaps: out may be the residual's rows and nothing else that is read
+    for bad in (dict(o=1 << 20), dict(o=(2 << 20) - 16), dict(r=3 << 20, rs=72), dict(r=(3 << 20) + 128), dict(r=3 << 20, rs=0),
+                dict(o=None, oc=1 << 20, osc=5 << 20), dict(o=None, oc=4 << 20, osc=(4 << 20) + 100), dict(o=None, oc=4 << 20, osc=2 << 20),
+                dict(o=None, oc=4 << 20, osc=5 << 20, r=4 << 20)):
+        assert linear_call(lib, **bad) == A, bad
+    assert linear_call(lib, m=0, c=None, s=None, o=None) == 0
+    for rows, k, gated, want in ((64, 96, 0, 16896), (136, 160, 0, 4 * 16896), (64, 32, 1, 16896), (192, 128, 1, 2 * 16896), (64, 40, 0, 0),
+                                 (60, 96, 0, 0), (96, 96, 1, 0), (1 << 20, 1 << 20, 0, 0)):
+        assert lib.b200moe_linear_weight_bytes(rows, k, gated) == want
+    assert lib.b200moe_preshuffle_linear(at(256), at(256), 64, 96, 0, None, None) == A
+    assert lib.b200moe_preshuffle_linear(at(256), at(256), 60, 96, 0, at(256), None) == A
+    assert lib.b200moe_preshuffle_linear(at(264), at(256), 64, 96, 0, at(256), None) == L_
+    assert lib.b200moe_preshuffle_linear(at(256), at(256), 64, 96, 0, at(272), None) == L_
+    quant = lambda x=256, st=96, m=4, k=96, c=4096, s=8192: lib.b200moe_quant_mxfp8(at(x), st, m, k, at(c), at(s), None)  # noqa: E731
+    assert all(quant(**bad) == A for bad in (dict(x=None), dict(c=None), dict(s=None), dict(m=-1), dict(k=40), dict(k=0), dict(st=88)))
+    assert all(quant(**bad) == L_ for bad in (dict(x=264), dict(st=100), dict(c=4100)))
+    assert quant(m=0, x=None) == 0
+
+
+def test_product_refuses_bad_tensors():
+    u8 = lambda *s: torch.zeros(s, dtype=U8)  # noqa: E731
+    bf = lambda *s: torch.zeros(s, dtype=BF16)  # noqa: E731
+    x = u8(4, 96), u8(4, 3)
+    w, g = weights(), weights(gated=True)
+    for args, kw in [((x, w), dict(activation="tanh")), ((x, w), dict(activation="swiglu")), ((x, g), {}), ((x, g), dict(activation="relu")),
+                     (((u8(4, 64), u8(4, 2)), w), {}), (((u8(4, 96), u8(4, 4)), w), {}), (((u8(4, 96), u8(3, 3)), w), {}),
+                     (((u8(4, 192)[:, ::2], u8(4, 3)), w), {}), (((bf(4, 96), u8(4, 3)), w), {}), (((u8(4, 96), None), w), {}),
+                     ((bf(4, 64), w), {}), ((bf(96), w), {}), ((torch.zeros((4, 96)), w), {}), (("x", w), {}),
+                     ((x, w), dict(residual=bf(4, 32))), ((x, w), dict(residual=bf(3, 64))), ((x, w), dict(residual=torch.zeros((4, 64)))),
+                     ((x, w), dict(residual=bf(4, 68)[:, :64])), ((x, w), dict(out=bf(4, 72))), ((x, w), dict(out=torch.zeros((4, 64)))),
+                     ((x, w), dict(out=bf(1, 64).expand(4, 64))), ((x, w), dict(out=(u8(4, 64), u8(4, 3)))), ((x, w), dict(out=(u8(4, 64), None))),
+                     ((x, w), dict(out=(None, None))), ((x, weights(rows=40)), dict(mxfp8_out=True)),
+                     ((x, w), dict(residual=bf(4, 64).to("meta"))), (((u8(4, 96).to("meta"), u8(4, 3).to("meta")), w), {}),
+                     ((x, w), {}), ((bf(4, 96), w), {})]:  # (the last two: host tensors)
+        with pytest.raises(ValueError):
+            P.mxfp8_linear(*args, **kw)
+    for bad in (bf(4, 40), bf(96), u8(4, 96), torch.zeros((4, 96)), bf(4, 200)[:, ::2], bf(4, 100)[:, :96]):
+        with pytest.raises(ValueError):
+            P.mxfp8_quant(bad)
+
+
+def test_weights_refuse_bad_tensors():
+    u8 = lambda *s: torch.zeros(s, dtype=U8)  # noqa: E731
+    for args in ((u8(64, 96), u8(64, 3)), (torch.zeros(64, 96), u8(64, 3)), (u8(64), u8(64, 3))):
+        with pytest.raises(ValueError):
+            P.LinearWeights.from_row_major(*args)  # host tensors, types, ranks
+
+
+def test_layout_and_struct():
+    w = weights(bias=True)
+    a = w.abi()
+    assert (a.tiles, a.bias, a.rows, a.k, a.gated) == (w.tiles.data_ptr(), w.bias.data_ptr(), 64, 96, 0) and w.abi() is a
+    w.bias = torch.ones(64)
+    assert w.abi().bias == w.bias.data_ptr()
+    assert weights(gated=True).n == 32 and L.MAX_DIM == 1 << 20
