@@ -1,7 +1,8 @@
 // The MXFP8 matrix product with bias, activation and residual in its epilogue: weight layout, row quantiser, entry point.
+#include <math.h>
+
 #include "linear.cuh"
 #include "tc_host.cuh"
-#include "tc_ptx.cuh"
 
 namespace b200moe {
 
@@ -56,90 +57,23 @@ __global__ void __launch_bounds__(256) quant_mxfp8_kernel(const uint4* x, int64_
   if ((c & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(e);
 }
 
-// ------------------------------------------------------------------------------------------------ product on CUDA cores
-// 16 tokens x one weight tile per CTA, fp32 FMAs on values decoded into shared memory; sums in rising K.
-__device__ __forceinline__ float e4m3_value(uint32_t c) {
-  const uint32_t m = c & 0x7fu;
-  float v = m < 8u ? static_cast<float>(m) * 0.001953125f : __uint_as_float((m << 20) + (120u << 23));
-  if (m == 0x7fu) v = __uint_as_float(0x7fc00000u);
-  return (c & 0x80u) ? -v : v;
-}
+// ------------------------------------------------------------------------------------------------ the call
+int linear_tc(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_tc.cu
+int set_wait_limit_linear_tc(unsigned long long ns);
 
-__global__ void __launch_bounds__(256) linear_simt_kernel(const LinearArgs args) {
-  pdl_launch_dependents();
-  pdl_wait();
-  LinearArgs a = args;
-  launder(a.tiles);
-  launder(a.codes);
-  launder(a.scales);
-  launder(a.residual);
-  extern __shared__ float sm[];
-  float* ws = sm;               // [128][129]
-  float* xs = sm + 128 * 129;   // [16][128], later the sums
-  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16;
-  const int tn = blockIdx.x, r = threadIdx.x & 127, half = threadIdx.x >> 7;
-  float acc[8] = {};
-  for (int kt = 0; kt < a.tiles_k; ++kt) {
-    const uint8_t* rec = a.tiles + (static_cast<int64_t>(tn) * a.tiles_k + kt) * kLinearRecordBytes;
-    for (int i = threadIdx.x; i < 128 * 128; i += 256) {
-      const int rr = i >> 7, c = i & 127;
-      const float s = e8m0_value(__ldcg(rec + kLinearCodeBytes + atom_offset(rr, c >> 5)));
-      ws[rr * 129 + c] = e4m3_value(__ldcg(rec + rr * 128 + (((c >> 4) ^ (rr & 7)) << 4) + (c & 15))) * s;
-    }
-    for (int i = threadIdx.x; i < 16 * 128; i += 256) {
-      const int64_t row = row0 + (i >> 7);
-      const int c = kt * 128 + (i & 127);
-      xs[i] = row < a.m && c < a.k ? e4m3_value(__ldcg(a.codes + row * a.k + c)) * e8m0_value(__ldcg(a.scales + row * (a.k / 32) + c / 32)) : 0.0f;
-    }
-    __syncthreads();
-    for (int c = 0; c < 128; ++c)
-#pragma unroll
-      for (int t = 0; t < 8; ++t) acc[t] = fmaf(ws[r * 129 + c], xs[(half * 8 + t) * 128 + c], acc[t]);
-    __syncthreads();
+static LinearAct act_args(int activation) {
+  LinearAct a = {kLinear, -INFINITY, 1.0f, 0.0f, INFINITY, 0.0f};
+  switch (activation) {
+    case B200MOE_ACT_RELU: a.floor = 0.0f; break;
+    case B200MOE_ACT_SILU: a.kind = kSigmoid; break;
+    case B200MOE_ACT_GELU: a.kind = kGelu; break;
+    case B200MOE_ACT_GELU_TANH:  // 2 sqrt(2 / pi) (p + 0.044715 p^3)
+      a.kind = kSigmoid, a.c1 = 1.5957691216f, a.c3 = 1.5957691216f * 0.044715f;
+      break;
+    case B200MOE_ACT_SWIGLU: a.kind = kGated; break;
+    case B200MOE_ACT_SWIGLU_OAI: a.kind = kGated, a.c1 = 1.702f, a.top = 7.0f, a.beta = 1.0f; break;
   }
-#pragma unroll
-  for (int t = 0; t < 8; ++t) xs[(half * 8 + t) * 128 + r] = acc[t];
-  __syncthreads();
-  const bool gated = linear_gated(a.act);
-  const int groups = gated ? 2 : 4;  // of 32 output columns
-  const int t = threadIdx.x / groups, g = threadIdx.x % groups;
-  const int64_t row = row0 + t;
-  const int col0 = tn * 32 * groups + 32 * g;
-  if (t >= 16 || row >= a.m || col0 >= a.n) return;
-  float y[32], amax = 0.0f;
-  for (int j = 0; j < 32; ++j) {
-    const int c = col0 + j;
-    if (gated) {
-      float p = xs[t * 128 + 64 * g + j], u = xs[t * 128 + 64 * g + 32 + j];
-      if (a.bias != nullptr) p += __ldcg(a.bias + c), u += __ldcg(a.bias + a.n + c);
-      y[j] = activate_gated(p, u, a.act);
-    } else {
-      float p = xs[t * 128 + 32 * g + j];
-      if (a.bias != nullptr && c < a.n) p += __ldcg(a.bias + c);
-      y[j] = activate(p, a.act);
-    }
-    if (a.residual != nullptr && c < a.n) y[j] += __bfloat162float(a.residual[row * a.residual_stride + c]);
-    amax = fmaxf(amax, fabsf(y[j]));
-  }
-  if (a.out != nullptr) {
-    for (int j = 0; j < 32 && col0 + j < a.n; ++j) a.out[row * a.out_stride + col0 + j] = __float2bfloat16_rn(y[j]);
-    return;
-  }
-  const int e = linear_scale(amax);
-  const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
-  for (int j = 0; j < 32; ++j) a.out_codes[row * a.n + col0 + j] = static_cast<uint8_t>(cvt_e4m3x2(y[j] * inv, 0.0f));
-  a.out_scales[row * (a.n / 32) + col0 / 32] = static_cast<uint8_t>(e);
-}
-
-static int launch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
-  constexpr int kSmem = (128 * 129 + 16 * 128) * 4;
-  static PerDeviceOnce once;
-  const int rc = once.run([] {
-    return static_cast<int>(cudaFuncSetAttribute(linear_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  });
-  if (rc) return rc;
-  B200MOE_LAUNCH(linear_simt_kernel, dim3(a.tiles_n, static_cast<unsigned>((a.m + 15) / 16)), 256, kSmem, stream, a);
-  return 0;
+  return a;
 }
 
 static int64_t linear_row_tiles(int64_t rows) { return (rows + 127) / 128; }  // gated: 64 output columns, 128 rows, as well
@@ -156,7 +90,7 @@ static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && pa < pb + nb && pb < pa + na;
 }
 
-int set_wait_limit_linear(unsigned long long ns) { return set_wait_limit_here(ns); }
+int set_wait_limit_linear(unsigned long long ns) { return set_wait_limit_linear_tc(ns); }
 
 }  // namespace b200moe
 
@@ -208,7 +142,7 @@ extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* co
   if (out_codes8 && n % 32) return B200MOE_E_ARG;
   if (m > 1 && ((out_bf16 && out_stride < n) || (residual_bf16 && residual_stride < n && residual_stride != 0))) return B200MOE_E_ARG;
   if (misaligned(w->tiles, 128) || misaligned(codes8, 16) || misaligned(out_bf16, 16) || misaligned(out_codes8, 16) ||
-      misaligned(residual_bf16, 16) || misaligned(w->bias, 4) || (m > 1 && ((out_bf16 && (out_stride & 7)) || (residual_bf16 && (residual_stride & 7)))))
+      misaligned(residual_bf16, 16) || misaligned(w->bias, 16) || (m > 1 && ((out_bf16 && (out_stride & 7)) || (residual_bf16 && (residual_stride & 7)))))
     return B200MOE_E_ALIGN;
   // the rows of out may be those of the residual (a thread stores where it has loaded); any other overlap with an input is refused
   const void* outs[3] = {out_bf16, out_codes8, out_scales8};
@@ -236,6 +170,6 @@ extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* co
   a.n = static_cast<int>(n);
   a.tiles_n = static_cast<int>(linear_row_tiles(w->rows));
   a.tiles_k = static_cast<int>(linear_k_tiles(w->k));
-  a.act = activation;
-  return launch_linear(a, status, static_cast<cudaStream_t>(stream));
+  a.act = act_args(activation);
+  return linear_tc(a, status, static_cast<cudaStream_t>(stream));
 }

@@ -1,6 +1,7 @@
-// The MXFP8 matrix product y = act(x @ w^T + bias) + residual: what its kernels share. Formats, epilogue arithmetic, arguments.
+// The MXFP8 matrix product y = act(x @ w^T + bias) + residual: what its kernels share. Formats, arguments, epilogue arithmetic.
 #pragma once
 #include "add_rmsnorm.cuh"
+#include "tc_ptx.cuh"
 
 namespace b200moe {
 
@@ -8,41 +9,67 @@ namespace b200moe {
 // shared-memory image, then one scale atom. Rows and columns beyond the matrix are zeros. Gated weights (gate rows, then up rows) are
 // interleaved in groups of 32, [gate 32 | up 32 | gate 32 | up 32], so that a tile holds 64 output columns with both halves.
 constexpr int kLinearCodeBytes = 128 * 128;
-constexpr int kLinearRecordBytes = kLinearCodeBytes + kAtomBytes;  // 132 rows of 128 bytes
+constexpr int kLinearRecordBytes = kLinearCodeBytes + kAtomBytes;
+constexpr int kLinearRecordRows = kLinearRecordBytes / 128;  // 132: the tiles seen as rows of 128 bytes
+
+// What the epilogue does with a sum p (or a gate g and an up u):
+//   kLinear   p, or 0 where p < floor (ReLU: 0, none: -inf)
+//   kSigmoid  p * sigmoid(c1 p + c3 p^3): SiLU, and GELU in its tanh form, 0.5 (1 + tanh(v)) = sigmoid(2 v)
+//   kGelu     p * Phi(p)
+//   kGated    min(g, top) * sigmoid(c1 min(g, top)) * (clamp(u, -top, top) + beta)
+enum LinearKind { kLinear = 0, kSigmoid = 1, kGelu = 2, kGated = 3 };
+struct LinearAct {
+  int kind;
+  float floor, c1, c3, top, beta;
+};
 
 struct LinearArgs {
   const uint8_t* tiles;
-  const float* bias;         // [weight rows] or null
-  const uint8_t* codes;      // [m][k]
-  const uint8_t* scales;     // [m][k / 32]
+  const float* bias;              // [weight rows] or null
+  const uint8_t* codes;           // [m][k]
+  const uint8_t* scales;          // [m][k / 32]
   const __nv_bfloat16* residual;  // rows residual_stride apart, or null
-  __nv_bfloat16* out;        // rows out_stride apart; or, for MXFP8 output, null:
-  uint8_t* out_codes;        // [m][n]
-  uint8_t* out_scales;       // [m][n / 32]
+  __nv_bfloat16* out;             // rows out_stride apart; or null:
+  uint8_t* out_codes;             // [m][n]
+  uint8_t* out_scales;            // [m][n / 32]
   int64_t m, residual_stride, out_stride;
-  int k, n;                  // n: output columns
+  int k, n;  // n: output columns
   int tiles_n, tiles_k;
-  int act;
+  LinearAct act;
 };
 
-__device__ __forceinline__ bool linear_gated(int act) { return act >= B200MOE_ACT_SWIGLU; }
-
-// p is multiplied by the logistic function of c * p
-__device__ __forceinline__ float times_sigmoid(float p, float c) { return __fdividef(p, 1.0f + __expf(-c * p)); }
-
-__device__ __forceinline__ float activate(float p, int act) {
-  switch (act) {
-    case B200MOE_ACT_RELU: return p < 0.0f ? 0.0f : p;  // (NaN stays)
-    case B200MOE_ACT_SILU: return times_sigmoid(p, 1.0f);
-    case B200MOE_ACT_GELU: return p * normcdff(p);
-    case B200MOE_ACT_GELU_TANH:  // 0.5 p (1 + tanh(u)) = p / (1 + exp(-2 u)), u = sqrt(2 / pi) (p + 0.044715 p^3)
-      return __fdividef(p, 1.0f + __expf(-1.5957691216f * (p + 0.044715f * p * p * p)));
-  }
-  return p;
+// NaN passes every clamp here (the comparison is false), as it does in the formulas
+__device__ __forceinline__ float act_linear(float p, const LinearAct& a) { return p < a.floor ? 0.0f : p; }
+__device__ __forceinline__ float act_sigmoid(float p, const LinearAct& a) {
+  const float v = p * fmaf(a.c3, fminf(p * p, 1e30f), a.c1);  // (bounded: 0 * inf is NaN)
+  return __fdividef(p, 1.0f + __expf(-v));
 }
-
-__device__ __forceinline__ float activate_gated(float g, float u, int act) {
-  return act == B200MOE_ACT_SWIGLU ? times_sigmoid(g, 1.0f) * u : swiglu_oai(g, u);
+// Phi(p) = erfc(-p / sqrt(2)) / 2. erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0: the Chebyshev fit of Numerical Recipes
+// (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision; a third of the
+// instructions of normcdff.
+__device__ __forceinline__ float act_gelu(float p) {
+  const float z = fabsf(p) * 0.70710678f, t = __fdividef(1.0f, fmaf(0.5f, z, 1.0f));
+  float q = 0.17087277f;
+  q = fmaf(q, t, -0.82215223f);
+  q = fmaf(q, t, 1.48851587f);
+  q = fmaf(q, t, -1.13520398f);
+  q = fmaf(q, t, 0.27886807f);
+  q = fmaf(q, t, -0.18628806f);
+  q = fmaf(q, t, 0.09678418f);
+  q = fmaf(q, t, 0.37409196f);
+  q = fmaf(q, t, 1.00002368f);
+  q = fmaf(q, t, -1.26551223f);
+  const float half = 0.5f * t * __expf(fmaf(-z, z, q));  // erfc(z) / 2
+  return p * (p < 0.0f ? half : 1.0f - half);
+}
+__device__ __forceinline__ float act_gated(float g, float u, const LinearAct& a) {
+  g = g > a.top ? a.top : g;
+  u = u > a.top ? a.top : u < -a.top ? -a.top : u;
+  return g * __fdividef(1.0f, 1.0f + __expf(-a.c1 * g)) * (u + a.beta);
+}
+template <int KIND>
+__device__ __forceinline__ float act_of(float p, const LinearAct& a) {
+  return KIND == kLinear ? act_linear(p, a) : KIND == kSigmoid ? act_sigmoid(p, a) : act_gelu(p);
 }
 
 // E8M0 byte of an MXFP8 block, the shared expert's rule (ceil_pow2(amax / 448), at least 1); an infinite block keeps a finite scale
@@ -50,9 +77,26 @@ __device__ __forceinline__ int linear_scale(float amax) {
   const int e = mxfp8_scale(amax);
   return e > 254 ? 254 : e;
 }
-
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
   return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
 }
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// The four scale bytes of K-tile kt of row `row` (0 beyond the rows or the columns). `words`: rows of scales begin at multiples of 4 bytes.
+__device__ __forceinline__ uint32_t row_scales(const uint8_t* scales, int64_t row, int64_t rows, int kt, int per_row, bool words) {
+  if (row >= rows) return 0u;
+  const uint8_t* p = scales + row * per_row + kt * 4;
+  if (words) return __ldcg(reinterpret_cast<const uint32_t*>(p));
+  uint32_t v = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (kt * 4 + j < per_row) v |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * j);
+  return v;
+}
+
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 }  // namespace b200moe

@@ -59,6 +59,8 @@ class LinearWeights:
             if bias.shape != (rows,) or not bias.is_floating_point():
                 raise ValueError(f"bias: needs [{rows}] of a floating type")
             bias = bias.detach().float().contiguous()
+            if bias.data_ptr() & 15:
+                bias = bias.clone()
         codes, scales = w.contiguous().view(torch.uint8), scale.contiguous().view(torch.uint8)
         if codes.data_ptr() & 15:
             codes = codes.clone()

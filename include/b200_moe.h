@@ -456,7 +456,7 @@ int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t rows, int6
 
 typedef struct b200moe_linear_weights {
   const uint8_t* tiles; /* b200moe_preshuffle_linear */
-  const float* bias;    /* fp32 [rows], in the order of the checkpoint's rows, or null */
+  const float* bias;    /* fp32 [rows], in the order of the checkpoint's rows, 16-byte aligned, or null */
   int64_t rows, k;
   int gated;
 } b200moe_linear_weights;

@@ -87,7 +87,7 @@ def test_c_abi_refuses_product_arguments(inter):
                 dict(rows=1 << 20, k=1 << 20)):
         assert linear_call(lib, **bad) == A, bad
     for bad in (dict(tiles=272), dict(c=(1 << 20) + 8), dict(o=(3 << 20) + 8), dict(os=68), dict(r=(4 << 20) + 8), dict(r=4 << 20, rs=66),
-                dict(o=None, oc=(4 << 20) + 8, osc=5 << 20), dict(bias=258)):
+                dict(o=None, oc=(4 << 20) + 8, osc=5 << 20), dict(bias=264)):
         assert linear_call(lib, **bad) == L_, bad
     # overlaps: out may be the residual's rows and nothing else that is read
     for bad in (dict(o=1 << 20), dict(o=(2 << 20) - 16), dict(r=3 << 20, rs=72), dict(r=(3 << 20) + 128), dict(r=3 << 20, rs=0),
