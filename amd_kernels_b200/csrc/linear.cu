@@ -58,8 +58,10 @@ __global__ void __launch_bounds__(256) quant_mxfp8_kernel(const uint4* x, int64_
 }
 
 // ------------------------------------------------------------------------------------------------ the call
-int linear_tc(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_tc.cu
+int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream);  // linear_tc.cu
+int linear_pair(const LinearArgs& a, int nt, int32_t* status, cudaStream_t stream);            // linear_pair.cu
 int set_wait_limit_linear_tc(unsigned long long ns);
+int set_wait_limit_linear_pair(unsigned long long ns);
 
 static LinearAct act_args(int activation) {
   LinearAct a = {kLinear, -INFINITY, 1.0f, 0.0f, INFINITY, 0.0f};
@@ -90,7 +92,20 @@ static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && pa < pb + nb && pb < pa + na;
 }
 
-int set_wait_limit_linear(unsigned long long ns) { return set_wait_limit_linear_tc(ns); }
+int set_wait_limit_linear(unsigned long long ns) {
+  const int r = set_wait_limit_linear_tc(ns);
+  return r ? r : set_wait_limit_linear_pair(ns);
+}
+
+// The kernel, its token block and its split of K for these sizes.
+static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+  if (a.m > 256) return linear_pair(a, 2, status, stream);
+  const int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : a.m <= 128 ? 128 : 256;
+  const int64_t units = (a.m + bm - 1) / bm * a.tiles_n;
+  int splits = 1;
+  while (splits < 8 && splits < a.tiles_k && units * (splits + 1) <= sm_count()) ++splits;
+  return linear_tc(a, bm, splits, status, stream);
+}
 
 }  // namespace b200moe
 
@@ -127,17 +142,18 @@ extern "C" int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t
   return 0;
 }
 
-extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
-                              int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
-                              uint8_t* out_codes8, uint8_t* out_scales8, int32_t* status, void* stream) {
-  using namespace b200moe;
+namespace b200moe {
+// Checks a call and fills the kernels' arguments; a.m is 0 where there is nothing to do.
+static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
+                       int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
+                       uint8_t* out_codes8, uint8_t* out_scales8, const int32_t* status) {
+  a.m = 0;
   if (!w || m < 0 || m > B200MOE_LINEAR_MAX_ROWS) return B200MOE_E_ARG;
   if (!linear_dims(w->rows, w->k, w->gated) || activation < B200MOE_ACT_NONE || activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
   if ((w->gated != 0) != (activation >= B200MOE_ACT_SWIGLU)) return B200MOE_E_ARG;
   if (m == 0) return 0;
   if (!w->tiles || !codes8 || !scales8 || !status) return B200MOE_E_ARG;
   if ((out_bf16 != nullptr) == (out_codes8 != nullptr) || (out_codes8 != nullptr) != (out_scales8 != nullptr)) return B200MOE_E_ARG;
-  LinearArgs a;
   const int64_t n = w->gated ? w->rows / 2 : w->rows;
   if (out_codes8 && n % 32) return B200MOE_E_ARG;
   if (m > 1 && ((out_bf16 && out_stride < n) || (residual_bf16 && residual_stride < n && residual_stride != 0))) return B200MOE_E_ARG;
@@ -171,5 +187,16 @@ extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* co
   a.tiles_n = static_cast<int>(linear_row_tiles(w->rows));
   a.tiles_k = static_cast<int>(linear_k_tiles(w->k));
   a.act = act_args(activation);
-  return linear_tc(a, status, static_cast<cudaStream_t>(stream));
+  return 0;
+}
+}  // namespace b200moe
+
+extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
+                              int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
+                              uint8_t* out_codes8, uint8_t* out_scales8, int32_t* status, void* stream) {
+  using namespace b200moe;
+  LinearArgs a;
+  const int r = linear_args(a, w, codes8, scales8, m, activation, residual_bf16, residual_stride, out_bf16, out_stride, out_codes8,
+                            out_scales8, status);
+  return r || a.m == 0 ? r : dispatch_linear(a, status, static_cast<cudaStream_t>(stream));
 }

@@ -97,6 +97,13 @@ __device__ __forceinline__ uint32_t row_scales(const uint8_t* scales, int64_t ro
   return v;
 }
 
+// 32 bytes, one sector, by one thread (32-byte aligned)
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 }  // namespace b200moe

@@ -1,0 +1,465 @@
+// The MXFP8 product for many rows, on CTA pairs: tcgen05.mma.cta_group::2 kind::mxf8f6f4 with M = 256 token rows (two blocks of 128) x
+// N = 256 or 128 weight rows (NT = two tiles or one) x K = 32 per instruction, each CTA staging its own 128 token rows and half of the
+// weight rows. No multicast.
+//
+// Unit = (pair of token blocks) x (NT weight tiles). Two rings: 6 stages of codes, and 8 slots of scales that travel ahead of them, so
+// that the MMA warp waits for codes only. The token scales come row-major, as every producer of this package writes them: the scale
+// warp turns them into atoms on the way, so no launch in front of the product re-lays them.
+//
+//   warp 0      code producer (both CTAs): TMA of the CTA's 128 token rows and of its weight rows, counted on the leader's barrier
+//   warp 1      tensor memory (both CTAs); in the leader it issues the MMAs for both, the whole warp around one elected lane
+//   warp 2      leader: copies the scales into tensor memory in both CTAs, in the same way
+//   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
+//   warps 4-11  epilogue (both CTAs): thread = one token row, 64 * NT columns. The sums are pulled into registers and the accumulator
+//               is handed back; then bias, activation, residual and one rounding, 32 columns at a time, stored as 32-byte sectors
+// 12 warps start with 168 registers; the issuing warpgroup drops to 72, the epilogue's rise to 216 (4 x 72 + 8 x 216 = 12 x 168: the
+// exchange must balance inside what the CTA was given at launch).
+#include "linear.cuh"
+#include "tc_pair.cuh"
+
+namespace b200moe {
+
+template <int NT>
+struct LinearPairCfg {
+  static constexpr int kStages = 6;                     // code ring
+  static constexpr int kSfStages = 8;                   // scale ring = scale sets in tensor memory
+  static constexpr int kWRows = 64 * NT;                // weight rows of one CTA
+  static constexpr int kWOff = 128 * 128;               // behind the CTA's 128 token rows
+  static constexpr int kStageBytes = kWOff + kWRows * 128;
+  static constexpr int kSfOff = kStages * kStageBytes;
+  static constexpr int kSfSlotBytes = (1 + NT) * kAtomBytes;  // token atom, weight atoms
+  static constexpr int kBiasOff = kSfOff + kSfStages * kSfSlotBytes;
+  static constexpr int kCols = 64 * NT;                 // accumulator columns of an epilogue thread
+  static constexpr int kSmemBytes = kBiasOff + 8 * kCols * 4 + 1024;
+  static constexpr int kThreads = 32 * 12;
+  static constexpr int kAccs = NT == 1 ? 2 : 1;         // accumulators of 128 * NT columns
+  static constexpr int kSfCol = 256;                    // tensor memory: accumulators, then 8 sets of 16 columns
+  static constexpr int kTmemCols = 512;
+  static_assert(kSmemBytes <= 227 * 1024 && kSfStages >= kStages, "a scale set is free once the code stage is");
+};
+
+__device__ __forceinline__ void tc_mma_mxf8_two(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .b64 da, db;\n.reg .pred p;\nmov.b64 da, {%1, %7};\nmov.b64 db, {%2, %7};\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kOperandDescHi)
+      : "memory");
+}
+
+// Arrival on a barrier of another CTA of the cluster that orders this thread's (and, behind a __syncwarp, its warp's) shared-memory
+// writes before it, and the wait that sees them.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+  if (!mbar_wait(bar, parity, abort_flag, status)) return false;
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return true;
+}
+
+// The units in groups of 8 pairs of token blocks: a group sweeps the weights once, tile by tile, so that its tokens (2048 rows) and the
+// few tiles in work stay in L2 whatever the size of the weights.
+struct LinearUnits {
+  int pairs, steps_n;  // pairs of token blocks, units along N
+  __device__ __forceinline__ int total() const { return pairs * steps_n; }
+  __device__ __forceinline__ void at(int u, int& pair, int& step) const {
+    const int group = u / (8 * steps_n), first = group * 8, rest = u - group * 8 * steps_n;
+    const int rows = pairs - first < 8 ? pairs - first : 8;
+    step = rest / rows;
+    pair = first + rest % rows;
+  }
+};
+
+template <int KIND, bool MX, int NT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::kThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_wc,
+                       const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ LinearArgs args, int32_t* status) {
+  using C = LinearPairCfg<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[C::kStages];     // leader: both CTAs' codes of the stage have landed
+  __shared__ __align__(8) uint64_t bar_empty[C::kStages];    // in each CTA: the MMAs that read the stage have completed
+  __shared__ __align__(8) uint64_t bar_sfull[C::kSfStages];  // leader: both CTAs' scales of the slot are there
+  __shared__ __align__(8) uint64_t bar_sf[C::kSfStages];     // in each CTA: they have been copied to tensor memory
+  __shared__ __align__(8) uint64_t bar_tfull[C::kAccs];      // in each CTA: the unit's accumulator is complete
+  __shared__ __align__(8) uint64_t bar_tempty[C::kAccs];     // leader: both CTAs' epilogues have read it
+  __shared__ __align__(8) uint64_t bar_drain[2];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const tiles_ptr = smem_raw + (tiles - smem_u32(smem_raw));
+  const uint32_t sf_ring = tiles + C::kSfOff;
+  volatile int* abort_v = &abort_flag;
+  pdl_launch_dependents();
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+    }
+    for (int j = 0; j < C::kSfStages; ++j) {
+      mbar_init(smem_u32(&bar_sfull[j]), 3);  // the leader's byte count, the token scales of both CTAs
+      mbar_init(smem_u32(&bar_sf[j]), 1);
+    }
+    for (int i = 0; i < C::kAccs; ++i) {
+      mbar_init(smem_u32(&bar_tfull[i]), 1);
+      mbar_init(smem_u32(&bar_tempty[i]), 16);  // one arrival per epilogue warp of both CTAs
+    }
+    mbar_init(smem_u32(&bar_drain[0]), 1);
+    mbar_init(smem_u32(&bar_drain[1]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
+                 "r"(static_cast<uint32_t>(C::kTmemCols))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before anything signals across the pair
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_slot;
+  pdl_wait();
+  LinearArgs a = args;
+  launder(a.scales);
+  launder(a.bias);
+  launder(a.residual);
+
+  const int n_clusters = static_cast<int>(gridDim.x >> 1), cluster = static_cast<int>(blockIdx.x >> 1);
+  const LinearUnits units = {static_cast<int>((a.m + 255) / 256), (a.tiles_n + NT - 1) / NT};
+  const int total = units.total(), tiles_k = a.tiles_k;
+  int pair, step;
+
+  // The issuing warpgroup and the two epilogue warpgroups do not meet again before the kernel's last lines.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ---------------------------------------------------------------- code producer (both CTAs)
+      if (lane == 0) {
+        const uint32_t full0 = map_to_cta(smem_u32(&bar_full[0]), 0);  // the leader's barriers, as seen from this CTA
+        uint32_t it = 0, s = 0, ph = 1u;
+        bool ok = true;
+        for (int u = cluster; u < total && ok; u += n_clusters) {
+          units.at(u, pair, step);
+          const int row = pair * 256 + static_cast<int>(rank) * 128;
+          // NT = 2: the whole tile 2 step + rank; NT = 1: half of tile `step`
+          int rec = NT == 2 ? (2 * step + static_cast<int>(rank)) * tiles_k * kLinearRecordRows
+                            : step * tiles_k * kLinearRecordRows + static_cast<int>(rank) * 64;
+          for (int kt = 0; kt < tiles_k; ++kt, ++it, rec += kLinearRecordRows) {
+            if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
+            const uint32_t full = full0 + 8u * s, base = tiles + s * C::kStageBytes;
+            if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), 2 * C::kStageBytes);
+            // rows beyond the last token or the last weight tile are read as zeros and count all the same
+            tma_load_2d_pair(base, &map_x, kt * 128, row, full);
+            tma_load_2d_pair(base + C::kWOff, &map_wc, 0, rec, full);
+            if (++s == C::kStages) { s = 0; ph ^= 1u; }
+          }
+        }
+        if (!ok && leader) drain_copies(bar_full, it, C::kStages);
+      }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- scales (both CTAs): lane l writes 16 bytes of the token atom, rows
+      // l, l + 32, l + 64 and l + 96, four K-tiles of loads ahead
+      const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
+      const int per_row = a.k / 32;
+      const bool words = (per_row & 3) == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 3) == 0;
+      uint32_t now[4][4], next[4][4];
+      uint32_t it = 0, j = 0, ph = 1u;
+      bool ok = true;
+      for (int u = cluster; u < total && ok; u += n_clusters) {
+        units.at(u, pair, step);
+        const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + lane;
+        const auto fetch = [&](int kt, uint32_t (&v)[4][4]) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[d][i] = kt + d < tiles_k ? row_scales(a.scales, row + 32 * i, a.m, kt + d, per_row, words) : 0u;
+        };
+        fetch(0, now);
+        int rec = NT * step * tiles_k * kLinearRecordRows + 128;
+        for (int kt0 = 0; kt0 < tiles_k && ok; kt0 += 4) {
+          fetch(kt0 + 4, next);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            if (kt0 + d >= tiles_k || !ok) break;
+            // free once its previous contents are in tensor memory
+            if (!warp_wait(smem_u32(&bar_sf[j]), ph, abort_v, status)) { ok = false; break; }
+            const uint32_t sfull = sfull0 + 8u * j, slot = sf_ring + j * C::kSfSlotBytes;
+            if (lane == 0) {
+              if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[j]), 2 * NT * kAtomBytes);
+              tma_load_2d_pair(slot + kAtomBytes, &map_ws, 0, rec, sfull);
+              if (NT == 2) tma_load_2d_pair(slot + 2 * kAtomBytes, &map_ws, 0, rec + tiles_k * kLinearRecordRows, sfull);
+            }
+            *(reinterpret_cast<uint4*>(tiles_ptr + C::kSfOff + j * C::kSfSlotBytes) + lane) = make_uint4(now[d][0], now[d][1], now[d][2], now[d][3]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_release_cluster(sfull);
+            rec += kLinearRecordRows;
+            ++it;
+            if (++j == C::kSfStages) { j = 0; ph ^= 1u; }
+          }
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[d][i] = next[d][i];
+        }
+      }
+      if (!ok && leader && lane == 0) drain_copies(bar_sfull, it, C::kSfStages);
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issue (leader only)
+      if (leader) {
+        // E4M3 x E4M3, UE8M0 scales, M = 256, N = 128 NT; scale byte k of a row's cell for MMA k
+        constexpr uint32_t kIdesc = (static_cast<uint32_t>(128 * NT >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24);
+        uint32_t ui = 0, s = 0, ph = 0, j = 0, sph = 0;
+        bool ok = true, sf_ready = false, full_ready = false;
+        for (int u = cluster; u < total && ok; u += n_clusters, ++ui) {
+          const uint32_t acc = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
+          if (!warp_wait(smem_u32(&bar_tempty[acc]), aph ^ 1u, abort_v, status)) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + acc * 128 * NT;
+          for (int kt = 0; kt < tiles_k; ++kt) {
+            if (!__all_sync(0xffffffffu, (sf_ready || mbar_wait(smem_u32(&bar_sf[j]), sph, abort_v, status)) &&
+                                             (full_ready || mbar_wait(smem_u32(&bar_full[s]), ph, abort_v, status)))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t s_now = s, j_now = j;
+            if (++s == C::kStages) { s = 0; ph ^= 1u; }
+            if (++j == C::kSfStages) { j = 0; sph ^= 1u; }
+            sf_ready = mbar_test(smem_u32(&bar_sf[j]), sph);
+            full_ready = mbar_test(smem_u32(&bar_full[s]), ph);
+            const uint32_t x_lo = (tiles + s_now * C::kStageBytes) >> 4, w_lo = x_lo + (C::kWOff >> 4);
+            const uint32_t t_sft = tmem_base + C::kSfCol + 16u * j_now, t_sfw = t_sft + 8u;
+            if (elect_one()) {
+              tc_mma_mxf8_two(d_tmem, x_lo, w_lo, kIdesc, t_sft, t_sfw, static_cast<uint32_t>(kt != 0));
+              tc_mma_mxf8_two(d_tmem, x_lo + 2, w_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sft, t_sfw, 1u);
+              tc_mma_mxf8_two(d_tmem, x_lo + 4, w_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sft, t_sfw, 1u);
+              tc_mma_mxf8_two(d_tmem, x_lo + 6, w_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sft, t_sfw, 1u);
+              tc_commit_both(smem_u32(&bar_empty[s_now]));  // the stage is free again, in both CTAs
+            }
+            __syncwarp();
+          }
+          if (ok && elect_one()) tc_commit_both(smem_u32(&bar_tfull[acc]));
+        }
+        if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05_pair(smem_u32(&bar_drain[0]));
+      }
+    } else {
+      // ---------------------------------------------------------------- scale copies into both CTAs' tensor memory (leader)
+      if (leader) {
+        uint32_t s = 0, ph = 1u, j = 0, sph = 0;
+        bool ok = true;
+        for (int u = cluster; u < total && ok; u += n_clusters) {
+          for (int kt = 0; kt < tiles_k; ++kt) {
+            // set j was last read by the MMAs 8 K-tiles back: complete once those that read stage s, kStages back, are
+            if (!__all_sync(0xffffffffu, mbar_wait_acquire_cluster(smem_u32(&bar_sfull[j]), sph, abort_v, status) &&
+                                             mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t lo = (sf_ring + j * C::kSfSlotBytes) >> 4, sf_bar = smem_u32(&bar_sf[j]);
+            const uint32_t t_sft = tmem_base + C::kSfCol + 16u * j, t_sfw = t_sft + 8u;
+            if (++s == C::kStages) { s = 0; ph ^= 1u; }
+            if (++j == C::kSfStages) { j = 0; sph ^= 1u; }
+            if (elect_one()) {
+              tc_cp_scales_pair(t_sft, lo);                         // each CTA its own token rows
+              tc_cp_scales_pair(t_sfw, lo + (kAtomBytes >> 4));     // weight rows 0..127 of N
+              if (NT == 2) tc_cp_scales_pair(t_sfw + 4, lo + (2 * kAtomBytes >> 4));  // 128..255
+              tc_commit_both(sf_bar);
+            }
+            __syncwarp();
+          }
+        }
+        if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05_pair(smem_u32(&bar_drain[1]));
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (both CTAs, warps 4..11)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    constexpr int kParts = C::kCols / 32;                       // accumulator pieces of 32 columns
+    constexpr int kOuts = KIND == kGated ? kParts / 2 : kParts; // pieces of 32 output columns
+    const int q = warp & 3;                  // the TMEM lane quarter this warp may read
+    const int half = (warp >> 2) - 1;        // which half of the unit's columns
+    const uint32_t tempty_leader = map_to_cta(smem_u32(&bar_tempty[0]), 0);
+    float* const bias = reinterpret_cast<float*>(tiles_ptr + C::kBiasOff) + (warp - 4) * C::kCols;
+    const bool wide = !MX ? (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (a.out_stride & 15) == 0
+                          : (reinterpret_cast<uintptr_t>(a.out_codes) & 31) == 0;
+    uint32_t ui = 0;
+    for (int u = cluster; u < total; u += n_clusters, ++ui) {
+      units.at(u, pair, step);
+      const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + q * 32 + lane;
+      const bool in_row = row < a.m;
+      const int col_tile = NT == 2 ? 2 * step + half : step;
+      const int col0 = KIND == kGated ? col_tile * 64 + (NT == 1 ? 32 * half : 0) : col_tile * 128 + (NT == 1 ? 64 * half : 0);
+      // the bias in the order of the accumulator's columns; the residual's first columns
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const int col = col0 + 32 * (KIND == kGated ? i >> 1 : i) + lane;
+        const int64_t from = KIND == kGated && (i & 1) ? static_cast<int64_t>(a.n) + col : col;
+        bias[32 * i + lane] = a.bias != nullptr && col < a.n ? __ldcg(a.bias + from) : 0.0f;
+      }
+      __syncwarp();
+      uint4 res[2][4];
+      const auto load_residual = [&](int i, uint4 (&r)[4]) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int col = col0 + 32 * i + 8 * p;
+          r[p] = in_row && col < a.n ? __ldcg(reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col)) : uint4{};
+        }
+      };
+      if (a.residual != nullptr) load_residual(0, res[0]);
+      const uint32_t acc_i = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
+      // the warp decides together: tcgen05.ld below needs all 32 lanes
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull[acc_i]), aph, abort_v, status))) break;
+      tc_fence_after();
+      const uint32_t t_acc = tmem_base + acc_i * 128 * NT + C::kCols * half + (static_cast<uint32_t>(q * 32) << 16);
+      uint32_t acc[kParts][32];
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) tc_ld32_nowait(t_acc + 32 * i, acc[i]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * acc_i);
+#pragma unroll
+      for (int i = 0; i < kOuts; ++i) {
+        const int col = col0 + 32 * i;
+        if (a.residual != nullptr && i + 1 < kOuts) load_residual(i + 1, res[(i + 1) & 1]);
+        float y[32];
+#pragma unroll
+        for (int k4 = 0; k4 < 8; ++k4) {
+          const int part = KIND == kGated ? 2 * i : i;
+          const float4 b = *reinterpret_cast<const float4*>(bias + 32 * part + 4 * k4);
+          const float bb[4] = {b.x, b.y, b.z, b.w};
+          if (KIND == kGated) {
+            const float4 bu = *reinterpret_cast<const float4*>(bias + 32 * (part + (KIND == kGated)) + 4 * k4);
+            const float bbu[4] = {bu.x, bu.y, bu.z, bu.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              y[4 * k4 + k] = act_gated(__uint_as_float(acc[part][4 * k4 + k]) + bb[k],
+                                        __uint_as_float(acc[part + (KIND == kGated)][4 * k4 + k]) + bbu[k], a.act);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[4 * k4 + k] = act_of<KIND>(__uint_as_float(acc[part][4 * k4 + k]) + bb[k], a.act);
+          }
+        }
+        if (a.residual != nullptr) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint4 r = res[i & 1][p];
+            const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              y[8 * p + 2 * k] += __uint_as_float(rr[k] << 16);
+              y[8 * p + 2 * k + 1] += __uint_as_float(rr[k] & 0xffff0000u);
+            }
+          }
+        }
+        if (MX) {
+          float amax = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) amax = fmaxf(amax, fabsf(y[k]));
+          const int e = linear_scale(amax);
+          const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = pack_e4m3x4(y[4 * k] * inv, y[4 * k + 1] * inv, y[4 * k + 2] * inv, y[4 * k + 3] * inv);
+          if (in_row && col < a.n) {  // (n is a multiple of 32 here)
+            uint8_t* o = a.out_codes + row * a.n + col;
+            if (wide) {
+              st_sector(o, w);
+            } else {
+              reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            a.out_scales[row * (a.n / 32) + col / 32] = static_cast<uint8_t>(e);
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(y[16 * p + 2 * k], y[16 * p + 2 * k + 1]);
+            const int c = col + 16 * p;
+            if (in_row && c < a.n) {
+              __nv_bfloat16* o = a.out + row * a.out_stride + c;
+              if (wide && c + 8 < a.n) {
+                st_sector(o, w);
+              } else {
+                reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (c + 8 < a.n) reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();  // all lanes have read this unit's bias
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA frees tensor memory or leaves while the partner may still signal or read it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(static_cast<uint32_t>(C::kTmemCols))
+                 : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+template <int KIND, bool MX, int NT>
+static int linear_pairs() {
+  static std::mutex mu;
+  static int pairs[kMaxDevices] = {};
+  static bool known[kMaxDevices] = {};
+  return resident_pairs_of(linear_pair_kernel<KIND, MX, NT>, LinearPairCfg<NT>::kThreads, LinearPairCfg<NT>::kSmemBytes, mu, known, pairs);
+}
+
+template <int KIND, bool MX, int NT>
+static int launch_linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+  using C = LinearPairCfg<NT>;
+  CUtensorMap mx, mwc, mws;
+  const uint64_t w_rows = static_cast<uint64_t>(a.tiles_n) * a.tiles_k * kLinearRecordRows;
+  int r;
+  if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), 128))) return r;
+  if ((r = make_flat_map(&mwc, a.tiles, w_rows, C::kWRows))) return r;
+  if ((r = make_flat_map(&mws, a.tiles, w_rows, 4))) return r;
+  const int64_t units = (a.m + 255) / 256 * ((a.tiles_n + NT - 1) / NT);
+  if (units > 0x7fffffff) return B200MOE_E_ARG;
+  const int pairs = linear_pairs<KIND, MX, NT>();
+  if (pairs <= 0) return B200MOE_E_DRIVER;
+  return launch_pairs(linear_pair_kernel<KIND, MX, NT>, units < pairs ? static_cast<int>(units) : pairs, C::kThreads, C::kSmemBytes, stream,
+                      mx, mwc, mws, a, status);
+}
+
+template <int KIND, int NT>
+static int linear_pair_out(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+  return a.out ? launch_linear_pair<KIND, false, NT>(a, status, stream) : launch_linear_pair<KIND, true, NT>(a, status, stream);
+}
+
+template <int NT>
+static int linear_pair_kind(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+  switch (a.act.kind) {
+    case kLinear: return linear_pair_out<kLinear, NT>(a, status, stream);
+    case kSigmoid: return linear_pair_out<kSigmoid, NT>(a, status, stream);
+    case kGelu: return linear_pair_out<kGelu, NT>(a, status, stream);
+  }
+  return linear_pair_out<kGated, NT>(a, status, stream);
+}
+
+int linear_pair(const LinearArgs& a, int nt, int32_t* status, cudaStream_t stream) {
+  return nt == 2 ? linear_pair_kind<2>(a, status, stream) : linear_pair_kind<1>(a, status, stream);
+}
+
+int set_wait_limit_linear_pair(unsigned long long ns) { return set_wait_limit_here(ns); }
+
+}  // namespace b200moe

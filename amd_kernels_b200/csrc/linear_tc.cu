@@ -333,12 +333,8 @@ static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cu
   return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM>, mx, a, splits, static_cast<int>(n_blocks), status));
 }
 
-// Token block and split of K for `m` rows.
-int linear_tc(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
-  const int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : a.m <= 128 ? 128 : 256;
-  const int64_t units = (a.m + bm - 1) / bm * a.tiles_n;
-  int splits = 1;
-  while (splits < 8 && splits < a.tiles_k && units * (splits + 1) <= sm_count()) ++splits;
+// bm: 16, 32, 64, 128 or 256 token rows a block; splits: CTAs along K, 1 to 8 and at most the K-tiles
+int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream) {
   switch (bm) {
     case 16: return launch_linear_tc<16>(a, splits, status, stream);
     case 32: return launch_linear_tc<32>(a, splits, status, stream);
