@@ -7,10 +7,10 @@
 namespace b200moe {
 
 // ------------------------------------------------------------------------------------------------ weight layout
-// One CTA per (row of a tile, tile): 16-byte pieces of the source row into the swizzled image, its scales into the atoms.
+// One CTA per (row of a tile, tile): 16-byte pieces of the source row into the swizzled images, its scales into the atoms.
 __global__ void preshuffle_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int k,
                                          int tiles_k, int gated, uint8_t* __restrict__ out) {
-  const int64_t t = blockIdx.x >> 7;
+  const int64_t t = blockIdx.x >> 7, tiles = static_cast<int64_t>(gridDim.x >> 7) * tiles_k;
   const int r = static_cast<int>(blockIdx.x & 127u);
   int64_t src = t * 128 + r;
   bool have = src < rows;
@@ -20,15 +20,16 @@ __global__ void preshuffle_linear_kernel(const uint8_t* __restrict__ codes, cons
     have = i < half;
     src = (g & 1) ? half + i : i;
   }
-  uint8_t* tile0 = out + t * tiles_k * kLinearRecordBytes;
+  uint8_t* image0 = out + t * tiles_k * kLinearImageBytes;
+  uint8_t* atom0 = out + tiles * kLinearImageBytes + t * tiles_k * kAtomBytes;
   for (int j = threadIdx.x; j < tiles_k * 8; j += blockDim.x) {
     const int kt = j >> 3, c = j & 7;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (have && j * 16 < k) v = *reinterpret_cast<const uint4*>(codes + src * k + j * 16);
-    *reinterpret_cast<uint4*>(tile0 + static_cast<int64_t>(kt) * kLinearRecordBytes + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+    *reinterpret_cast<uint4*>(image0 + static_cast<int64_t>(kt) * kLinearImageBytes + r * 128 + ((c ^ (r & 7)) << 4)) = v;
   }
   for (int j = threadIdx.x; j < tiles_k * 4; j += blockDim.x)
-    tile0[static_cast<int64_t>(j >> 2) * kLinearRecordBytes + kLinearCodeBytes + atom_offset(r, j & 3)] =
+    atom0[static_cast<int64_t>(j >> 2) * kAtomBytes + atom_offset(r, j & 3)] =
         have && j * 32 < k ? scales[src * (k / 32) + j] : static_cast<uint8_t>(127);
 }
 
@@ -83,8 +84,8 @@ static int64_t linear_k_tiles(int64_t k) { return (k + 127) / 128; }
 
 static bool linear_dims(int64_t rows, int64_t k, int gated) {
   if (rows < 8 || k < 32 || k % 32 || rows % (gated ? 64 : 8) || rows > B200MOE_LINEAR_MAX_DIM || k > B200MOE_LINEAR_MAX_DIM) return false;
-  // the weights seen as rows of 128 bytes are counted in 32 bits (274 GB)
-  return linear_row_tiles(rows) * linear_k_tiles(k) <= INT32_MAX / 132;
+  // the images seen as rows of 128 bytes are counted in 32 bits (274 GB)
+  return linear_row_tiles(rows) * linear_k_tiles(k) <= INT32_MAX / 128;
 }
 
 static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
@@ -112,7 +113,7 @@ static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t st
 extern "C" size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated) {
   using namespace b200moe;
   if (!linear_dims(rows, k, gated)) return 0;
-  return static_cast<size_t>(linear_row_tiles(rows)) * linear_k_tiles(k) * kLinearRecordBytes;
+  return static_cast<size_t>(linear_row_tiles(rows)) * linear_k_tiles(k) * kLinearTileBytes;
 }
 
 extern "C" int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated,
@@ -186,6 +187,7 @@ static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const uin
   a.n = static_cast<int>(n);
   a.tiles_n = static_cast<int>(linear_row_tiles(w->rows));
   a.tiles_k = static_cast<int>(linear_k_tiles(w->k));
+  a.atoms = w->tiles + static_cast<int64_t>(a.tiles_n) * a.tiles_k * kLinearImageBytes;
   a.act = act_args(activation);
   return 0;
 }

@@ -5,12 +5,16 @@
 
 namespace b200moe {
 
-// Weights: records of 128 weight rows x 128 K-elements, [row tile][K-tile]: 16384 bytes of E4M3 codes in the 128-byte-swizzled
-// shared-memory image, then one scale atom. Rows and columns beyond the matrix are zeros. Gated weights (gate rows, then up rows) are
-// interleaved in groups of 32, [gate 32 | up 32 | gate 32 | up 32], so that a tile holds 64 output columns with both halves.
-constexpr int kLinearCodeBytes = 128 * 128;
-constexpr int kLinearRecordBytes = kLinearCodeBytes + kAtomBytes;
-constexpr int kLinearRecordRows = kLinearRecordBytes / 128;  // 132: the tiles seen as rows of 128 bytes
+// Weights: first the codes, [row tile][K-tile] images of 128 weight rows x 128 K-elements, 16384 bytes of E4M3 as the 128-byte swizzle
+// lays them in shared memory; behind them the scales, [row tile][K-tile] atoms of 512 bytes, so that those of several K-tiles are one
+// copy. Rows and columns beyond the matrix are zeros. Gated weights (gate rows, then up rows) are interleaved in groups of 32,
+// [gate 32 | up 32 | gate 32 | up 32], so that a tile holds 64 output columns with both halves.
+constexpr int kLinearImageBytes = 128 * 128;
+constexpr int kLinearTileBytes = kLinearImageBytes + kAtomBytes;
+
+// Scales travel in groups of four K-tiles, ahead of the codes: two or three groups in shared memory, kSfSets in tensor memory. A copy, its
+// waits and its commit then cost the issuing warps a quarter, and the MMAs never wait for a scale that came with its codes.
+constexpr int kSfGroup = 4, kSfSets = 2;
 
 // What the epilogue does with a sum p (or a gate g and an up u):
 //   kLinear   p, or 0 where p < floor (ReLU: 0, none: -inf)
@@ -24,7 +28,8 @@ struct LinearAct {
 };
 
 struct LinearArgs {
-  const uint8_t* tiles;
+  const uint8_t* tiles;           // images
+  const uint8_t* atoms;           // scale atoms
   const float* bias;              // [weight rows] or null
   const uint8_t* codes;           // [m][k]
   const uint8_t* scales;          // [m][k / 32]
@@ -85,17 +90,31 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// The four scale bytes of K-tile kt of row `row` (0 beyond the rows or the columns). `words`: rows of scales begin at multiples of 4 bytes.
-__device__ __forceinline__ uint32_t row_scales(const uint8_t* scales, int64_t row, int64_t rows, int kt, int per_row, bool words) {
-  if (row >= rows) return 0u;
-  const uint8_t* p = scales + row * per_row + kt * 4;
-  if (words) return __ldcg(reinterpret_cast<const uint32_t*>(p));
-  uint32_t v = 0u;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (kt * 4 + j < per_row) v |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * j);
-  return v;
+// How rows of scales begin: at multiples of 16 bytes (K a multiple of 512), of 4 (of 128), or anywhere.
+__device__ __forceinline__ int scale_alignment(const uint8_t* scales, int k) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(k / 32);
+  return (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
 }
+// The scale bytes of K-tiles kt .. kt + 3 of a row, 4 a K-tile; 0 beyond the rows and the columns
+__device__ __forceinline__ uint4 row_scales(const uint8_t* scales, int64_t row, int64_t rows, int kt, int k, int alignment) {
+  uint32_t v[4] = {0u, 0u, 0u, 0u};
+  const int per_row = k / 32;
+  if (row < rows) {
+    const uint8_t* p = scales + row * per_row + kt * 4;
+    if (alignment == 16 && (kt & 3) == 0) return __ldcg(reinterpret_cast<const uint4*>(p));  // (16 bytes divide the row)
+    if (alignment >= 4) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if ((kt + d) * 4 < per_row) v[d] = __ldcg(reinterpret_cast<const uint32_t*>(p) + d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (kt * 4 + j < per_row) v[j >> 2] |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * (j & 3));
+    }
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4 v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
 
 // 32 bytes, one sector, by one thread (32-byte aligned)
 __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {

@@ -2,8 +2,8 @@
 // N = 256 or 128 weight rows (NT = two tiles or one) x K = 32 per instruction, each CTA staging its own 128 token rows and half of the
 // weight rows. No multicast.
 //
-// Unit = (pair of token blocks) x (NT weight tiles). Two rings: 6 stages of codes, and 8 slots of scales that travel ahead of them, so
-// that the MMA warp waits for codes only. The token scales come row-major, as every producer of this package writes them: the scale
+// Unit = (pair of token blocks) x (NT weight tiles). Two rings: 6 stages of codes, and 3 slots of the scales of four K-tiles that travel
+// ahead of them, so that the MMA warp waits for codes and, once in four K-tiles, for scales. The token scales come row-major, as every producer of this package writes them: the scale
 // warp turns them into atoms on the way, so no launch in front of the product re-lays them.
 //
 //   warp 0      code producer (both CTAs): TMA of the CTA's 128 token rows and of its weight rows, counted on the leader's barrier
@@ -22,20 +22,20 @@ namespace b200moe {
 template <int NT>
 struct LinearPairCfg {
   static constexpr int kStages = 6;                     // code ring
-  static constexpr int kSfStages = 8;                   // scale ring = scale sets in tensor memory
   static constexpr int kWRows = 64 * NT;                // weight rows of one CTA
   static constexpr int kWOff = 128 * 128;               // behind the CTA's 128 token rows
   static constexpr int kStageBytes = kWOff + kWRows * 128;
+  static constexpr int kSfSlots = 3;                    // groups of scales in shared memory
   static constexpr int kSfOff = kStages * kStageBytes;
-  static constexpr int kSfSlotBytes = (1 + NT) * kAtomBytes;  // token atom, weight atoms
-  static constexpr int kBiasOff = kSfOff + kSfStages * kSfSlotBytes;
+  static constexpr int kSfSlotBytes = kSfGroup * (1 + NT) * kAtomBytes;  // four token atoms, four atoms of each weight tile
+  static constexpr int kBiasOff = kSfOff + kSfSlots * kSfSlotBytes;
   static constexpr int kCols = 64 * NT;                 // accumulator columns of an epilogue thread
   static constexpr int kSmemBytes = kBiasOff + 8 * kCols * 4 + 1024;
   static constexpr int kThreads = 32 * 12;
   static constexpr int kAccs = NT == 1 ? 2 : 1;         // accumulators of 128 * NT columns
-  static constexpr int kSfCol = 256;                    // tensor memory: accumulators, then 8 sets of 16 columns
+  static constexpr int kSfCol = 256;                    // tensor memory: accumulators, then 2 sets of 4 x 16 columns
   static constexpr int kTmemCols = 512;
-  static_assert(kSmemBytes <= 227 * 1024 && kSfStages >= kStages, "a scale set is free once the code stage is");
+  static_assert(kSmemBytes <= 227 * 1024 && kSfCol + kSfSets * kSfGroup * 16 <= kTmemCols, "shared and tensor memory");
 };
 
 __device__ __forceinline__ void tc_mma_mxf8_two(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -54,8 +54,13 @@ __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_add
 }
 __device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
   if (!mbar_wait(bar, parity, abort_flag, status)) return false;
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return true;
+  uint32_t ok;  // the phase is complete: this look succeeds at once, and acquires at the writers' scope
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // The units in groups of 8 pairs of token blocks: a group sweeps the weights once, tile by tile, so that its tokens (2048 rows) and the
@@ -79,8 +84,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[C::kStages];     // leader: both CTAs' codes of the stage have landed
   __shared__ __align__(8) uint64_t bar_empty[C::kStages];    // in each CTA: the MMAs that read the stage have completed
-  __shared__ __align__(8) uint64_t bar_sfull[C::kSfStages];  // leader: both CTAs' scales of the slot are there
-  __shared__ __align__(8) uint64_t bar_sf[C::kSfStages];     // in each CTA: they have been copied to tensor memory
+  __shared__ __align__(8) uint64_t bar_sfull[C::kSfSlots];      // leader: both CTAs' scales of the group are there
+  __shared__ __align__(8) uint64_t bar_sf[C::kSfSlots];         // in each CTA: they have been copied to tensor memory
+  __shared__ __align__(8) uint64_t bar_set[kSfSets];         // leader: the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull[C::kAccs];      // in each CTA: the unit's accumulator is complete
   __shared__ __align__(8) uint64_t bar_tempty[C::kAccs];     // leader: both CTAs' epilogues have read it
   __shared__ __align__(8) uint64_t bar_drain[2];
@@ -92,7 +98,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   const bool leader = rank == 0;
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const tiles_ptr = smem_raw + (tiles - smem_u32(smem_raw));
-  const uint32_t sf_ring = tiles + C::kSfOff;
   volatile int* abort_v = &abort_flag;
   pdl_launch_dependents();
 
@@ -102,7 +107,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
-    for (int j = 0; j < C::kSfStages; ++j) {
+    for (int j = 0; j < kSfSets; ++j) mbar_init(smem_u32(&bar_set[j]), 1);
+    for (int j = 0; j < C::kSfSlots; ++j) {
       mbar_init(smem_u32(&bar_sfull[j]), 3);  // the leader's byte count, the token scales of both CTAs
       mbar_init(smem_u32(&bar_sf[j]), 1);
     }
@@ -150,9 +156,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
           units.at(u, pair, step);
           const int row = pair * 256 + static_cast<int>(rank) * 128;
           // NT = 2: the whole tile 2 step + rank; NT = 1: half of tile `step`
-          int rec = NT == 2 ? (2 * step + static_cast<int>(rank)) * tiles_k * kLinearRecordRows
-                            : step * tiles_k * kLinearRecordRows + static_cast<int>(rank) * 64;
-          for (int kt = 0; kt < tiles_k; ++kt, ++it, rec += kLinearRecordRows) {
+          int rec = NT == 2 ? (2 * step + static_cast<int>(rank)) * tiles_k * 128
+                            : step * tiles_k * 128 + static_cast<int>(rank) * 64;
+          for (int kt = 0; kt < tiles_k; ++kt, ++it, rec += 128) {
             if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
             const uint32_t full = full0 + 8u * s, base = tiles + s * C::kStageBytes;
             if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), 2 * C::kStageBytes);
@@ -165,87 +171,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
         if (!ok && leader) drain_copies(bar_full, it, C::kStages);
       }
     } else if (warp == 3) {
-      // ---------------------------------------------------------------- scales (both CTAs): lane l writes 16 bytes of the token atom, rows
-      // l, l + 32, l + 64 and l + 96, four K-tiles of loads ahead
+      // ---------------------------------------------------------------- scales (both CTAs): lane l writes 16 bytes of a token atom, rows l,
+      // l + 32, l + 64 and l + 96. A group's bytes are asked for as soon as those of the group before it are stored.
       const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
-      const int per_row = a.k / 32;
-      const bool words = (per_row & 3) == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 3) == 0;
-      uint32_t now[4][4], next[4][4];
-      uint32_t it = 0, j = 0, ph = 1u;
-      bool ok = true;
-      for (int u = cluster; u < total && ok; u += n_clusters) {
+      const int alignment = scale_alignment(a.scales, a.k);
+      uint4 v[4];
+      const auto fetch = [&](int u, int kt) {
         units.at(u, pair, step);
         const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + lane;
-        const auto fetch = [&](int kt, uint32_t (&v)[4][4]) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[d][i] = kt + d < tiles_k ? row_scales(a.scales, row + 32 * i, a.m, kt + d, per_row, words) : 0u;
-        };
-        fetch(0, now);
-        int rec = NT * step * tiles_k * kLinearRecordRows + 128;
-        for (int kt0 = 0; kt0 < tiles_k && ok; kt0 += 4) {
-          fetch(kt0 + 4, next);
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            if (kt0 + d >= tiles_k || !ok) break;
-            // free once its previous contents are in tensor memory
-            if (!warp_wait(smem_u32(&bar_sf[j]), ph, abort_v, status)) { ok = false; break; }
-            const uint32_t sfull = sfull0 + 8u * j, slot = sf_ring + j * C::kSfSlotBytes;
-            if (lane == 0) {
-              if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[j]), 2 * NT * kAtomBytes);
-              tma_load_2d_pair(slot + kAtomBytes, &map_ws, 0, rec, sfull);
-              if (NT == 2) tma_load_2d_pair(slot + 2 * kAtomBytes, &map_ws, 0, rec + tiles_k * kLinearRecordRows, sfull);
-            }
-            *(reinterpret_cast<uint4*>(tiles_ptr + C::kSfOff + j * C::kSfSlotBytes) + lane) = make_uint4(now[d][0], now[d][1], now[d][2], now[d][3]);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_release_cluster(sfull);
-            rec += kLinearRecordRows;
-            ++it;
-            if (++j == C::kSfStages) { j = 0; ph ^= 1u; }
+        for (int i = 0; i < 4; ++i) v[i] = row_scales(a.scales, row + 32 * i, a.m, kt, a.k, alignment);
+      };
+      uint32_t it = 0, slot = 0, ph = 1u;
+      bool ok = true;
+      if (cluster < total) fetch(cluster, 0);
+      for (int u = cluster; u < total && ok; u += n_clusters) {
+        units.at(u, pair, step);
+        int atom = NT * step * tiles_k * 4;  // the atoms seen as rows of 128 bytes
+        for (int kt = 0; kt < tiles_k; kt += kSfGroup, atom += kSfGroup * 4) {
+          // free once its previous contents are in tensor memory
+          if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; break; }
+          const uint32_t sfull = sfull0 + 8u * slot, at = C::kSfOff + slot * C::kSfSlotBytes;
+          if (lane == 0) {
+            if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 2 * NT * kSfGroup * kAtomBytes);
+            // (a last group of fewer K-tiles brings the next tile's atoms or zeros along, which nothing reads)
+            tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
+            if (NT == 2) tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
           }
+          ++it;
+          uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at) + lane;
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) now[d][i] = next[d][i];
+          for (int d = 0; d < kSfGroup; ++d) cells[d * 32] = make_uint4(word_of(v[0], d), word_of(v[1], d), word_of(v[2], d), word_of(v[3], d));
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_release_cluster(sfull);
+          if (kt + kSfGroup < tiles_k) fetch(u, kt + kSfGroup);
+          else if (u + n_clusters < total) fetch(u + n_clusters, 0);
+          if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
         }
       }
-      if (!ok && leader && lane == 0) drain_copies(bar_sfull, it, C::kSfStages);
+      if (!ok && leader && lane == 0) drain_copies(bar_sfull, it, C::kSfSlots);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue (leader only)
       if (leader) {
         // E4M3 x E4M3, UE8M0 scales, M = 256, N = 128 NT; scale byte k of a row's cell for MMA k
         constexpr uint32_t kIdesc = (static_cast<uint32_t>(128 * NT >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24);
-        uint32_t ui = 0, s = 0, ph = 0, j = 0, sph = 0;
-        bool ok = true, sf_ready = false, full_ready = false;
+        uint32_t ui = 0, s = 0, ph = 0, slot = 0, sph = 0, set = 0;
+        bool ok = true, ready = false;
         for (int u = cluster; u < total && ok; u += n_clusters, ++ui) {
           const uint32_t acc = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
           if (!warp_wait(smem_u32(&bar_tempty[acc]), aph ^ 1u, abort_v, status)) break;
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * 128 * NT;
-          for (int kt = 0; kt < tiles_k; ++kt) {
-            if (!__all_sync(0xffffffffu, (sf_ready || mbar_wait(smem_u32(&bar_sf[j]), sph, abort_v, status)) &&
-                                             (full_ready || mbar_wait(smem_u32(&bar_full[s]), ph, abort_v, status)))) {
-              ok = false;
-              break;
+          for (int kt = 0; kt < tiles_k && ok; kt += kSfGroup) {
+            if (!warp_wait(smem_u32(&bar_sf[slot]), sph, abort_v, status)) { ok = false; break; }
+            if (++slot == C::kSfSlots) { slot = 0; sph ^= 1u; }
+            const int n = tiles_k - kt < kSfGroup ? tiles_k - kt : kSfGroup;
+            uint32_t t_sft = tmem_base + C::kSfCol + set * kSfGroup * 16;
+#pragma unroll 1
+            for (int d = 0; d < n; ++d, t_sft += 16) {
+              if (!__all_sync(0xffffffffu, ready || mbar_wait(smem_u32(&bar_full[s]), ph, abort_v, status))) { ok = false; break; }
+              tc_fence_after();
+              const uint32_t x_lo = (tiles + s * C::kStageBytes) >> 4, w_lo = x_lo + (C::kWOff >> 4), empty = smem_u32(&bar_empty[s]);
+              const uint32_t t_sfw = t_sft + 8u;
+              if (++s == C::kStages) { s = 0; ph ^= 1u; }
+              ready = mbar_test(smem_u32(&bar_full[s]), ph);
+              if (elect_one()) {
+                tc_mma_mxf8_two(d_tmem, x_lo, w_lo, kIdesc, t_sft, t_sfw, static_cast<uint32_t>(kt + d != 0));
+                tc_mma_mxf8_two(d_tmem, x_lo + 2, w_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sft, t_sfw, 1u);
+                tc_mma_mxf8_two(d_tmem, x_lo + 4, w_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sft, t_sfw, 1u);
+                tc_mma_mxf8_two(d_tmem, x_lo + 6, w_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sft, t_sfw, 1u);
+                tc_commit_both(empty);  // the stage is free again, in both CTAs
+                if (d == n - 1) tc_commit_pair(smem_u32(&bar_set[set]));
+              }
+              __syncwarp();
             }
-            tc_fence_after();
-            const uint32_t s_now = s, j_now = j;
-            if (++s == C::kStages) { s = 0; ph ^= 1u; }
-            if (++j == C::kSfStages) { j = 0; sph ^= 1u; }
-            sf_ready = mbar_test(smem_u32(&bar_sf[j]), sph);
-            full_ready = mbar_test(smem_u32(&bar_full[s]), ph);
-            const uint32_t x_lo = (tiles + s_now * C::kStageBytes) >> 4, w_lo = x_lo + (C::kWOff >> 4);
-            const uint32_t t_sft = tmem_base + C::kSfCol + 16u * j_now, t_sfw = t_sft + 8u;
-            if (elect_one()) {
-              tc_mma_mxf8_two(d_tmem, x_lo, w_lo, kIdesc, t_sft, t_sfw, static_cast<uint32_t>(kt != 0));
-              tc_mma_mxf8_two(d_tmem, x_lo + 2, w_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sft, t_sfw, 1u);
-              tc_mma_mxf8_two(d_tmem, x_lo + 4, w_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sft, t_sfw, 1u);
-              tc_mma_mxf8_two(d_tmem, x_lo + 6, w_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sft, t_sfw, 1u);
-              tc_commit_both(smem_u32(&bar_empty[s_now]));  // the stage is free again, in both CTAs
-            }
-            __syncwarp();
+            if (++set == kSfSets) set = 0;
           }
           if (ok && elect_one()) tc_commit_both(smem_u32(&bar_tfull[acc]));
         }
@@ -254,28 +255,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     } else {
       // ---------------------------------------------------------------- scale copies into both CTAs' tensor memory (leader)
       if (leader) {
-        uint32_t s = 0, ph = 1u, j = 0, sph = 0;
+        uint32_t slot = 0, ph = 0, set = 0, set_ph = 1u;
         bool ok = true;
         for (int u = cluster; u < total && ok; u += n_clusters) {
-          for (int kt = 0; kt < tiles_k; ++kt) {
-            // set j was last read by the MMAs 8 K-tiles back: complete once those that read stage s, kStages back, are
-            if (!__all_sync(0xffffffffu, mbar_wait_acquire_cluster(smem_u32(&bar_sfull[j]), sph, abort_v, status) &&
-                                             mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status))) {
+          for (int kt = 0; kt < tiles_k; kt += kSfGroup) {
+            if (!__all_sync(0xffffffffu, mbar_wait_acquire_cluster(smem_u32(&bar_sfull[slot]), ph, abort_v, status) &&
+                                             mbar_wait(smem_u32(&bar_set[set]), set_ph, abort_v, status))) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t lo = (sf_ring + j * C::kSfSlotBytes) >> 4, sf_bar = smem_u32(&bar_sf[j]);
-            const uint32_t t_sft = tmem_base + C::kSfCol + 16u * j, t_sfw = t_sft + 8u;
-            if (++s == C::kStages) { s = 0; ph ^= 1u; }
-            if (++j == C::kSfStages) { j = 0; sph ^= 1u; }
+            const int n = tiles_k - kt < kSfGroup ? tiles_k - kt : kSfGroup;
+            const uint32_t lo = (tiles + C::kSfOff + slot * C::kSfSlotBytes) >> 4;
+            const uint32_t t_sft = tmem_base + C::kSfCol + set * kSfGroup * 16, t_sfw = t_sft + 8u;
             if (elect_one()) {
-              tc_cp_scales_pair(t_sft, lo);                         // each CTA its own token rows
-              tc_cp_scales_pair(t_sfw, lo + (kAtomBytes >> 4));     // weight rows 0..127 of N
-              if (NT == 2) tc_cp_scales_pair(t_sfw + 4, lo + (2 * kAtomBytes >> 4));  // 128..255
-              tc_commit_both(sf_bar);
+              for (int d = 0; d < n; ++d) {
+                const uint32_t from = lo + d * (kAtomBytes >> 4);
+                tc_cp_scales_pair(t_sft + 16 * d, from);                                         // each CTA its own token rows
+                tc_cp_scales_pair(t_sfw + 16 * d, from + (kSfGroup * kAtomBytes >> 4));          // weight rows 0..127 of N
+                if (NT == 2) tc_cp_scales_pair(t_sfw + 16 * d + 4, from + (2 * kSfGroup * kAtomBytes >> 4));  // 128..255
+              }
+              tc_commit_both(smem_u32(&bar_sf[slot]));
             }
             __syncwarp();
+            if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+            if (++set == kSfSets) { set = 0; set_ph ^= 1u; }
           }
         }
         if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05_pair(smem_u32(&bar_drain[1]));
@@ -428,11 +432,11 @@ template <int KIND, bool MX, int NT>
 static int launch_linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   using C = LinearPairCfg<NT>;
   CUtensorMap mx, mwc, mws;
-  const uint64_t w_rows = static_cast<uint64_t>(a.tiles_n) * a.tiles_k * kLinearRecordRows;
+  const uint64_t n_tiles = static_cast<uint64_t>(a.tiles_n) * a.tiles_k;
   int r;
   if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), 128))) return r;
-  if ((r = make_flat_map(&mwc, a.tiles, w_rows, C::kWRows))) return r;
-  if ((r = make_flat_map(&mws, a.tiles, w_rows, 4))) return r;
+  if ((r = make_flat_map(&mwc, a.tiles, n_tiles * 128, C::kWRows))) return r;
+  if ((r = make_flat_map(&mws, a.atoms, n_tiles * 4, kSfGroup * 4))) return r;
   const int64_t units = (a.m + 255) / 256 * ((a.tiles_n + NT - 1) / NT);
   if (units > 0x7fffffff) return B200MOE_E_ARG;
   const int pairs = linear_pairs<KIND, MX, NT>();

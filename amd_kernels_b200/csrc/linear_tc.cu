@@ -6,10 +6,10 @@
 // the CTAs share out the block's rows: the parts of a row are added in the order of K through distributed shared memory, then
 // bias, activation, residual and the only rounding. No workspace, no atomics, one launch, sums in a fixed order.
 //
-//   warp 0     producer: the weight record (codes and scales, one bulk copy of consecutive HBM bytes) and the token rows (TMA)
+//   warp 0     code producer: the weight image (one bulk copy of consecutive HBM bytes) and the token rows (TMA)
 //   warp 1     tensor memory; issues the MMAs, the whole warp around one elected lane
 //   warp 2     scales: shared memory -> tensor memory
-//   warp 3     token scales: row-major global memory -> scale atoms in shared memory, four K-tiles of loads ahead
+//   warp 3     scale producer: the weights' atoms (bulk copy); the tokens' from row-major global memory through registers
 //   warps 4-7  the sum out of tensor memory; all warps take part in what follows
 #include "linear.cuh"
 #include "tc_pair.cuh"
@@ -18,17 +18,19 @@ namespace b200moe {
 
 template <int BM>
 struct LinearCfg {
-  static constexpr int kAtoms = BM > 128 ? 2 : 1;           // token scale atoms of a K-tile
-  static constexpr int kTokOff = 17408;                     // weight record padded to the token tile's 1024-byte alignment
+  static constexpr int kAtoms = BM > 128 ? 2 : 1;                            // token scale atoms of a K-tile
+  static constexpr int kTokOff = kLinearImageBytes;                          // token rows behind the weight image
   static constexpr int kStageBytes = kTokOff + BM * 128;
-  static constexpr int kTxBytes = kLinearRecordBytes + BM * 128;
-  static constexpr int kCtasPerSm = BM > 128 ? 1 : 2;       // two: one's start and end under the other's stream
+  static constexpr int kCtasPerSm = BM > 128 ? 1 : 2;                        // two: one's start and end under the other's stream
   static constexpr int kStages = BM > 128 ? 4 : BM > 64 ? 3 : BM > 32 ? 4 : 5;
-  static constexpr int kSfOff = kStages * kStageBytes;      // token scale atoms, one slot a stage
-  static constexpr int kSumRow = 132;                       // floats of a token's 128 columns in the parts (aliases the ring)
-  static constexpr int kSmemBytes = kSfOff + kStages * kAtoms * kAtomBytes + 1024;
-  static constexpr int kSfCols = kAtoms > 1 ? 16 : 8;       // tensor memory columns of a stage's scales: weights 4, tokens from 4 (8) on
-  static constexpr int kColsUsed = BM + kStages * kSfCols;
+  static constexpr int kSfSlots = 2;                                         // groups of scales in shared memory
+  static constexpr int kSfOff = kStages * kStageBytes;
+  static constexpr int kSfTileBytes = (1 + kAtoms) * kAtomBytes;             // a K-tile's scales in a slot: see below
+  static constexpr int kSfSlotBytes = kSfGroup * kSfTileBytes;               // weight atoms of the group, then token atoms by K-tile
+  static constexpr int kSumRow = 132;                                        // floats of a token's 128 columns in the parts (alias the ring)
+  static constexpr int kSmemBytes = kSfOff + kSfSlots * kSfSlotBytes + 1024;
+  static constexpr int kSfCols = kAtoms > 1 ? 16 : 8;                        // tensor memory columns of a K-tile's scales: weights, tokens
+  static constexpr int kColsUsed = BM + kSfSets * kSfGroup * kSfCols;
   static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static_assert(BM * kSumRow * 4 <= kSfOff, "the parts fit the ring");
   static_assert(kSmemBytes <= 227 * 1024 / kCtasPerSm - 1024 && kTmemCols * kCtasPerSm <= 512, "shared and tensor memory");
@@ -123,10 +125,11 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
                      int32_t* status) {
   using C = LinearCfg<BM>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[C::kStages];   // weight record and token rows of the stage have landed
-  __shared__ __align__(8) uint64_t bar_xs[C::kStages];     // its token scales are written
-  __shared__ __align__(8) uint64_t bar_sf[C::kStages];     // its scales are in tensor memory
+  __shared__ __align__(8) uint64_t bar_full[C::kStages];   // weight image and token rows of the stage have landed
   __shared__ __align__(8) uint64_t bar_empty[C::kStages];  // the MMAs that read it have completed
+  __shared__ __align__(8) uint64_t bar_sfull[C::kSfSlots];    // the scales of the group are in shared memory
+  __shared__ __align__(8) uint64_t bar_sf[C::kSfSlots];       // they are in tensor memory
+  __shared__ __align__(8) uint64_t bar_set[kSfSets];       // the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull;
   __shared__ __align__(8) uint64_t bar_drain[2];
   __shared__ uint32_t tmem_base_slot;
@@ -134,16 +137,20 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const tiles_ptr = smem_raw + (tiles - smem_u32(smem_raw));
   volatile int* abort_v = &abort_flag;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_xs[s]), 1);
-      mbar_init(smem_u32(&bar_sf[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
+    for (int j = 0; j < C::kSfSlots; ++j) {
+      mbar_init(smem_u32(&bar_sfull[j]), 2);  // the byte count of the weights' atoms, the tokens' atoms
+      mbar_init(smem_u32(&bar_sf[j]), 1);
+    }
+    for (int j = 0; j < kSfSets; ++j) mbar_init(smem_u32(&bar_set[j]), 1);
     mbar_init(smem_u32(&bar_tfull), 1);
     mbar_init(smem_u32(&bar_drain[0]), 1);
     mbar_init(smem_u32(&bar_drain[1]), 1);
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   pdl_wait();
   LinearArgs a = args;
   launder(a.tiles);
+  launder(a.atoms);
   launder(a.scales);
   launder(a.bias);
   launder(a.residual);
@@ -174,15 +182,15 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   const int kt1 = static_cast<int>(static_cast<int64_t>(a.tiles_k) * (rank + 1) / splits);
 
   if (warp == 0) {
-    if (lane == 0) {  // ------------------------------------------------ producer
-      const uint8_t* w_src = a.tiles + (static_cast<int64_t>(tile) * a.tiles_k + kt0) * kLinearRecordBytes;
+    if (lane == 0) {  // ------------------------------------------------ code producer
+      const uint8_t* w_src = a.tiles + (static_cast<int64_t>(tile) * a.tiles_k + kt0) * kLinearImageBytes;
       uint32_t it = 0, s = 0, ph = 1u;
       bool ok = true;
-      for (int kt = kt0; kt < kt1; ++kt, ++it, w_src += kLinearRecordBytes) {
+      for (int kt = kt0; kt < kt1; ++kt, ++it, w_src += kLinearImageBytes) {
         if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
         const uint32_t full = smem_u32(&bar_full[s]), base = tiles + s * C::kStageBytes;
-        mbar_arrive_expect_tx(full, C::kTxBytes);
-        bulk_load(base, w_src, kLinearRecordBytes, full);
+        mbar_arrive_expect_tx(full, C::kStageBytes);
+        bulk_load(base, w_src, kLinearImageBytes, full);
         tma_load_2d(base + C::kTokOff, &map_x, kt * 128, static_cast<int>(row0), full);
         if (++s == C::kStages) { s = 0; ph ^= 1u; }
       }
@@ -191,89 +199,102 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issue: E4M3 x E4M3, UE8M0 scales, M = 128, N = BM
     constexpr uint32_t kIdesc = (static_cast<uint32_t>(BM >> 3) << 17) | (1u << 23) | (8u << 24);
-    uint32_t s = 0, ph = 0;
-    bool ok = true;
-    for (int kt = kt0; kt < kt1; ++kt) {
-      if (!warp_wait(smem_u32(&bar_sf[s]), ph, abort_v, status)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t w_lo = (tiles + s * C::kStageBytes) >> 4, x_lo = w_lo + (C::kTokOff >> 4);
-      const uint32_t t_sfw = tmem_base + BM + C::kSfCols * s, t_sfx = t_sfw + C::kSfCols / 2;
-      if (elect_one()) {
-        tc_mma_mxf8_lo<2>(tmem_base, w_lo, x_lo, kIdesc, t_sfw, t_sfx, static_cast<uint32_t>(kt != kt0));
-        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 2, x_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sfw, t_sfx);
-        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 4, x_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sfw, t_sfx);
-        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 6, x_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sfw, t_sfx);
-        tc_commit(smem_u32(&bar_empty[s]));
+    uint32_t s = 0, ph = 0, slot = 0, sph = 0, set = 0;
+    bool ok = true, ready = false;
+    for (int kt = kt0; kt < kt1 && ok; kt += kSfGroup) {
+      if (!warp_wait(smem_u32(&bar_sf[slot]), sph, abort_v, status)) { ok = false; break; }
+      if (++slot == C::kSfSlots) { slot = 0; sph ^= 1u; }
+      const int n = kt1 - kt < kSfGroup ? kt1 - kt : kSfGroup;
+      uint32_t t_sfw = tmem_base + BM + set * kSfGroup * C::kSfCols;
+#pragma unroll 1
+      for (int d = 0; d < n; ++d, t_sfw += C::kSfCols) {
+        if (!__all_sync(0xffffffffu, ready || mbar_wait(smem_u32(&bar_full[s]), ph, abort_v, status))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t w_lo = (tiles + s * C::kStageBytes) >> 4, x_lo = w_lo + (C::kTokOff >> 4), empty = smem_u32(&bar_empty[s]);
+        const uint32_t t_sfx = t_sfw + C::kSfCols / 2;
+        if (++s == C::kStages) { s = 0; ph ^= 1u; }
+        ready = mbar_test(smem_u32(&bar_full[s]), ph);
+        if (elect_one()) {
+          tc_mma_mxf8_lo<2>(tmem_base, w_lo, x_lo, kIdesc, t_sfw, t_sfx, static_cast<uint32_t>(kt + d != kt0));
+          tc_mma_mxf8_lo<1>(tmem_base, w_lo + 2, x_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sfw, t_sfx);
+          tc_mma_mxf8_lo<1>(tmem_base, w_lo + 4, x_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sfw, t_sfx);
+          tc_mma_mxf8_lo<1>(tmem_base, w_lo + 6, x_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sfw, t_sfx);
+          tc_commit(empty);
+          if (d == n - 1) tc_commit(smem_u32(&bar_set[set]));
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (++s == C::kStages) { s = 0; ph ^= 1u; }
+      if (++set == kSfSets) set = 0;
     }
     if (ok && elect_one()) tc_commit(smem_u32(&bar_tfull));
     if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[0]));
   } else if (warp == 2) {
     // ------------------------------------------------ scale copies into tensor memory
-    uint32_t s = 0, ph = 0;
-    for (int kt = kt0; kt < kt1; ++kt) {
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[s]), ph, abort_v, status) &&
-                                       mbar_wait(smem_u32(&bar_xs[s]), ph, abort_v, status)))
+    uint32_t slot = 0, ph = 0, set = 0, set_ph = 1u;
+    for (int kt = kt0; kt < kt1; kt += kSfGroup) {
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_sfull[slot]), ph, abort_v, status) &&
+                                       mbar_wait(smem_u32(&bar_set[set]), set_ph, abort_v, status)))
         break;
       tc_fence_after();
-      const uint32_t w_atom = (tiles + s * C::kStageBytes + kLinearCodeBytes) >> 4;
-      const uint32_t x_atom = (tiles + C::kSfOff + s * C::kAtoms * kAtomBytes) >> 4;
-      const uint32_t t_sfw = tmem_base + BM + C::kSfCols * s, t_sfx = t_sfw + C::kSfCols / 2;
+      const int n = kt1 - kt < kSfGroup ? kt1 - kt : kSfGroup;
+      const uint32_t w_atom = (tiles + C::kSfOff + slot * C::kSfSlotBytes) >> 4, x_atom = w_atom + (kSfGroup * kAtomBytes >> 4);
+      const uint32_t t_sfw = tmem_base + BM + set * kSfGroup * C::kSfCols, t_sfx = t_sfw + C::kSfCols / 2;
       if (elect_one()) {
-        tc_cp_scales_lo(t_sfw, w_atom);
-        tc_cp_scales_lo(t_sfx, x_atom);
-        if (C::kAtoms > 1) tc_cp_scales_lo(t_sfx + 4, x_atom + (kAtomBytes >> 4));
-        tc_commit(smem_u32(&bar_sf[s]));
+        for (int d = 0; d < n; ++d) {
+          tc_cp_scales_lo(t_sfw + d * C::kSfCols, w_atom + d * (kAtomBytes >> 4));
+#pragma unroll
+          for (int h = 0; h < C::kAtoms; ++h) tc_cp_scales_lo(t_sfx + d * C::kSfCols + 4 * h, x_atom + (d * C::kAtoms + h) * (kAtomBytes >> 4));
+        }
+        tc_commit(smem_u32(&bar_sf[slot]));
       }
       __syncwarp();
-      if (++s == C::kStages) { s = 0; ph ^= 1u; }
+      if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+      if (++set == kSfSets) { set = 0; set_ph ^= 1u; }
     }
     if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[1]));
   } else if (warp == 3) {
-    // ------------------------------------------------ token scales: lane l writes the atom's 16 bytes of rows l, l + 32, l + 64, l + 96
-    constexpr int kRows = (BM + 31) / 32, kAhead = 4;
-    const int per_row = a.k / 32;
-    const bool words = (per_row & 3) == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 3) == 0;
-    uint32_t now[kAhead][kRows], next[kAhead][kRows];
-    const auto fetch = [&](int kt, uint32_t (&v)[kAhead][kRows]) {
+    // ------------------------------------------------ scale producer: lane l writes an atom's 16 bytes of rows l, l + 32, l + 64, l + 96.
+    // A group's bytes are asked for as soon as those of the group before it are stored.
+    constexpr int kRows = (BM + 31) / 32;
+    const int alignment = scale_alignment(a.scales, a.k);
+    uint4 v[kRows];
+    const auto fetch = [&](int kt) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-        for (int i = 0; i < kRows; ++i)
-          v[j][i] = kt + j < kt1 && (BM >= 32 || lane < BM) ? row_scales(a.scales, row0 + 32 * i + lane, a.m, kt + j, per_row, words) : 0u;
+      for (int i = 0; i < kRows; ++i) v[i] = BM >= 32 || lane < BM ? row_scales(a.scales, row0 + 32 * i + lane, a.m, kt, a.k, alignment) : uint4{};
     };
-    uint32_t s = 0, ph = 1u;
+    const uint8_t* w_src = a.atoms + (static_cast<int64_t>(tile) * a.tiles_k + kt0) * kAtomBytes;
+    uint32_t slot = 0, ph = 1u, it = 0;
     bool ok = true;
-    fetch(kt0, now);
-    for (int kt = kt0; kt < kt1 && ok; kt += kAhead) {
-      if (kt + kAhead < kt1) fetch(kt + kAhead, next);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (kt + j >= kt1 || !ok) break;
-        if (!warp_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
-#pragma unroll
-        for (int h = 0; h < C::kAtoms; ++h) {
-          uint4* cell = reinterpret_cast<uint4*>(smem_raw + (tiles - smem_u32(smem_raw)) + C::kSfOff + (s * C::kAtoms + h) * kAtomBytes) + lane;
-          *cell = make_uint4(now[j][4 * h], kRows > 1 ? now[j][(4 * h + 1) % kRows] : 0u, kRows > 2 ? now[j][(4 * h + 2) % kRows] : 0u,
-                             kRows > 2 ? now[j][(4 * h + 3) % kRows] : 0u);
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_xs[s]));
-        if (++s == C::kStages) { s = 0; ph ^= 1u; }
+    fetch(kt0);
+    for (int kt = kt0; kt < kt1; kt += kSfGroup, w_src += kSfGroup * kAtomBytes) {
+      if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; break; }
+      const uint32_t sfull = smem_u32(&bar_sfull[slot]), at = C::kSfOff + slot * C::kSfSlotBytes;
+      if (lane == 0) {
+        const uint32_t bytes = (kt1 - kt < kSfGroup ? kt1 - kt : kSfGroup) * kAtomBytes;
+        mbar_arrive_expect_tx(sfull, bytes);
+        bulk_load(tiles + at, w_src, bytes, sfull);
       }
+      ++it;
+      uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at + kSfGroup * kAtomBytes) + lane;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
+      for (int d = 0; d < kSfGroup; ++d)
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) now[j][i] = next[j][i];
+        for (int h = 0; h < C::kAtoms; ++h)
+          cells[(d * C::kAtoms + h) * 32] = make_uint4(word_of(v[4 * h], d), kRows > 1 ? word_of(v[(4 * h + 1) % kRows], d) : 0u,
+                                                       kRows > 2 ? word_of(v[(4 * h + 2) % kRows], d) : 0u,
+                                                       kRows > 2 ? word_of(v[(4 * h + 3) % kRows], d) : 0u);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sfull);
+      if (kt + kSfGroup < kt1) fetch(kt + kSfGroup);
+      if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
     }
+    if (!ok && lane == 0) drain_copies(bar_sfull, it, C::kSfSlots);
   } else {
     // ------------------------------------------------ the part: lane = weight row, column = token. All copies have landed and all MMAs have
     // read them (the last commit), so the ring's memory is free.
     const int q = warp & 3;
-    float* mine = reinterpret_cast<float*>(smem_raw + (tiles - smem_u32(smem_raw))) + q * 32 + lane;
+    float* mine = reinterpret_cast<float*>(tiles_ptr) + q * 32 + lane;
     if (__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull), 0, abort_v, status))) {
       tc_fence_after();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16);

@@ -18,9 +18,9 @@ MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
 
 @dataclass
 class LinearWeights:
-    """A weight [rows, k] in the kernels' layout, built once by ``from_row_major`` before graph capture. ``tiles`` u8 [row tiles, K-tiles,
-    16896]: records of 128 rows x 128 K-elements of E4M3 codes in the 128-byte-swizzled shared-memory image, then the tile's scale
-    atom. ``bias`` fp32 [rows] or None."""
+    """A weight [rows, k] in the kernels' layout, built once by ``from_row_major`` before graph capture. ``tiles`` u8: [row tile][K-tile]
+    images of 128 rows x 128 K-elements of E4M3 codes as the 128-byte swizzle lays them in shared memory, then the tiles' scale
+    atoms. ``bias`` fp32 [rows] or None."""
     tiles: torch.Tensor
     bias: torch.Tensor | None
     rows: int
@@ -64,7 +64,7 @@ class LinearWeights:
         codes, scales = w.contiguous().view(torch.uint8), scale.contiguous().view(torch.uint8)
         if codes.data_ptr() & 15:
             codes = codes.clone()
-        tiles = torch.empty((-(-rows // 128), -(-k // 128), nbytes // (-(-rows // 128) * -(-k // 128))), dtype=torch.uint8, device=w.device)
+        tiles = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
         launch_on(w.device, _lib.load().b200moe_preshuffle_linear,
                   (codes.data_ptr(), scales.data_ptr(), rows, k, int(gated), tiles.data_ptr()), "preshuffle_linear")
         return cls(tiles, bias, rows, k, bool(gated))

@@ -444,8 +444,8 @@ int b200moe_add_rmsnorm_quant(const void* x_bf16, int64_t x_stride, const void* 
 #define B200MOE_ACT_SWIGLU_OAI 6
 
 /* Weights: row-major E4M3 codes [rows][k] (16-byte aligned) and E8M0 scales [rows][k/32] -> tiles, b200moe_linear_weight_bytes bytes
- * (0: a shape that is not taken), 128-byte aligned. Layout: [row tile of 128][K-tile of 128] records of 16384 bytes of codes in the
- * 128-byte-swizzled image and one scale atom; what is beyond the matrix is zero; gated rows interleaved [gate 32 | up 32] twice a tile. */
+ * (0: a shape that is not taken), 128-byte aligned. Layout: [row tile of 128][K-tile of 128] images of 16384 bytes of codes (128-byte
+ * swizzle), then [row tile][K-tile] scale atoms; what is beyond the matrix is zero; gated rows interleaved [gate 32 | up 32] twice a tile. */
 size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated);
 int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated, uint8_t* tiles,
                               void* stream);
