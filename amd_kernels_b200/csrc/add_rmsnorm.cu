@@ -111,24 +111,24 @@ static size_t span_bytes(int64_t n, int64_t width, int64_t stride, int size) {
 
 }  // namespace b200moe
 
-extern "C" int b200moe_add_rmsnorm_quant(const void* x_bf16, int64_t x_stride, const void* residual_bf16, int64_t residual_stride,
-                                         const void* weight_bf16, float weight_offset, float eps, int64_t rows, int64_t h,
-                                         void* residual_out_bf16, int64_t residual_out_stride, void* normed_bf16,
-                                         int64_t normed_stride, uint8_t* codes8, uint8_t* scales8, void* stream) {
+extern "C" int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* stream) {
   using namespace b200moe;
+  if (!call) return B200MOE_E_ARG;
+  const b200moe_norm_call& c = *call;
+  const int64_t rows = c.rows, h = c.h;
   if (rows < 0 || h < 32 || h > B200MOE_NORM_MAX_H || h % 32) return B200MOE_E_ARG;
   if (rows == 0) return 0;
-  if (!x_bf16 || !weight_bf16) return B200MOE_E_ARG;
-  if ((codes8 != nullptr) != (scales8 != nullptr) || (residual_out_bf16 && !residual_bf16)) return B200MOE_E_ARG;
-  if (!residual_out_bf16 && !normed_bf16 && !codes8) return B200MOE_E_ARG;
+  if (!c.x || !c.weight) return B200MOE_E_ARG;
+  if ((c.codes8 != nullptr) != (c.scales8 != nullptr) || (c.residual_out && !c.residual)) return B200MOE_E_ARG;
+  if (!c.residual_out && !c.normed && !c.codes8) return B200MOE_E_ARG;
   struct Rows { const void* p; int64_t stride, width; int size; bool out; };
-  const Rows all[] = {{x_bf16, x_stride, h, 2, false},
-                      {residual_bf16, residual_stride, h, 2, false},
-                      {residual_out_bf16, residual_out_stride, h, 2, true},
-                      {normed_bf16, normed_stride, h, 2, true},
-                      {codes8, h, h, 1, true},
-                      {scales8, h / 32, h / 32, 1, true},
-                      {weight_bf16, h, h, 2, false}};
+  const Rows all[] = {{c.x, c.x_stride, h, 2, false},
+                      {c.residual, c.residual_stride, h, 2, false},
+                      {c.residual_out, c.residual_out_stride, h, 2, true},
+                      {c.normed, c.normed_stride, h, 2, true},
+                      {c.codes8, h, h, 1, true},
+                      {c.scales8, h / 32, h / 32, 1, true},
+                      {c.weight, h, h, 2, false}};
   constexpr int kAll = sizeof(all) / sizeof(all[0]);
   for (int i = 0; i < kAll; ++i) {
     const Rows& r = all[i];
@@ -149,22 +149,22 @@ extern "C" int b200moe_add_rmsnorm_quant(const void* x_bf16, int64_t x_stride, c
     }
   }
   NormArgs a;
-  a.x = static_cast<const uint4*>(x_bf16);
-  a.residual = static_cast<const uint4*>(residual_bf16);
-  a.weight = static_cast<const uint4*>(weight_bf16);
-  a.residual_out = static_cast<uint4*>(residual_out_bf16);
-  a.normed = static_cast<uint4*>(normed_bf16);
-  a.codes8 = reinterpret_cast<uint2*>(codes8);
-  a.scales8 = scales8;
-  a.x_stride = x_stride / 8;
-  a.residual_stride = residual_stride / 8;
-  a.residual_out_stride = residual_out_stride / 8;
-  a.normed_stride = normed_stride / 8;
+  a.x = static_cast<const uint4*>(c.x);
+  a.residual = static_cast<const uint4*>(c.residual);
+  a.weight = static_cast<const uint4*>(c.weight);
+  a.residual_out = static_cast<uint4*>(c.residual_out);
+  a.normed = static_cast<uint4*>(c.normed);
+  a.codes8 = reinterpret_cast<uint2*>(c.codes8);
+  a.scales8 = c.scales8;
+  a.x_stride = c.x_stride / 8;
+  a.residual_stride = c.residual_stride / 8;
+  a.residual_out_stride = c.residual_out_stride / 8;
+  a.normed_stride = c.normed_stride / 8;
   a.rows = rows;
   a.vectors = static_cast<int>(h / 8);
   a.h = static_cast<float>(h);
-  a.offset = weight_offset;
-  a.eps = eps;
+  a.offset = c.weight_offset;
+  a.eps = c.eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int v = a.vectors;
   const auto threads = [v](int per_thread) { return ((v + per_thread - 1) / per_thread + 31) / 32 * 32; };

@@ -145,60 +145,65 @@ extern "C" int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t
 
 namespace b200moe {
 // Checks a call and fills the kernels' arguments; a.m is 0 where there is nothing to do.
-static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
-                       int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
-                       uint8_t* out_codes8, uint8_t* out_scales8, const int32_t* status) {
+static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const b200moe_linear_call* call, const int32_t* status) {
   a.m = 0;
-  if (!w || m < 0 || m > B200MOE_LINEAR_MAX_ROWS) return B200MOE_E_ARG;
-  if (!linear_dims(w->rows, w->k, w->gated) || activation < B200MOE_ACT_NONE || activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
-  if ((w->gated != 0) != (activation >= B200MOE_ACT_SWIGLU)) return B200MOE_E_ARG;
+  if (!w || !call) return B200MOE_E_ARG;
+  const b200moe_linear_call& c = *call;
+  const int64_t m = c.m;
+  if (m < 0 || m > B200MOE_LINEAR_MAX_ROWS || !linear_dims(w->rows, w->k, w->gated)) return B200MOE_E_ARG;
+  if (c.activation < B200MOE_ACT_NONE || c.activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
+  if ((w->gated != 0) != (c.activation >= B200MOE_ACT_SWIGLU)) return B200MOE_E_ARG;
   if (m == 0) return 0;
-  if (!w->tiles || !codes8 || !scales8 || !status) return B200MOE_E_ARG;
-  if ((out_bf16 != nullptr) == (out_codes8 != nullptr) || (out_codes8 != nullptr) != (out_scales8 != nullptr)) return B200MOE_E_ARG;
+  if (!w->tiles || !c.codes8 || !c.scales8 || !status) return B200MOE_E_ARG;
+  if ((c.out != nullptr) == (c.out_codes8 != nullptr) || (c.out_codes8 != nullptr) != (c.out_scales8 != nullptr)) return B200MOE_E_ARG;
   const int64_t n = w->gated ? w->rows / 2 : w->rows;
-  if (out_codes8 && n % 32) return B200MOE_E_ARG;
-  if (m > 1 && ((out_bf16 && out_stride < n) || (residual_bf16 && residual_stride < n && residual_stride != 0))) return B200MOE_E_ARG;
-  if (misaligned(w->tiles, 128) || misaligned(codes8, 16) || misaligned(out_bf16, 16) || misaligned(out_codes8, 16) ||
-      misaligned(residual_bf16, 16) || misaligned(w->bias, 16) || (m > 1 && ((out_bf16 && (out_stride & 7)) || (residual_bf16 && (residual_stride & 7)))))
+  if (c.out_codes8 && n % 32) return B200MOE_E_ARG;
+  const auto bad_stride = [m](const void* p, int64_t stride, int64_t width, bool shared) {
+    return p && m > 1 && stride < width && !(shared && stride == 0);
+  };
+  if (bad_stride(c.out, c.out_stride, n, false) || bad_stride(c.residual, c.residual_stride, n, true)) return B200MOE_E_ARG;
+  const auto bad_rows = [m](const void* p, int64_t stride) { return misaligned(p, 16) || (p && m > 1 && (stride & 7)); };
+  if (misaligned(w->tiles, 128) || misaligned(w->bias, 16) || misaligned(c.codes8, 16) || misaligned(c.out_codes8, 16) ||
+      bad_rows(c.out, c.out_stride) || bad_rows(c.residual, c.residual_stride))
     return B200MOE_E_ALIGN;
   // the rows of out may be those of the residual (a thread stores where it has loaded); any other overlap with an input is refused
-  const void* outs[3] = {out_bf16, out_codes8, out_scales8};
-  const size_t out_bytes[3] = {((m - 1) * static_cast<size_t>(out_stride) + n) * 2, static_cast<size_t>(m) * n, static_cast<size_t>(m) * (n / 32)};
-  const size_t res_bytes = ((m - 1) * static_cast<size_t>(residual_stride) + n) * 2;
+  const void* outs[3] = {c.out, c.out_codes8, c.out_scales8};
+  const size_t rows = static_cast<size_t>(m);
+  const size_t out_bytes[3] = {((rows - 1) * c.out_stride + n) * 2, rows * n, rows * (n / 32)};
+  const size_t res_bytes = ((rows - 1) * c.residual_stride + n) * 2;
   for (int i = 0; i < 3; ++i) {
-    if (overlap(outs[i], out_bytes[i], codes8, static_cast<size_t>(m) * w->k) || overlap(outs[i], out_bytes[i], scales8, static_cast<size_t>(m) * (w->k / 32)))
+    if (overlap(outs[i], out_bytes[i], c.codes8, rows * w->k) || overlap(outs[i], out_bytes[i], c.scales8, rows * (w->k / 32)))
       return B200MOE_E_ARG;
-    const bool same = i == 0 && out_bf16 == residual_bf16 && (m == 1 || out_stride == residual_stride);
-    if (!same && overlap(outs[i], out_bytes[i], residual_bf16, res_bytes)) return B200MOE_E_ARG;
+    const bool same = i == 0 && c.out == c.residual && (m == 1 || c.out_stride == c.residual_stride);
+    if (!same && overlap(outs[i], out_bytes[i], c.residual, res_bytes)) return B200MOE_E_ARG;
   }
-  if (overlap(out_codes8, out_bytes[1], out_scales8, out_bytes[2])) return B200MOE_E_ARG;
+  if (overlap(c.out_codes8, out_bytes[1], c.out_scales8, out_bytes[2])) return B200MOE_E_ARG;
   a.tiles = w->tiles;
   a.bias = w->bias;
-  a.codes = codes8;
-  a.scales = scales8;
-  a.residual = static_cast<const __nv_bfloat16*>(residual_bf16);
-  a.out = static_cast<__nv_bfloat16*>(out_bf16);
-  a.out_codes = out_codes8;
-  a.out_scales = out_scales8;
+  a.codes = c.codes8;
+  a.scales = c.scales8;
+  a.residual = static_cast<const __nv_bfloat16*>(c.residual);
+  a.out = static_cast<__nv_bfloat16*>(c.out);
+  a.out_codes = c.out_codes8;
+  a.out_scales = c.out_scales8;
   a.m = m;
-  a.residual_stride = residual_stride;
-  a.out_stride = out_stride;
+  a.residual_stride = c.residual_stride;
+  a.out_stride = c.out_stride;
   a.k = static_cast<int>(w->k);
   a.n = static_cast<int>(n);
   a.tiles_n = static_cast<int>(linear_row_tiles(w->rows));
   a.tiles_k = static_cast<int>(linear_k_tiles(w->k));
   a.atoms = w->tiles + static_cast<int64_t>(a.tiles_n) * a.tiles_k * kLinearImageBytes;
-  a.act = act_args(activation);
+  a.act = act_args(c.activation);
   return 0;
 }
 }  // namespace b200moe
 
-extern "C" int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m,
-                              int activation, const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride,
-                              uint8_t* out_codes8, uint8_t* out_scales8, int32_t* status, void* stream) {
+extern "C" int b200moe_linear(const b200moe_linear_weights* w, const b200moe_linear_call* call, int32_t* status, void* stream) {
   using namespace b200moe;
   LinearArgs a;
-  const int r = linear_args(a, w, codes8, scales8, m, activation, residual_bf16, residual_stride, out_bf16, out_stride, out_codes8,
-                            out_scales8, status);
-  return r || a.m == 0 ? r : dispatch_linear(a, status, static_cast<cudaStream_t>(stream));
+  int r = linear_args(a, w, call, status);
+  if (r || a.m == 0) return r;
+  if (call->x && (r = b200moe_quant_mxfp8(call->x, call->x_stride, call->m, w->k, call->codes8, call->scales8, stream))) return r;
+  return dispatch_linear(a, status, static_cast<cudaStream_t>(stream));
 }

@@ -90,30 +90,50 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// How rows of scales begin: at multiples of 16 bytes (K a multiple of 512), of 4 (of 128), or anywhere.
-__device__ __forceinline__ int scale_alignment(const uint8_t* scales, int k) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(k / 32);
-  return (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
-}
-// The scale bytes of K-tiles kt .. kt + 3 of a row, 4 a K-tile; 0 beyond the rows and the columns
-__device__ __forceinline__ uint4 row_scales(const uint8_t* scales, int64_t row, int64_t rows, int kt, int k, int alignment) {
-  uint32_t v[4] = {0u, 0u, 0u, 0u};
-  const int per_row = k / 32;
-  if (row < rows) {
-    const uint8_t* p = scales + row * per_row + kt * 4;
+// The row-major scales of the tokens. `alignment`: rows begin at multiples of 16 bytes (K a multiple of 512), of 4 (of 128), or anywhere.
+struct RowScales {
+  const uint8_t* base;
+  int64_t rows;
+  int per_row, alignment;
+  __device__ __forceinline__ RowScales(const uint8_t* scales, int64_t m, int k) : base(scales), rows(m), per_row(k / 32) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(per_row);
+    alignment = (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
+  }
+  // The four bytes from the aligned address p on, those outside the array as zeros.
+  __device__ __forceinline__ uint32_t word(const uint8_t* p) const {
+    const uint8_t* end = base + rows * per_row;
+    if (p >= base && p + 4 <= end) return __ldcg(reinterpret_cast<const uint32_t*>(p));
+    uint32_t v = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (p + j >= base && p + j < end) v |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * j);
+    return v;
+  }
+  // The bytes of K-tiles kt .. kt + 3 of a row, 4 a K-tile; 0 beyond the rows and the columns
+  __device__ __forceinline__ uint4 at(int64_t row, int kt) const {
+    if (row >= rows) return make_uint4(0u, 0u, 0u, 0u);
+    const uint8_t* p = base + row * per_row + kt * 4;
     if (alignment == 16 && (kt & 3) == 0) return __ldcg(reinterpret_cast<const uint4*>(p));  // (16 bytes divide the row)
+    uint32_t v[4] = {0u, 0u, 0u, 0u};
+    const int left = per_row - kt * 4;  // bytes of the row from p on
     if (alignment >= 4) {
 #pragma unroll
       for (int d = 0; d < 4; ++d)
-        if ((kt + d) * 4 < per_row) v[d] = __ldcg(reinterpret_cast<const uint32_t*>(p) + d);
-    } else {
+        if (4 * d < left) v[d] = __ldcg(reinterpret_cast<const uint32_t*>(p) + d);
+    } else {  // aligned words, shifted
+      const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+      uint32_t w[5];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (kt * 4 + j < per_row) v[j >> 2] |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * (j & 3));
+      for (int d = 0; d < 5; ++d) w[d] = 4 * d - shift < left ? word(p - shift + 4 * d) : 0u;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        v[d] = __funnelshift_r(w[d], w[d + 1], 8 * shift);
+        if (left < 4 * d + 4) v[d] &= left <= 4 * d ? 0u : 0xffffffffu >> (8 * (4 * d + 4 - left));  // the next row's bytes
+      }
     }
+    return make_uint4(v[0], v[1], v[2], v[3]);
   }
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
+};
 __device__ __forceinline__ uint32_t word_of(const uint4 v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
 
 // 32 bytes, one sector, by one thread (32-byte aligned)

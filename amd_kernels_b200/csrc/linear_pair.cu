@@ -8,11 +8,11 @@
 //
 //   warp 0      code producer (both CTAs): TMA of the CTA's 128 token rows and of its weight rows, counted on the leader's barrier
 //   warp 1      tensor memory (both CTAs); in the leader it issues the MMAs for both, the whole warp around one elected lane
-//   warp 2      leader: copies the scales into tensor memory in both CTAs, in the same way
+//   warp 2      leader: copies the scales into tensor memory in both CTAs, in the same way; partner: tells the leader of its token scales
 //   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
 //   warps 4-11  epilogue (both CTAs): thread = one token row, 64 * NT columns. The sums are pulled into registers and the accumulator
 //               is handed back; then bias, activation, residual and one rounding, 32 columns at a time, stored as 32-byte sectors
-// 12 warps start with 168 registers; the issuing warpgroup drops to 72, the epilogue's rise to 216 (4 x 72 + 8 x 216 = 12 x 168: the
+// 12 warps start with 168 registers; the issuing warpgroup drops to 88, the epilogue's rise to 208 (4 x 88 + 8 x 208 = 12 x 168: the
 // exchange must balance inside what the CTA was given at launch).
 #include "linear.cuh"
 #include "tc_pair.cuh"
@@ -47,8 +47,9 @@ __device__ __forceinline__ void tc_mma_mxf8_two(uint32_t d, uint32_t a_lo, uint3
       : "memory");
 }
 
-// Arrival on a barrier of another CTA of the cluster that orders this thread's (and, behind a __syncwarp, its warp's) shared-memory
-// writes before it, and the wait that sees them.
+// Arrival on a barrier of another CTA of the cluster that orders what this thread has seen before it, and the wait that sees it. The
+// arrival waits for everything that its thread has in flight, so a thread without loads does it for the scale warp, whose own arrival is
+// local: with the scale warp arriving itself a group of K-tiles took 3400 cycles instead of 2300 (8192 rows 256 -> 219 us).
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -86,6 +87,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   __shared__ __align__(8) uint64_t bar_empty[C::kStages];    // in each CTA: the MMAs that read the stage have completed
   __shared__ __align__(8) uint64_t bar_sfull[C::kSfSlots];      // leader: both CTAs' scales of the group are there
   __shared__ __align__(8) uint64_t bar_sf[C::kSfSlots];         // in each CTA: they have been copied to tensor memory
+  __shared__ __align__(8) uint64_t bar_relay[C::kSfSlots];   // partner: its token scales of the group are in its shared memory
   __shared__ __align__(8) uint64_t bar_set[kSfSets];         // leader: the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull[C::kAccs];      // in each CTA: the unit's accumulator is complete
   __shared__ __align__(8) uint64_t bar_tempty[C::kAccs];     // leader: both CTAs' epilogues have read it
@@ -111,6 +113,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     for (int j = 0; j < C::kSfSlots; ++j) {
       mbar_init(smem_u32(&bar_sfull[j]), 3);  // the leader's byte count, the token scales of both CTAs
       mbar_init(smem_u32(&bar_sf[j]), 1);
+      mbar_init(smem_u32(&bar_relay[j]), 1);
     }
     for (int i = 0; i < C::kAccs; ++i) {
       mbar_init(smem_u32(&bar_tfull[i]), 1);
@@ -145,7 +148,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
 
   // The issuing warpgroup and the two epilogue warpgroups do not meet again before the kernel's last lines.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
       // ---------------------------------------------------------------- code producer (both CTAs)
       if (lane == 0) {
@@ -172,43 +175,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       }
     } else if (warp == 3) {
       // ---------------------------------------------------------------- scales (both CTAs): lane l writes 16 bytes of a token atom, rows l,
-      // l + 32, l + 64 and l + 96. A group's bytes are asked for as soon as those of the group before it are stored.
+      // l + 32, l + 64 and l + 96. A group's bytes are asked for two groups ahead.
       const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
-      const int alignment = scale_alignment(a.scales, a.k);
-      uint4 v[4];
-      const auto fetch = [&](int u, int kt) {
-        units.at(u, pair, step);
+      const RowScales scales(a.scales, a.m, a.k);
+      uint4 even[4], odd[4];
+      int fu = cluster, fkt = 0;  // the group that is asked for next
+      const auto fetch = [&](uint4 (&v)[4]) {
+        if (fu >= total) return;
+        units.at(fu, pair, step);
         const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + lane;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = row_scales(a.scales, row + 32 * i, a.m, kt, a.k, alignment);
+        for (int i = 0; i < 4; ++i) v[i] = scales.at(row + 32 * i, fkt);
+        if ((fkt += kSfGroup) >= tiles_k) fkt = 0, fu += n_clusters;
       };
       uint32_t it = 0, slot = 0, ph = 1u;
+      int u = cluster, kt = 0;  // the group that is stored next
       bool ok = true;
-      if (cluster < total) fetch(cluster, 0);
-      for (int u = cluster; u < total && ok; u += n_clusters) {
-        units.at(u, pair, step);
-        int atom = NT * step * tiles_k * 4;  // the atoms seen as rows of 128 bytes
-        for (int kt = 0; kt < tiles_k; kt += kSfGroup, atom += kSfGroup * 4) {
-          // free once its previous contents are in tensor memory
-          if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; break; }
-          const uint32_t sfull = sfull0 + 8u * slot, at = C::kSfOff + slot * C::kSfSlotBytes;
-          if (lane == 0) {
-            if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 2 * NT * kSfGroup * kAtomBytes);
-            // (a last group of fewer K-tiles brings the next tile's atoms or zeros along, which nothing reads)
-            tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
-            if (NT == 2) tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
-          }
-          ++it;
-          uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at) + lane;
-#pragma unroll
-          for (int d = 0; d < kSfGroup; ++d) cells[d * 32] = make_uint4(word_of(v[0], d), word_of(v[1], d), word_of(v[2], d), word_of(v[3], d));
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_release_cluster(sfull);
-          if (kt + kSfGroup < tiles_k) fetch(u, kt + kSfGroup);
-          else if (u + n_clusters < total) fetch(u + n_clusters, 0);
-          if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+      const auto group = [&](uint4 (&v)[4]) {
+        if (u >= total || !ok) return;
+        // free once its previous contents are in tensor memory
+        if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; return; }
+        const uint32_t sfull = sfull0 + 8u * slot, at = C::kSfOff + slot * C::kSfSlotBytes;
+        if (lane == 0) {
+          units.at(u, pair, step);
+          const int atom = (NT * step * tiles_k + kt) * 4;  // the atoms seen as rows of 128 bytes
+          if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 2 * NT * kSfGroup * kAtomBytes);
+          // (a last group of fewer K-tiles brings the next tile's atoms or zeros along, which nothing reads)
+          tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
+          if (NT == 2) tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
         }
+        ++it;
+        uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at) + lane;
+#pragma unroll
+        for (int d = 0; d < kSfGroup; ++d) cells[d * 32] = make_uint4(word_of(v[0], d), word_of(v[1], d), word_of(v[2], d), word_of(v[3], d));
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(leader ? smem_u32(&bar_sfull[slot]) : smem_u32(&bar_relay[slot]));
+        fetch(v);
+        if ((kt += kSfGroup) >= tiles_k) kt = 0, u += n_clusters;
+        if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+      };
+      fetch(even);
+      fetch(odd);
+      while (u < total && ok) {
+        group(even);
+        group(odd);
       }
       if (!ok && leader && lane == 0) drain_copies(bar_sfull, it, C::kSfSlots);
     } else if (warp == 1) {
@@ -283,11 +294,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
           }
         }
         if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05_pair(smem_u32(&bar_drain[1]));
+      } else if (lane == 0) {
+        // -------------------------------------------------------------- the partner's token atoms are told to the leader
+        const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
+        uint32_t slot = 0, ph = 0;
+        bool ok = true;
+        for (int u = cluster; u < total && ok; u += n_clusters) {
+          for (int kt = 0; kt < tiles_k; kt += kSfGroup) {
+            if (!mbar_wait(smem_u32(&bar_relay[slot]), ph, abort_v, status)) { ok = false; break; }
+            mbar_arrive_release_cluster(sfull0 + 8u * slot);
+            if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+          }
+        }
       }
     }
   } else {
     // ---------------------------------------------------------------- epilogue (both CTAs, warps 4..11)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     constexpr int kParts = C::kCols / 32;                       // accumulator pieces of 32 columns
     constexpr int kOuts = KIND == kGated ? kParts / 2 : kParts; // pieces of 32 output columns
     const int q = warp & 3;                  // the TMEM lane quarter this warp may read

@@ -23,7 +23,7 @@ struct LinearCfg {
   static constexpr int kStageBytes = kTokOff + BM * 128;
   static constexpr int kCtasPerSm = BM > 128 ? 1 : 2;                        // two: one's start and end under the other's stream
   static constexpr int kStages = BM > 128 ? 4 : BM > 64 ? 3 : BM > 32 ? 4 : 5;
-  static constexpr int kSfSlots = 2;                                         // groups of scales in shared memory
+  static constexpr int kSfSlots = BM == 32 ? 2 : 3;                          // groups of scales in shared memory
   static constexpr int kSfOff = kStages * kStageBytes;
   static constexpr int kSfTileBytes = (1 + kAtoms) * kAtomBytes;             // a K-tile's scales in a slot: see below
   static constexpr int kSfSlotBytes = kSfGroup * kSfTileBytes;               // weight atoms of the group, then token atoms by K-tile
@@ -254,25 +254,24 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[1]));
   } else if (warp == 3) {
     // ------------------------------------------------ scale producer: lane l writes an atom's 16 bytes of rows l, l + 32, l + 64, l + 96.
-    // A group's bytes are asked for as soon as those of the group before it are stored.
+    // A group's bytes are asked for two groups ahead.
     constexpr int kRows = (BM + 31) / 32;
-    const int alignment = scale_alignment(a.scales, a.k);
-    uint4 v[kRows];
-    const auto fetch = [&](int kt) {
+    const RowScales scales(a.scales, a.m, a.k);
+    uint4 even[kRows], odd[kRows];
+    const auto fetch = [&](int kt, uint4 (&v)[kRows]) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) v[i] = BM >= 32 || lane < BM ? row_scales(a.scales, row0 + 32 * i + lane, a.m, kt, a.k, alignment) : uint4{};
+      for (int i = 0; i < kRows; ++i) v[i] = kt < kt1 && (BM >= 32 || lane < BM) ? scales.at(row0 + 32 * i + lane, kt) : uint4{};
     };
-    const uint8_t* w_src = a.atoms + (static_cast<int64_t>(tile) * a.tiles_k + kt0) * kAtomBytes;
     uint32_t slot = 0, ph = 1u, it = 0;
     bool ok = true;
-    fetch(kt0);
-    for (int kt = kt0; kt < kt1; kt += kSfGroup, w_src += kSfGroup * kAtomBytes) {
-      if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; break; }
+    const auto group = [&](int kt, uint4 (&v)[kRows]) {
+      if (kt >= kt1 || !ok) return;
+      if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; return; }
       const uint32_t sfull = smem_u32(&bar_sfull[slot]), at = C::kSfOff + slot * C::kSfSlotBytes;
       if (lane == 0) {
         const uint32_t bytes = (kt1 - kt < kSfGroup ? kt1 - kt : kSfGroup) * kAtomBytes;
         mbar_arrive_expect_tx(sfull, bytes);
-        bulk_load(tiles + at, w_src, bytes, sfull);
+        bulk_load(tiles + at, a.atoms + (static_cast<int64_t>(tile) * a.tiles_k + kt) * kAtomBytes, bytes, sfull);
       }
       ++it;
       uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at + kSfGroup * kAtomBytes) + lane;
@@ -286,8 +285,14 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(sfull);
-      if (kt + kSfGroup < kt1) fetch(kt + kSfGroup);
+      fetch(kt + 2 * kSfGroup, v);
       if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
+    };
+    fetch(kt0, even);
+    fetch(kt0 + kSfGroup, odd);
+    for (int kt = kt0; kt < kt1 && ok; kt += 2 * kSfGroup) {
+      group(kt, even);
+      group(kt + kSfGroup, odd);
     }
     if (!ok && lane == 0) drain_copies(bar_sfull, it, C::kSfSlots);
   } else {

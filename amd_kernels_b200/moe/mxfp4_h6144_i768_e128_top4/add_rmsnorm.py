@@ -6,20 +6,45 @@ from __future__ import annotations
 import torch
 
 from ... import _lib
-from .chain import _raw_stream
 from .tail import TailOutput
 
 MAX_H = 65536
+_BF16 = torch.bfloat16
 
 
-def _rows(name, t, m, h, dev, shared_row=False):
-    """Checks bf16 rows [m, h] with unit column stride and 16-byte aligned rows; their stride in elements."""
-    if t.dtype != torch.bfloat16 or t.shape != (m, h) or t.stride(1) != 1 or t.device != dev:
-        raise ValueError(f"{name}: expected BF16 [{m}, {h}] with unit stride along the row, on {dev}")
-    stride = t.stride(0)
+def rows_of(name, t, m, h, dev, shared_row=False):
+    """Checks bf16 rows [m, h] with unit column stride, a multiple of 8 elements apart; that distance."""
+    if t.dtype is not _BF16 or t.shape != (m, h) or t.device != dev:
+        raise ValueError(f"{name}: expected BF16 [{m}, {h}] on {dev}")
+    stride, unit = t.stride()
+    if unit != 1:
+        raise ValueError(f"{name}: expected unit stride along the row")
     if m > 1 and (stride & 7 or (stride < h and not (shared_row and stride == 0))):
         raise ValueError(f"{name}: rows {stride} elements apart (needs a multiple of 8, at least {h})")
     return stride
+
+
+def check_mxfp8(name, codes, scales, m, width, dev):
+    """Contiguous [m, width] and [m, width / 32] of one byte each (uint8, or float8 of the two formats)."""
+    if codes is None or scales is None:
+        raise ValueError(f"{name}: codes and scales come together")
+    if (codes.element_size() != 1 or codes.shape != (m, width) or not codes.is_contiguous() or codes.device != dev
+            or scales.element_size() != 1 or scales.shape != (m, width // 32) or not scales.is_contiguous() or scales.device != dev):
+        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] and scales [{m}, {width // 32}] of one byte each on {dev}")
+
+
+def launch_on(dev, call, *args):
+    """``call(*args, stream)`` on the current stream of ``dev``, which is made the current device where it is not. A device that is no
+    CUDA device is a ValueError."""
+    if dev.type != "cuda":
+        raise ValueError(f"expected tensors on a CUDA device, got {dev}")
+    if dev.index == torch._C._cuda_getDevice():
+        code = call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            code = call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if code:
+        _lib.check(code, call.__name__)
 
 
 def add_rmsnorm_mxfp8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6, *,
@@ -31,61 +56,41 @@ def add_rmsnorm_mxfp8(x: torch.Tensor, residual: torch.Tensor | None, weight: to
 
     ``x`` and ``residual`` bf16 [M, H], rows any multiple of 8 elements apart; M may be 0. ``residual`` None: ``s = x``, and no residual
     comes back. A residual expanded from one row (stride 0) is added to every row. ``out``: where the results go; its tensors
-    that are not None say what is computed (``mxfp8`` and ``bf16_out`` are not read). Its ``residual`` may be ``residual`` or ``x``
-    itself, its ``normed`` ``x``; codes and scales are contiguous. A row's bits depend on nothing but the row."""
+    that are not None say what is computed (``mxfp8`` and ``bf16_out`` are not read). Its ``residual`` and ``normed`` may be ``x`` or
+    ``residual`` itself; codes and scales are contiguous. A row's bits depend on nothing but the row."""
     if x.ndim != 2 or weight.ndim != 1:
         raise ValueError("expected BF16 [M, H] rows and a [H] weight")
-    (m, h), dev = x.shape, x.device
+    m, h = x.shape
+    dev = x.device
     if h < 32 or h % 32 or h > MAX_H:
         raise ValueError(f"rows of {h} columns (needs a multiple of 32, up to {MAX_H})")
-    xs = _rows("x", x, m, h, dev)
-    rs = 0 if residual is None else _rows("residual", residual, m, h, dev, shared_row=True)
-    if weight.dtype != torch.bfloat16 or weight.shape[0] != h or not weight.is_contiguous() or weight.device != dev:
+    xs = rows_of("x", x, m, h, dev)
+    rs = 0 if residual is None else rows_of("residual", residual, m, h, dev, True)
+    if weight.dtype is not _BF16 or weight.shape != (h,) or not weight.is_contiguous() or weight.device != dev:
         raise ValueError(f"weight: expected contiguous BF16 [{h}] on {dev}")
     ros = ns = h
     if out is None:
         empty = torch.empty
-        out = TailOutput(None if residual is None else empty((m, h), dtype=torch.bfloat16, device=dev),
+        out = TailOutput(None if residual is None else empty((m, h), dtype=_BF16, device=dev),
                          empty((m, h), dtype=torch.uint8, device=dev) if mxfp8 else None,
                          empty((m, h // 32), dtype=torch.uint8, device=dev) if mxfp8 else None,
-                         empty((m, h), dtype=torch.bfloat16, device=dev) if bf16_out else None)
-        if residual is None and not mxfp8 and not bf16_out:
-            raise ValueError("no output asked for")
+                         empty((m, h), dtype=_BF16, device=dev) if bf16_out else None)
+        ro, codes, scales, normed = out.residual, out.codes, out.scales, out.normed
     else:
-        if out.residual is not None:
+        ro, codes, scales, normed = out.residual, out.codes, out.scales, out.normed
+        if ro is not None:
             if residual is None:
                 raise ValueError("out.residual without a residual")
-            ros = _rows("out.residual", out.residual, m, h, dev)
-        if out.normed is not None:
-            ns = _rows("out.normed", out.normed, m, h, dev)
-        if out.codes is not None or out.scales is not None:
-            check_mxfp8("out", out.codes, out.scales, m, h, dev)
-        if out.residual is None and out.normed is None and out.codes is None:
-            raise ValueError("no output asked for")
-    call = _lib.load().b200moe_add_rmsnorm_quant
-    args = (x.data_ptr(), xs, None if residual is None else residual.data_ptr(), rs, weight.data_ptr(), weight_offset, eps, m, h,
-            None if out.residual is None else out.residual.data_ptr(), ros, None if out.normed is None else out.normed.data_ptr(), ns,
-            None if out.codes is None else out.codes.data_ptr(), None if out.scales is None else out.scales.data_ptr())
-    launch_on(dev, call, args, "add_rmsnorm_quant")
+            ros = rows_of("out.residual", ro, m, h, dev)
+        if normed is not None:
+            ns = rows_of("out.normed", normed, m, h, dev)
+        if codes is not None or scales is not None:
+            check_mxfp8("out", codes, scales, m, h, dev)
+    if ro is None and normed is None and codes is None:
+        raise ValueError("no output asked for")
+    call = _lib.NORM_CALL.pack(x.data_ptr(), xs, 0 if residual is None else residual.data_ptr(), rs, weight.data_ptr(),
+                               0 if ro is None else ro.data_ptr(), ros, 0 if normed is None else normed.data_ptr(), ns,
+                               0 if codes is None else codes.data_ptr(), 0 if scales is None else scales.data_ptr(), m, h,
+                               weight_offset, eps)
+    launch_on(dev, _lib.load().b200moe_add_rmsnorm_quant, call)
     return out
-
-
-def check_mxfp8(name, codes, scales, m, width, dev):
-    """Contiguous uint8 (or float8 of the two formats) [m, width], [m, width / 32]."""
-    if codes is None or scales is None:
-        raise ValueError(f"{name}: codes and scales come together")
-    if (codes.element_size() != 1 or codes.shape != (m, width) or not codes.is_contiguous() or codes.device != dev
-            or scales.element_size() != 1 or scales.shape != (m, width // 32) or not scales.is_contiguous() or scales.device != dev):
-        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] and scales [{m}, {width // 32}] of one byte each on {dev}")
-
-
-def launch_on(dev, call, args, what):
-    """``call(*args, stream)`` on the current stream of ``dev``, which is made the current device where it is not."""
-    stream = _raw_stream(dev)
-    if dev.index == torch.cuda.current_device():
-        code = call(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            code = call(*args, stream)
-    if code:
-        _lib.check(code, what)

@@ -4,13 +4,12 @@ rows, added to the residual stream if asked, or MXFP8 rows for the next product.
 on both sides, fp32 accumulation; the shared expert (``SharedWeights``) is two such products of fixed shape."""
 from __future__ import annotations
 
-import ctypes
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 
 from ... import _lib
-from .add_rmsnorm import _rows, check_mxfp8, launch_on
+from .add_rmsnorm import check_mxfp8, launch_on, rows_of
 from .chain import status_word
 
 MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
@@ -26,19 +25,15 @@ class LinearWeights:
     rows: int
     k: int
     gated: bool
-    _abi: object = field(default=None, repr=False, compare=False)
 
     @property
     def n(self) -> int:
         """Output columns."""
         return self.rows // 2 if self.gated else self.rows
 
-    def abi(self) -> _lib.LinearWeights:
+    def abi(self) -> bytes:
         """``struct b200moe_linear_weights`` over this object's tensors as they are now."""
-        a, bias = self._abi, None if self.bias is None else self.bias.data_ptr()
-        if a is None or a.tiles != self.tiles.data_ptr() or a.bias != bias:
-            a = self._abi = _lib.LinearWeights(self.tiles.data_ptr(), bias, self.rows, self.k, int(self.gated))
-        return a
+        return _lib.LINEAR_WEIGHTS.pack(self.tiles.data_ptr(), 0 if self.bias is None else self.bias.data_ptr(), self.rows, self.k, self.gated)
 
     @classmethod
     def from_row_major(cls, w, scale, bias=None, *, gated: bool = False):
@@ -65,8 +60,8 @@ class LinearWeights:
         if codes.data_ptr() & 15:
             codes = codes.clone()
         tiles = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-        launch_on(w.device, _lib.load().b200moe_preshuffle_linear,
-                  (codes.data_ptr(), scales.data_ptr(), rows, k, int(gated), tiles.data_ptr()), "preshuffle_linear")
+        launch_on(w.device, _lib.load().b200moe_preshuffle_linear, codes.data_ptr(), scales.data_ptr(), rows, k, int(gated),
+                  tiles.data_ptr())
         return cls(tiles, bias, rows, k, bool(gated))
 
 
@@ -75,15 +70,16 @@ def mxfp8_quant(x: torch.Tensor, *, out=None):
     (the same bits at 6144; an infinite value saturates and keeps its block's scale finite). Rows any multiple of 8 elements apart."""
     if x.ndim != 2:
         raise ValueError("expected BF16 [M, K]")
-    (m, k), dev = x.shape, x.device
+    m, k = x.shape
+    dev = x.device
     if k < 32 or k % 32 or k > MAX_DIM or m > MAX_ROWS:
         raise ValueError(f"rows of {k} columns (needs a multiple of 32, up to {MAX_DIM}; up to {MAX_ROWS} rows)")
-    stride = _rows("x", x, m, k, dev, shared_row=True)
+    stride = rows_of("x", x, m, k, dev, True)
     if out is None:
         out = torch.empty((m, k), dtype=torch.uint8, device=dev), torch.empty((m, k // 32), dtype=torch.uint8, device=dev)
     else:
         check_mxfp8("out", *out, m, k, dev)
-    launch_on(dev, _lib.load().b200moe_quant_mxfp8, (x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr()), "quant_mxfp8")
+    launch_on(dev, _lib.load().b200moe_quant_mxfp8, x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr())
     return out
 
 
@@ -103,37 +99,38 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
     if (act >= 5) != w.gated:
         raise ValueError(f"activation {activation!r} on {'gated' if w.gated else 'plain'} weights")
     k, n, dev = w.k, w.n, w.tiles.device
-    pair = isinstance(x, (tuple, list))
-    if not pair and not isinstance(x, torch.Tensor):
-        raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
-    rows = x[0] if pair else x
-    if rows.ndim != 2 or rows.shape[1] != k:
-        raise ValueError(f"expected rows of {k} columns")
-    m = rows.shape[0]
-    if m > MAX_ROWS:
-        raise ValueError(f"more than {MAX_ROWS} rows")
-    if rows.device != dev or dev.type != "cuda":
-        raise ValueError(f"x is on {rows.device}, the weights on {dev}: expected one CUDA device")
-    if pair:
+    if dev.type != "cuda":
+        raise ValueError(f"expected weights on a CUDA device, got {dev}")
+    xs = x_at = 0
+    if isinstance(x, torch.Tensor):
+        if x.ndim != 2:
+            raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
+        m = x.shape[0]
+        xs, x_at = rows_of("x", x, m, k, dev, True), x.data_ptr()
+        rows8 = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=dev)  # the quantised rows
+        c_at = rows8.data_ptr()
+        s_at = c_at + m * k
+    elif isinstance(x, (tuple, list)) and len(x) == 2 and x[0] is not None and x[0].ndim == 2:
         codes, scales = x
+        m = codes.shape[0]
         check_mxfp8("x", codes, scales, m, k, dev)
+        c_at, s_at = codes.data_ptr(), scales.data_ptr()
     else:
-        codes, scales = mxfp8_quant(x)
-    rs = 0 if residual is None else _rows("residual", residual, m, n, dev, shared_row=True)
-    os, oc, osc = n, None, None
+        raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
+    rs = 0 if residual is None else rows_of("residual", residual, m, n, dev, True)
+    os, y, oc, osc = n, 0, 0, 0
     if out is None:
         if mxfp8_out:
             out = torch.empty((m, n), dtype=torch.uint8, device=dev), torch.empty((m, n // 32), dtype=torch.uint8, device=dev)
         else:
             out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
     if isinstance(out, torch.Tensor):
-        os, y = _rows("out", out, m, n, dev), out.data_ptr()
+        os, y = rows_of("out", out, m, n, dev), out.data_ptr()
     else:
         if n % 32:
             raise ValueError(f"MXFP8 output of {n} columns (needs a multiple of 32)")
         check_mxfp8("out", *out, m, n, dev)
-        y, oc, osc = None, out[0].data_ptr(), out[1].data_ptr()
-    launch_on(dev, _lib.load().b200moe_linear,
-              (ctypes.byref(w.abi()), codes.data_ptr(), scales.data_ptr(), m, act, None if residual is None else residual.data_ptr(), rs,
-               y, os, oc, osc, status_word(dev).data_ptr()), "linear")
+        oc, osc = out[0].data_ptr(), out[1].data_ptr()
+    call = _lib.LINEAR_CALL.pack(x_at, xs, c_at, s_at, m, 0 if residual is None else residual.data_ptr(), rs, y, os, oc, osc, act)
+    launch_on(dev, _lib.load().b200moe_linear, w.abi(), call, status_word(dev).data_ptr())
     return out

@@ -420,10 +420,22 @@ int b200moe_forward_x(const b200moe_weights* w, const void* x_bf16, int64_t toke
  * B200MOE_NORM_MAX_H. residual_out or normed may be x or residual (the same address and stride); any other overlap of an output is
  * B200MOE_E_ARG. The bits of a row do not depend on the other rows. rows may be 0. */
 #define B200MOE_NORM_MAX_H 65536
-int b200moe_add_rmsnorm_quant(const void* x_bf16, int64_t x_stride, const void* residual_bf16, int64_t residual_stride,
-                              const void* weight_bf16, float weight_offset, float eps, int64_t rows, int64_t h,
-                              void* residual_out_bf16, int64_t residual_out_stride, void* normed_bf16, int64_t normed_stride,
-                              uint8_t* codes8, uint8_t* scales8, void* stream);
+typedef struct b200moe_norm_call {
+  const void* x;
+  int64_t x_stride;
+  const void* residual; /* or null */
+  int64_t residual_stride;
+  const void* weight;
+  void* residual_out; /* or null */
+  int64_t residual_out_stride;
+  void* normed; /* or null */
+  int64_t normed_stride;
+  uint8_t* codes8; /* both or neither */
+  uint8_t* scales8;
+  int64_t rows, h;
+  float weight_offset, eps;
+} b200moe_norm_call;
+int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* stream);
 
 /* The MXFP8 matrix product with its epilogue, any shape: what reads the rows of the tail and of the norm above (the next
  * projection), and the dense SwiGLU blocks around MoE layers.
@@ -461,12 +473,25 @@ typedef struct b200moe_linear_weights {
   int gated;
 } b200moe_linear_weights;
 
-/* codes8 16-byte aligned; residual and out are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a residual stride of
- * 0 is one row for all). Either out or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the residual (same
- * address and stride); any other overlap of an output with an input is B200MOE_E_ARG. No workspace, one launch. m may be 0. */
-int b200moe_linear(const b200moe_linear_weights* w, const uint8_t* codes8, const uint8_t* scales8, int64_t m, int activation,
-                   const void* residual_bf16, int64_t residual_stride, void* out_bf16, int64_t out_stride, uint8_t* out_codes8,
-                   uint8_t* out_scales8, int32_t* status, void* stream);
+/* x: codes8 (16-byte aligned) and scales8; or bf16 rows x (16-byte aligned), which are first quantised into codes8 and scales8 by a launch
+ * in front (b200moe_quant_mxfp8). residual, out and x are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a stride of 0
+ * of residual or x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
+ * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG. m may be 0. */
+typedef struct b200moe_linear_call {
+  const void* x; /* or null */
+  int64_t x_stride;
+  uint8_t* codes8;
+  uint8_t* scales8;
+  int64_t m;
+  const void* residual; /* or null */
+  int64_t residual_stride;
+  void* out;
+  int64_t out_stride;
+  uint8_t* out_codes8;
+  uint8_t* out_scales8;
+  int activation;
+} b200moe_linear_call;
+int b200moe_linear(const b200moe_linear_weights* w, const b200moe_linear_call* call, int32_t* status, void* stream);
 
 /* The whole layer in one call, with or without the shared expert (MOE/chain.py:127-197 mxfp4_moe; the shared expert runs
  * beside the routed experts inside the same launches up to 512 tokens; above, its two GEMMs are launches of their own, on

@@ -23,7 +23,8 @@ def test_both_packages_have_them():
 
 # ------------------------------------------------------------------------------------------------ the norm
 def norm_call(lib, x=4096, xs=64, r=1 << 20, rs=64, w=256, rows=4, h=64, ro=2 << 20, ros=64, n=3 << 20, ns=64, c=4 << 20, s=5 << 20):
-    return lib.b200moe_add_rmsnorm_quant(at(x), xs, at(r), rs, at(w), 1.0, 1e-6, rows, h, at(ro), ros, at(n), ns, at(c), at(s), None)
+    p = [0 if a is None else a for a in (x, r, w, ro, n, c, s)]
+    return lib.b200moe_add_rmsnorm_quant(_lib.NORM_CALL.pack(p[0], xs, p[1], rs, p[2], p[3], ros, p[4], ns, p[5], p[6], rows, h, 1.0, 1e-6), None)
 
 
 @pytest.mark.parametrize("inter", [768, 1536])
@@ -71,9 +72,10 @@ def weights(rows=64, k=96, gated=False, bias=False):
 
 
 def linear_call(lib, rows=64, k=96, gated=0, tiles=256, bias=None, c=1 << 20, s=2 << 20, m=4, act=0, r=None, rs=64, o=3 << 20, os=64,
-                oc=None, osc=None, status=256):
-    w = _lib.LinearWeights(tiles, bias, rows, k, gated)
-    return lib.b200moe_linear(ctypes.byref(w), at(c), at(s), m, act, at(r), rs, at(o), os, at(oc), at(osc), at(status), None)
+                oc=None, osc=None, status=256, x=None, xs=96):
+    p = [0 if a is None else a for a in (tiles, bias, c, s, r, o, oc, osc)]
+    return lib.b200moe_linear(_lib.LINEAR_WEIGHTS.pack(p[0], p[1], rows, k, gated),
+                              _lib.LINEAR_CALL.pack(0 if x is None else x, xs, p[2], p[3], m, p[4], rs, p[5], os, p[6], p[7], act), at(status), None)
 
 
 @pytest.mark.parametrize("inter", [768, 1536])
@@ -94,6 +96,7 @@ def test_c_abi_refuses_product_arguments(inter):
                 dict(o=None, oc=1 << 20, osc=5 << 20), dict(o=None, oc=4 << 20, osc=(4 << 20) + 100), dict(o=None, oc=4 << 20, osc=2 << 20),
                 dict(o=None, oc=4 << 20, osc=5 << 20, r=4 << 20)):
         assert linear_call(lib, **bad) == A, bad
+    assert linear_call(lib, x=(6 << 20) + 8) == L_ and linear_call(lib, x=6 << 20, xs=100) == L_ and linear_call(lib, x=6 << 20, xs=88) == A
     assert linear_call(lib, m=0, c=None, s=None, o=None) == 0
     for rows, k, gated, want in ((64, 96, 0, 16896), (136, 160, 0, 4 * 16896), (64, 32, 1, 16896), (192, 128, 1, 2 * 16896), (64, 40, 0, 0),
                                  (60, 96, 0, 0), (96, 96, 1, 0), (1 << 20, 1 << 20, 0, 0)):
@@ -139,8 +142,7 @@ def test_weights_refuse_bad_tensors():
 
 def test_layout_and_struct():
     w = weights(bias=True)
-    a = w.abi()
-    assert (a.tiles, a.bias, a.rows, a.k, a.gated) == (w.tiles.data_ptr(), w.bias.data_ptr(), 64, 96, 0) and w.abi() is a
-    w.bias = torch.ones(64)
-    assert w.abi().bias == w.bias.data_ptr()
+    assert w.abi() == _lib.LINEAR_WEIGHTS.pack(w.tiles.data_ptr(), w.bias.data_ptr(), 64, 96, 0)
+    w.bias = None
+    assert w.abi() == _lib.LINEAR_WEIGHTS.pack(w.tiles.data_ptr(), 0, 64, 96, 0)
     assert weights(gated=True).n == 32 and L.MAX_DIM == 1 << 20
