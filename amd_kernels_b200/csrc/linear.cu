@@ -158,10 +158,7 @@ static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const b20
   if ((c.out != nullptr) == (c.out_codes8 != nullptr) || (c.out_codes8 != nullptr) != (c.out_scales8 != nullptr)) return B200MOE_E_ARG;
   const int64_t n = w->gated ? w->rows / 2 : w->rows;
   if (c.out_codes8 && n % 32) return B200MOE_E_ARG;
-  const auto bad_stride = [m](const void* p, int64_t stride, int64_t width, bool shared) {
-    return p && m > 1 && stride < width && !(shared && stride == 0);
-  };
-  if (bad_stride(c.out, c.out_stride, n, false) || bad_stride(c.residual, c.residual_stride, n, true)) return B200MOE_E_ARG;
+  if (m > 1 && ((c.out && c.out_stride < n) || (c.residual && c.residual_stride < n))) return B200MOE_E_ARG;
   const auto bad_rows = [m](const void* p, int64_t stride) { return misaligned(p, 16) || (p && m > 1 && (stride & 7)); };
   if (misaligned(w->tiles, 128) || misaligned(w->bias, 16) || misaligned(c.codes8, 16) || misaligned(c.out_codes8, 16) ||
       bad_rows(c.out, c.out_stride) || bad_rows(c.residual, c.residual_stride))

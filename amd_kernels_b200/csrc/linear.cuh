@@ -17,7 +17,7 @@ constexpr int kLinearTileBytes = kLinearImageBytes + kAtomBytes;
 constexpr int kSfGroup = 4, kSfSets = 2;
 
 // What the epilogue does with a sum p (or a gate g and an up u):
-//   kLinear   p, or 0 where p < floor (ReLU: 0, none: -inf)
+//   kLinear   max(p, floor) (ReLU: 0, none: -inf)
 //   kSigmoid  p * sigmoid(c1 p + c3 p^3): SiLU, and GELU in its tanh form, 0.5 (1 + tanh(v)) = sigmoid(2 v)
 //   kGelu     p * Phi(p)
 //   kGated    min(g, top) * sigmoid(c1 min(g, top)) * (clamp(u, -top, top) + beta)
@@ -43,37 +43,94 @@ struct LinearArgs {
   LinearAct act;
 };
 
-// NaN passes every clamp here (the comparison is false), as it does in the formulas
-__device__ __forceinline__ float act_linear(float p, const LinearAct& a) { return p < a.floor ? 0.0f : p; }
-__device__ __forceinline__ float act_sigmoid(float p, const LinearAct& a) {
-  const float v = p * fmaf(a.c3, fminf(p * p, 1e30f), a.c1);  // (bounded: 0 * inf is NaN)
-  return __fdividef(p, 1.0f + __expf(-v));
+// Two fp32 values an instruction (add, mul and fma of f32x2, each half rounded as the scalar one): the epilogues of wide products are
+// bound by instructions, and by fetching them.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t f2_bits(F2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_of(uint64_t r) {
+  F2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ F2 f2_dup(float v) { return {v, v}; }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 f2_exp2(F2 a) {  // 2^a, within 2 units in the last place
+  F2 r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_rcp(F2 a) {  // 1 / a, within 1 unit in the last place; 0 for infinity
+  F2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN stays, as in the formulas
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950409f;
+// p * sigmoid(v), v given as -v log2(e)
+__device__ __forceinline__ F2 f2_times_sigmoid(F2 p, F2 w) { return p * f2_rcp(f2_exp2(w) + f2_dup(1.0f)); }
+
+__device__ __forceinline__ F2 act_linear(F2 p, const LinearAct& a) { return {max_nan(p.x, a.floor), max_nan(p.y, a.floor)}; }
+__device__ __forceinline__ F2 act_sigmoid(F2 p, const LinearAct& a) {
+  if (a.c3 == 0.0f) return f2_times_sigmoid(p, p * f2_dup(-kLog2e * a.c1));
+  return f2_times_sigmoid(p, p * f2_fma(p * p, f2_dup(-kLog2e * a.c3), f2_dup(-kLog2e * a.c1)));
 }
 // Phi(p) = erfc(-p / sqrt(2)) / 2. erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0: the Chebyshev fit of Numerical Recipes
-// (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision; a third of the
-// instructions of normcdff.
-__device__ __forceinline__ float act_gelu(float p) {
-  const float z = fabsf(p) * 0.70710678f, t = __fdividef(1.0f, fmaf(0.5f, z, 1.0f));
-  float q = 0.17087277f;
-  q = fmaf(q, t, -0.82215223f);
-  q = fmaf(q, t, 1.48851587f);
-  q = fmaf(q, t, -1.13520398f);
-  q = fmaf(q, t, 0.27886807f);
-  q = fmaf(q, t, -0.18628806f);
-  q = fmaf(q, t, 0.09678418f);
-  q = fmaf(q, t, 0.37409196f);
-  q = fmaf(q, t, 1.00002368f);
-  q = fmaf(q, t, -1.26551223f);
-  const float half = 0.5f * t * __expf(fmaf(-z, z, q));  // erfc(z) / 2
-  return p * (p < 0.0f ? half : 1.0f - half);
+// (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision.
+__device__ __forceinline__ F2 act_gelu(F2 p) {
+  const F2 z = F2{fabsf(p.x), fabsf(p.y)} * f2_dup(0.70710678f), t = f2_rcp(f2_fma(z, f2_dup(0.5f), f2_dup(1.0f)));
+  F2 q = f2_fma(t, f2_dup(0.17087277f), f2_dup(-0.82215223f));
+  q = f2_fma(q, t, f2_dup(1.48851587f));
+  q = f2_fma(q, t, f2_dup(-1.13520398f));
+  q = f2_fma(q, t, f2_dup(0.27886807f));
+  q = f2_fma(q, t, f2_dup(-0.18628806f));
+  q = f2_fma(q, t, f2_dup(0.09678418f));
+  q = f2_fma(q, t, f2_dup(0.37409196f));
+  q = f2_fma(q, t, f2_dup(1.00002368f));
+  q = f2_fma(q, t, f2_dup(-1.26551223f));
+  const F2 w = f2_fma(z * f2_dup(-1.0f), z, q) * f2_dup(kLog2e);
+  const F2 half = t * f2_dup(0.5f) * f2_exp2(w);  // erfc(z) / 2
+  const F2 other = f2_fma(half, f2_dup(-1.0f), f2_dup(1.0f));
+  return p * F2{p.x < 0.0f ? half.x : other.x, p.y < 0.0f ? half.y : other.y};
 }
-__device__ __forceinline__ float act_gated(float g, float u, const LinearAct& a) {
-  g = g > a.top ? a.top : g;
-  u = u > a.top ? a.top : u < -a.top ? -a.top : u;
-  return g * __fdividef(1.0f, 1.0f + __expf(-a.c1 * g)) * (u + a.beta);
+__device__ __forceinline__ F2 act_gated(F2 g, F2 u, const LinearAct& a) {
+  g = {min_nan(g.x, a.top), min_nan(g.y, a.top)};
+  u = {max_nan(min_nan(u.x, a.top), -a.top), max_nan(min_nan(u.y, a.top), -a.top)};
+  return f2_times_sigmoid(g, g * f2_dup(-kLog2e * a.c1)) * (u + f2_dup(a.beta));
 }
 template <int KIND>
-__device__ __forceinline__ float act_of(float p, const LinearAct& a) {
+__device__ __forceinline__ F2 act_of(F2 p, const LinearAct& a) {
   return KIND == kLinear ? act_linear(p, a) : KIND == kSigmoid ? act_sigmoid(p, a) : act_gelu(p);
 }
 

@@ -11,7 +11,10 @@
 //   warp 2      leader: copies the scales into tensor memory in both CTAs, in the same way; partner: tells the leader of its token scales
 //   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
 //   warps 4-11  epilogue (both CTAs): thread = one token row, 64 * NT columns. The sums are pulled into registers and the accumulator
-//               is handed back; then bias, activation, residual and one rounding, 32 columns at a time, stored as 32-byte sectors
+//               is handed back; then bias, activation, residual and one rounding, 32 columns at a time. bf16 rows go through a strip of
+//               shared memory per warp, 32 rows x 64 columns: the residual arrives there by TMA, the result leaves there by TMA. (A
+//               thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the operands of
+//               the MMAs wait: with them a residual made 16384 x 6144 -> 6144 28 % slower.)
 // 12 warps start with 168 registers; the issuing warpgroup drops to 88, the epilogue's rise to 208 (4 x 88 + 8 x 208 = 12 x 168: the
 // exchange must balance inside what the CTA was given at launch).
 #include "linear.cuh"
@@ -21,12 +24,14 @@ namespace b200moe {
 
 template <int NT>
 struct LinearPairCfg {
-  static constexpr int kStages = 6;                     // code ring
+  static constexpr int kStages = NT == 2 ? 5 : 6;       // code ring (NT = 2: 6 stages and no strips were 0 to 1 % faster, 4 were 5 % slower)
   static constexpr int kWRows = 64 * NT;                // weight rows of one CTA
   static constexpr int kWOff = 128 * 128;               // behind the CTA's 128 token rows
   static constexpr int kStageBytes = kWOff + kWRows * 128;
   static constexpr int kSfSlots = 3;                    // groups of scales in shared memory
-  static constexpr int kSfOff = kStages * kStageBytes;
+  static constexpr int kStripBytes = 32 * 128;          // one epilogue warp's rows x 64 bf16 columns, 128-byte swizzle
+  static constexpr int kStripOff = kStages * kStageBytes;
+  static constexpr int kSfOff = kStripOff + 8 * kStripBytes;
   static constexpr int kSfSlotBytes = kSfGroup * (1 + NT) * kAtomBytes;  // four token atoms, four atoms of each weight tile
   static constexpr int kBiasOff = kSfOff + kSfSlots * kSfSlotBytes;
   static constexpr int kCols = 64 * NT;                 // accumulator columns of an epilogue thread
@@ -77,10 +82,19 @@ struct LinearUnits {
   }
 };
 
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\ncp.async.bulk.commit_group;" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 template <int KIND, bool MX, int NT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_wc,
-                       const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ LinearArgs args, int32_t* status) {
+                       const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_res,
+                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LinearArgs args, int32_t* status) {
   using C = LinearPairCfg<NT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[C::kStages];     // leader: both CTAs' codes of the stage have landed
@@ -91,6 +105,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   __shared__ __align__(8) uint64_t bar_set[kSfSets];         // leader: the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull[C::kAccs];      // in each CTA: the unit's accumulator is complete
   __shared__ __align__(8) uint64_t bar_tempty[C::kAccs];     // leader: both CTAs' epilogues have read it
+  __shared__ __align__(8) uint64_t bar_res[8];               // an epilogue warp's residual has landed in its strip
   __shared__ __align__(8) uint64_t bar_drain[2];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
@@ -119,6 +134,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       mbar_init(smem_u32(&bar_tfull[i]), 1);
       mbar_init(smem_u32(&bar_tempty[i]), 16);  // one arrival per epilogue warp of both CTAs
     }
+    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&bar_res[i]), 1);
     mbar_init(smem_u32(&bar_drain[0]), 1);
     mbar_init(smem_u32(&bar_drain[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -317,16 +333,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     const int half = (warp >> 2) - 1;        // which half of the unit's columns
     const uint32_t tempty_leader = map_to_cta(smem_u32(&bar_tempty[0]), 0);
     float* const bias = reinterpret_cast<float*>(tiles_ptr + C::kBiasOff) + (warp - 4) * C::kCols;
+    constexpr bool kStore = !MX && kOuts >= 2;  // bf16 rows leave through the strip (a lone piece of 32 columns: directly)
     const bool wide = !MX ? (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (a.out_stride & 15) == 0
                           : (reinterpret_cast<uintptr_t>(a.out_codes) & 31) == 0;
-    uint32_t ui = 0;
+    const bool scale_words = (a.n & 127) == 0 && (reinterpret_cast<uintptr_t>(a.out_scales) & 3) == 0;
+    const uint32_t strip = tiles + C::kStripOff + (warp - 4) * C::kStripBytes;
+    uint8_t* const strip_row = tiles_ptr + C::kStripOff + (warp - 4) * C::kStripBytes + lane * 128;
+    const uint32_t res_bar = smem_u32(&bar_res[warp - 4]);
+    const bool residual = a.residual != nullptr;
+    // first token row and first output column of this warp's part of a unit
+    const auto place = [&](int v, int64_t& row, int& col) {
+      units.at(v, pair, step);
+      row = static_cast<int64_t>(pair) * 256 + rank * 128 + q * 32;
+      const int tile = NT == 2 ? 2 * step + half : step;
+      col = KIND == kGated ? tile * 64 + (NT == 1 ? 32 * half : 0) : tile * 128 + (NT == 1 ? 64 * half : 0);
+    };
+    // The residual of 64 columns (rows and columns beyond the matrix arrive as zeros); lane 0, once the strip is free.
+    const auto ask_residual = [&](int64_t row, int col) {
+      mbar_arrive_expect_tx(res_bar, C::kStripBytes);
+      tma_load_2d(strip, &map_res, col, static_cast<int>(row), res_bar);
+    };
+    uint32_t ui = 0, res_ph = 0;
+    int64_t row0;
+    int col0;
+    bool asked = false;
+    if (residual && cluster < total) {
+      place(cluster, row0, col0);
+      if (lane == 0) ask_residual(row0, col0);
+      asked = true;
+    }
     for (int u = cluster; u < total; u += n_clusters, ++ui) {
-      units.at(u, pair, step);
-      const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + q * 32 + lane;
+      place(u, row0, col0);
+      const int64_t row = row0 + lane;
       const bool in_row = row < a.m;
-      const int col_tile = NT == 2 ? 2 * step + half : step;
-      const int col0 = KIND == kGated ? col_tile * 64 + (NT == 1 ? 32 * half : 0) : col_tile * 128 + (NT == 1 ? 64 * half : 0);
-      // the bias in the order of the accumulator's columns; the residual's first columns
+      // the bias in the order of the accumulator's columns
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         const int col = col0 + 32 * (KIND == kGated ? i >> 1 : i) + lane;
@@ -334,15 +374,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
         bias[32 * i + lane] = a.bias != nullptr && col < a.n ? __ldcg(a.bias + from) : 0.0f;
       }
       __syncwarp();
-      uint4 res[2][4];
-      const auto load_residual = [&](int i, uint4 (&r)[4]) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int col = col0 + 32 * i + 8 * p;
-          r[p] = in_row && col < a.n ? __ldcg(reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col)) : uint4{};
-        }
-      };
-      if (a.residual != nullptr) load_residual(0, res[0]);
       const uint32_t acc_i = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
       // the warp decides together: tcgen05.ld below needs all 32 lanes
       if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull[acc_i]), aph, abort_v, status))) break;
@@ -355,49 +386,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * acc_i);
-#pragma unroll
+      // (a loop of one piece whose registers move up: unrolled, the code of a unit does not stay in the instruction cache)
+      uint32_t scale_bytes = 0;
+      bool ok = true;
+#pragma unroll 1
       for (int i = 0; i < kOuts; ++i) {
         const int col = col0 + 32 * i;
-        if (a.residual != nullptr && i + 1 < kOuts) load_residual(i + 1, res[(i + 1) & 1]);
-        float y[32];
+        F2 y[16];
 #pragma unroll
         for (int k4 = 0; k4 < 8; ++k4) {
-          const int part = KIND == kGated ? 2 * i : i;
-          const float4 b = *reinterpret_cast<const float4*>(bias + 32 * part + 4 * k4);
-          const float bb[4] = {b.x, b.y, b.z, b.w};
+          const float4 b = *reinterpret_cast<const float4*>(bias + 32 * (KIND == kGated ? 2 * i : i) + 4 * k4);
+          const F2 p0 = F2{__uint_as_float(acc[0][4 * k4]), __uint_as_float(acc[0][4 * k4 + 1])} + F2{b.x, b.y};
+          const F2 p1 = F2{__uint_as_float(acc[0][4 * k4 + 2]), __uint_as_float(acc[0][4 * k4 + 3])} + F2{b.z, b.w};
           if (KIND == kGated) {
-            const float4 bu = *reinterpret_cast<const float4*>(bias + 32 * (part + (KIND == kGated)) + 4 * k4);
-            const float bbu[4] = {bu.x, bu.y, bu.z, bu.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              y[4 * k4 + k] = act_gated(__uint_as_float(acc[part][4 * k4 + k]) + bb[k],
-                                        __uint_as_float(acc[part + (KIND == kGated)][4 * k4 + k]) + bbu[k], a.act);
+            constexpr int kUp = KIND == kGated ? 1 : 0;
+            const float4 bu = *reinterpret_cast<const float4*>(bias + 32 * (2 * i + 1) + 4 * k4);
+            const F2 u0 = F2{__uint_as_float(acc[kUp][4 * k4]), __uint_as_float(acc[kUp][4 * k4 + 1])} + F2{bu.x, bu.y};
+            const F2 u1 = F2{__uint_as_float(acc[kUp][4 * k4 + 2]), __uint_as_float(acc[kUp][4 * k4 + 3])} + F2{bu.z, bu.w};
+            y[2 * k4] = act_gated(p0, u0, a.act);
+            y[2 * k4 + 1] = act_gated(p1, u1, a.act);
           } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[4 * k4 + k] = act_of<KIND>(__uint_as_float(acc[part][4 * k4 + k]) + bb[k], a.act);
+            y[2 * k4] = act_of<KIND>(p0, a.act);
+            y[2 * k4 + 1] = act_of<KIND>(p1, a.act);
           }
         }
-        if (a.residual != nullptr) {
+        if (residual) {
+          if ((i & 1) == 0) {  // the next 64 columns
+            ok = __all_sync(0xffffffffu, mbar_wait(res_bar, res_ph, abort_v, status));
+            if (!ok) break;
+            res_ph ^= 1u;
+            asked = false;
+          }
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            const uint4 r = res[i & 1][p];
+            const uint4 r = *reinterpret_cast<const uint4*>(strip_row + (((4 * (i & 1) + p) ^ (lane & 7)) << 4));
             const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              y[8 * p + 2 * k] += __uint_as_float(rr[k] << 16);
-              y[8 * p + 2 * k + 1] += __uint_as_float(rr[k] & 0xffff0000u);
-            }
+            for (int k = 0; k < 4; ++k)
+              y[4 * p + k] = y[4 * p + k] + F2{__uint_as_float(rr[k] << 16), __uint_as_float(rr[k] & 0xffff0000u)};
           }
         }
         if (MX) {
           float amax = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) amax = fmaxf(amax, fabsf(y[k]));
+          for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fmaxf(fabsf(y[k].x), fabsf(y[k].y)));
           const int e = linear_scale(amax);
-          const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+          const F2 inv = f2_dup(e8m0_value(static_cast<uint32_t>(254 - e)));
           uint32_t w[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = pack_e4m3x4(y[4 * k] * inv, y[4 * k + 1] * inv, y[4 * k + 2] * inv, y[4 * k + 3] * inv);
+          for (int k = 0; k < 8; ++k) {
+            const F2 lo = y[2 * k] * inv, hi = y[2 * k + 1] * inv;
+            w[k] = pack_e4m3x4(lo.x, lo.y, hi.x, hi.y);
+          }
           if (in_row && col < a.n) {  // (n is a multiple of 32 here)
             uint8_t* o = a.out_codes + row * a.n + col;
             if (wide) {
@@ -406,14 +446,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
               reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
               reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
             }
-            a.out_scales[row * (a.n / 32) + col / 32] = static_cast<uint8_t>(e);
+            // four scales of a row are one store where they are one aligned word
+            if (!scale_words || kOuts < 4) {
+              a.out_scales[row * (a.n / 32) + col / 32] = static_cast<uint8_t>(e);
+            } else {
+              scale_bytes |= static_cast<uint32_t>(e) << (8 * i);
+              if (i == 3) *reinterpret_cast<uint32_t*>(a.out_scales + row * (a.n / 32) + col / 32 - 3) = scale_bytes;
+            }
           }
+        } else if (kStore) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            *reinterpret_cast<uint4*>(strip_row + (((4 * (i & 1) + p) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16x2(y[4 * p].x, y[4 * p].y), pack_bf16x2(y[4 * p + 1].x, y[4 * p + 1].y),
+                           pack_bf16x2(y[4 * p + 2].x, y[4 * p + 2].y), pack_bf16x2(y[4 * p + 3].x, y[4 * p + 3].y));
         } else {
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             uint32_t w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(y[16 * p + 2 * k], y[16 * p + 2 * k + 1]);
+            for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(y[8 * p + k].x, y[8 * p + k].y);
             const int c = col + 16 * p;
             if (in_row && c < a.n) {
               __nv_bfloat16* o = a.out + row * a.out_stride + c;
@@ -426,8 +478,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
             }
           }
         }
+        if ((i & 1) || i == kOuts - 1) {  // 64 columns are done
+          if (kStore) fence_proxy_async();
+          __syncwarp();
+          const bool more = i + 1 < kOuts || u + n_clusters < total;
+          int64_t next_row = row0;
+          int next_col = col + 32;
+          if (residual && i + 1 >= kOuts && more) place(u + n_clusters, next_row, next_col);
+          if (lane == 0) {
+            if (kStore) {
+              // (what lies beyond the matrix is not written)
+              if (row0 < a.m && col - 32 < a.n) tma_store_2d(&map_out, col - 32, static_cast<int>(row0), strip);
+              tma_store_wait_read();
+            }
+            if (residual && more) ask_residual(next_row, next_col);
+          }
+          asked = residual && more;
+          __syncwarp();  // the strip is free
+        }
+        constexpr int kMove = KIND == kGated ? 2 : 1;
+#pragma unroll
+        for (int j = 0; j + kMove < kParts; ++j)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) acc[j][k] = acc[j + kMove][k];
       }
+      if (!ok) break;
       __syncwarp();  // all lanes have read this unit's bias
+    }
+    if (asked && lane == 0) {  // after an abort: the copy lands before the CTA gives up its shared memory
+      const uint64_t t0 = global_timer(), limit = wait_limit_ns();
+      while (!mbar_try_wait(res_bar, res_ph) && global_timer() - t0 < limit) {}
     }
   }
 
@@ -443,6 +523,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+// bf16 rows [m][n], `stride` elements apart, boxes of 64 columns x 32 rows, 128-byte swizzle; columns and rows beyond are zeros / unwritten
+static int make_rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t m, int64_t stride) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return B200MOE_E_DRIVER;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(m)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(m > 1 ? stride : n) * 2};
+  const cuuint32_t box[2] = {64, 32}, estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : B200MOE_E_DRIVER;
+}
+
 template <int KIND, bool MX, int NT>
 static int linear_pairs() {
   static std::mutex mu;
@@ -454,18 +547,20 @@ static int linear_pairs() {
 template <int KIND, bool MX, int NT>
 static int launch_linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   using C = LinearPairCfg<NT>;
-  CUtensorMap mx, mwc, mws;
+  CUtensorMap mx, mwc, mws, mres = {}, mout = {};
   const uint64_t n_tiles = static_cast<uint64_t>(a.tiles_n) * a.tiles_k;
   int r;
   if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), 128))) return r;
   if ((r = make_flat_map(&mwc, a.tiles, n_tiles * 128, C::kWRows))) return r;
   if ((r = make_flat_map(&mws, a.atoms, n_tiles * 4, kSfGroup * 4))) return r;
+  if (a.residual && (r = make_rows_map(&mres, a.residual, a.n, a.m, a.residual_stride))) return r;
+  if (a.out && (r = make_rows_map(&mout, a.out, a.n, a.m, a.out_stride))) return r;
   const int64_t units = (a.m + 255) / 256 * ((a.tiles_n + NT - 1) / NT);
   if (units > 0x7fffffff) return B200MOE_E_ARG;
   const int pairs = linear_pairs<KIND, MX, NT>();
   if (pairs <= 0) return B200MOE_E_DRIVER;
   return launch_pairs(linear_pair_kernel<KIND, MX, NT>, units < pairs ? static_cast<int>(units) : pairs, C::kThreads, C::kSmemBytes, stream,
-                      mx, mwc, mws, a, status);
+                      mx, mwc, mws, mres, mout, a, status);
 }
 
 template <int KIND, int NT>

@@ -65,7 +65,8 @@ __device__ __forceinline__ void finish_row(const LinearArgs& a, int64_t row, int
       const float2 bp = __ldcg(reinterpret_cast<const float2*>(a.bias + col)), bu = __ldcg(reinterpret_cast<const float2*>(a.bias + a.n + col));
       p.x += bp.x, p.y += bp.y, u.x += bu.x, u.y += bu.y;
     }
-    y[0] = act_gated(p.x, u.x, a.act), y[1] = act_gated(p.y, u.y, a.act), y[2] = y[3] = 0.0f;
+    const F2 v = act_gated(F2{p.x, p.y}, F2{u.x, u.y}, a.act);
+    y[0] = v.x, y[1] = v.y, y[2] = y[3] = 0.0f;
   } else {
     col = tile * 128 + lane * 4;
     cols = 4;
@@ -78,17 +79,11 @@ __device__ __forceinline__ void finish_row(const LinearArgs& a, int64_t row, int
       const float4 b = __ldcg(reinterpret_cast<const float4*>(a.bias + col));
       p.x += b.x, p.y += b.y, p.z += b.z, p.w += b.w;
     }
-    y[0] = p.x, y[1] = p.y, y[2] = p.z, y[3] = p.w;
-    if (a.act.kind == kLinear) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = act_of<kLinear>(y[j], a.act);
-    } else if (a.act.kind == kSigmoid) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = act_of<kSigmoid>(y[j], a.act);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = act_of<kGelu>(y[j], a.act);
-    }
+    F2 lo = {p.x, p.y}, hi = {p.z, p.w};
+    if (a.act.kind == kLinear) lo = act_of<kLinear>(lo, a.act), hi = act_of<kLinear>(hi, a.act);
+    else if (a.act.kind == kSigmoid) lo = act_of<kSigmoid>(lo, a.act), hi = act_of<kSigmoid>(hi, a.act);
+    else lo = act_of<kGelu>(lo, a.act), hi = act_of<kGelu>(hi, a.act);
+    y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
   }
   const bool in = col < a.n;  // (n is a multiple of 8: a lane's columns are all inside or all outside)
   if (a.residual != nullptr && in) {

@@ -89,8 +89,8 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
 
     ``x``: MXFP8 rows as a pair (codes [M, K], scales [M, K / 32]), or bf16 [M, K], which ``mxfp8_quant`` quantises first. M may be 0.
     ``activation``: None, "relu", "silu", "gelu" (exact), "gelu_tanh"; for gated weights "swiglu" (silu(gate) * up) or "swiglu_oai"
-    (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart (or one
-    expanded row). Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.
+    (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart.
+    Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.
     ``out``: where the result goes, a bf16 tensor or a pair (``mxfp8_out`` is then not read); a bf16 ``out`` may be the residual
     itself. The sums of one call repeat bit for bit; between calls of different M they may be split along K in another way."""
     act = _lib.ACTIVATIONS.get(activation)
@@ -117,7 +117,7 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
         c_at, s_at = codes.data_ptr(), scales.data_ptr()
     else:
         raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
-    rs = 0 if residual is None else rows_of("residual", residual, m, n, dev, True)
+    rs = 0 if residual is None else rows_of("residual", residual, m, n, dev)
     os, y, oc, osc = n, 0, 0, 0
     if out is None:
         if mxfp8_out:

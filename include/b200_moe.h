@@ -475,7 +475,7 @@ typedef struct b200moe_linear_weights {
 
 /* x: codes8 (16-byte aligned) and scales8; or bf16 rows x (16-byte aligned), which are first quantised into codes8 and scales8 by a launch
  * in front (b200moe_quant_mxfp8). residual, out and x are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a stride of 0
- * of residual or x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
+ * of x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
  * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG. m may be 0. */
 typedef struct b200moe_linear_call {
   const void* x; /* or null */

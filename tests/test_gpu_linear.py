@@ -180,8 +180,8 @@ def test_bf16_rows_strides_and_in_place(P, m, k, n):
     assert P.mxfp8_linear(q, weights, residual=view, out=view) is view
     keep[:m, 16:n + 16] = want
     assert torch.equal(stream, keep)
-    one = res[:1].expand(m, n)
-    assert torch.equal(P.mxfp8_linear(q, weights, residual=one), P.mxfp8_linear(q, weights, residual=one.contiguous()))
+    one = x[:1].expand(m, k)
+    assert torch.equal(P.mxfp8_linear(one, weights), P.mxfp8_linear(one.contiguous(), weights))
 
 
 @pytest.mark.parametrize("m,k", [(40, 800), (700, 6144), (130, 160)])

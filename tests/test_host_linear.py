@@ -85,7 +85,7 @@ def test_c_abi_refuses_product_arguments(inter):
     for bad in (dict(c=None), dict(s=None), dict(o=None), dict(status=None), dict(tiles=None), dict(m=-1), dict(m=(1 << 24) + 1), dict(k=0),
                 dict(k=40), dict(k=(1 << 20) + 32), dict(rows=0), dict(rows=60), dict(rows=(1 << 20) + 8), dict(act=7), dict(act=-1), dict(act=5),
                 dict(gated=1), dict(gated=1, act=3), dict(rows=32, gated=1, act=5), dict(oc=4 << 20), dict(o=None, oc=4 << 20),
-                dict(oc=4 << 20, osc=5 << 20), dict(rows=40, o=None, oc=4 << 20, osc=5 << 20), dict(os=56), dict(r=4 << 20, rs=8),
+                dict(oc=4 << 20, osc=5 << 20), dict(rows=40, o=None, oc=4 << 20, osc=5 << 20), dict(os=56), dict(r=4 << 20, rs=8), dict(r=4 << 20, rs=0),
                 dict(rows=1 << 20, k=1 << 20)):
         assert linear_call(lib, **bad) == A, bad
     for bad in (dict(tiles=272), dict(c=(1 << 20) + 8), dict(o=(3 << 20) + 8), dict(os=68), dict(r=(4 << 20) + 8), dict(r=4 << 20, rs=66),
@@ -121,7 +121,7 @@ def test_product_refuses_bad_tensors():
                      (((u8(4, 192)[:, ::2], u8(4, 3)), w), {}), (((bf(4, 96), u8(4, 3)), w), {}), (((u8(4, 96), None), w), {}),
                      ((bf(4, 64), w), {}), ((bf(96), w), {}), ((torch.zeros((4, 96)), w), {}), (("x", w), {}),
                      ((x, w), dict(residual=bf(4, 32))), ((x, w), dict(residual=bf(3, 64))), ((x, w), dict(residual=torch.zeros((4, 64)))),
-                     ((x, w), dict(residual=bf(4, 68)[:, :64])), ((x, w), dict(out=bf(4, 72))), ((x, w), dict(out=torch.zeros((4, 64)))),
+                     ((x, w), dict(residual=bf(4, 68)[:, :64])), ((x, w), dict(residual=bf(1, 64).expand(4, 64))), ((x, w), dict(out=bf(4, 72))), ((x, w), dict(out=torch.zeros((4, 64)))),
                      ((x, w), dict(out=bf(1, 64).expand(4, 64))), ((x, w), dict(out=(u8(4, 64), u8(4, 3)))), ((x, w), dict(out=(u8(4, 64), None))),
                      ((x, w), dict(out=(None, None))), ((x, weights(rows=40)), dict(mxfp8_out=True)),
                      ((x, w), dict(residual=bf(4, 64).to("meta"))), (((u8(4, 96).to("meta"), u8(4, 3).to("meta")), w), {}),
