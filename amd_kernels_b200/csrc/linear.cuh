@@ -147,51 +147,76 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// The row-major scales of the tokens. `alignment`: rows begin at multiples of 16 bytes (K a multiple of 512), of 4 (of 128), or anywhere.
+// The row-major scales of the tokens: the 16 bytes of K-tiles kt .. kt + 3 (4 a K-tile) of ROWS rows, 32 apart, a lane. Asked for by load(),
+// without a branch between the loads of one call, so that all of them are in flight together; put in order by tiles().
+// `alignment`: rows begin at multiples of 16 bytes (K a multiple of 512), of 4 (of 128), or anywhere. Anywhere, a row's bytes are in five
+// aligned words; those that reach over the ends of the array are not read, and the rows beside the ends are read by bytes.
 struct RowScales {
-  const uint8_t* base;
+  const uint8_t *base, *end;
   int64_t rows;
   int per_row, alignment;
-  __device__ __forceinline__ RowScales(const uint8_t* scales, int64_t m, int k) : base(scales), rows(m), per_row(k / 32) {
+  __device__ __forceinline__ RowScales(const uint8_t* scales, int64_t m, int k)
+      : base(scales), end(scales + m * (k / 32)), rows(m), per_row(k / 32) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(per_row);
     alignment = (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
   }
-  // The four bytes from the aligned address p on, those outside the array as zeros.
-  __device__ __forceinline__ uint32_t word(const uint8_t* p) const {
-    const uint8_t* end = base + rows * per_row;
-    if (p >= base && p + 4 <= end) return __ldcg(reinterpret_cast<const uint32_t*>(p));
-    uint32_t v = 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (p + j >= base && p + j < end) v |= static_cast<uint32_t>(__ldcg(p + j)) << (8 * j);
-    return v;
-  }
-  // The bytes of K-tiles kt .. kt + 3 of a row, 4 a K-tile; 0 beyond the rows and the columns
-  __device__ __forceinline__ uint4 at(int64_t row, int kt) const {
-    if (row >= rows) return make_uint4(0u, 0u, 0u, 0u);
+  template <int ROWS>
+  __device__ __forceinline__ void load(int64_t row, int kt, uint32_t (&w)[ROWS][5]) const {
     const uint8_t* p = base + row * per_row + kt * 4;
-    if (alignment == 16 && (kt & 3) == 0) return __ldcg(reinterpret_cast<const uint4*>(p));  // (16 bytes divide the row)
-    uint32_t v[4] = {0u, 0u, 0u, 0u};
-    const int left = per_row - kt * 4;  // bytes of the row from p on
-    if (alignment >= 4) {
+    const int64_t step = 32 * static_cast<int64_t>(per_row);
+    if (alignment == 16 && (kt & 3) == 0) {  // (16 bytes divide the row)
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-        if (4 * d < left) v[d] = __ldcg(reinterpret_cast<const uint32_t*>(p) + d);
-    } else {  // aligned words, shifted
-      const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
-      uint32_t w[5];
-#pragma unroll
-      for (int d = 0; d < 5; ++d) w[d] = 4 * d - shift < left ? word(p - shift + 4 * d) : 0u;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        v[d] = __funnelshift_r(w[d], w[d + 1], 8 * shift);
-        if (left < 4 * d + 4) v[d] &= left <= 4 * d ? 0u : 0xffffffffu >> (8 * (4 * d + 4 - left));  // the next row's bytes
+      for (int i = 0; i < ROWS; ++i) {
+        const uint4 v = row + 32 * i < rows ? __ldcg(reinterpret_cast<const uint4*>(p + i * step)) : make_uint4(0u, 0u, 0u, 0u);
+        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
       }
+    } else if (alignment >= 4) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          w[i][d] = row + 32 * i < rows && (kt + d) * 4 < per_row ? __ldcg(reinterpret_cast<const uint32_t*>(p + i * step) + d) : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const uint8_t* q = p + i * step - (reinterpret_cast<uintptr_t>(p + i * step) & 3);
+#pragma unroll
+        for (int d = 0; d < 5; ++d)
+          w[i][d] = row + 32 * i < rows && q + 4 * d >= base && q + 4 * d + 4 <= end ? __ldcg(reinterpret_cast<const uint32_t*>(q) + d) : 0u;
+      }
+    }
+  }
+  // one row by bytes: the four words of K-tiles kt .. kt + 3
+  __device__ __noinline__ uint4 by_bytes(int64_t row, int kt) const {
+    uint32_t v[4] = {0u, 0u, 0u, 0u};
+    for (int j = 0; j < 16 && kt * 4 + j < per_row; ++j) {
+      const uint32_t b = static_cast<uint32_t>(__ldcg(base + row * per_row + kt * 4 + j)) << (8 * (j & 3));
+      v[0] |= j < 4 ? b : 0u, v[1] |= j >= 4 && j < 8 ? b : 0u, v[2] |= j >= 8 && j < 12 ? b : 0u, v[3] |= j >= 12 ? b : 0u;
     }
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
+  // the loaded words -> w[i][d]: the four bytes of K-tile kt + d; 0 beyond the rows and the columns
+  template <int ROWS>
+  __device__ __forceinline__ void tiles(int64_t row, int kt, uint32_t (&w)[ROWS][5]) const {
+    if (alignment >= 4) return;
+    const int left = per_row - kt * 4;  // bytes of a row from K-tile kt on
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t r = row + 32 * i;
+      const uint8_t* p = base + r * per_row + kt * 4;
+      const int shift = 8 * static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        w[i][d] = __funnelshift_r(w[i][d], w[i][d + 1], shift);
+        if (left < 4 * d + 4) w[i][d] &= left <= 4 * d ? 0u : 0xffffffffu >> (8 * (4 * d + 4 - left));  // the next row's bytes
+      }
+      if (r < rows && (p - base < 4 || end - p < 20)) {
+        const uint4 v = by_bytes(r, kt);
+        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+      }
+    }
+  }
 };
-__device__ __forceinline__ uint32_t word_of(const uint4 v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
 
 // 32 bytes, one sector, by one thread (32-byte aligned)
 __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
@@ -199,6 +224,11 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
                "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
+
+// The code producer (warp 0) starts behind the scale producer's (warp 3) first requests: behind a full ring of codes of all SMs the scales
+// took 5000 cycles to come.
+__device__ __forceinline__ void scales_first_wait() { asm volatile("bar.sync 3, 64;" ::: "memory"); }
+__device__ __forceinline__ void scales_first_arrive() { asm volatile("bar.arrive 3, 64;" ::: "memory"); }
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

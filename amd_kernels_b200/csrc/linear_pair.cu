@@ -146,6 +146,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  const int n_clusters = static_cast<int>(gridDim.x >> 1), cluster = static_cast<int>(blockIdx.x >> 1);
+  const LinearUnits units = {static_cast<int>((args.m + 255) / 256), (args.tiles_n + NT - 1) / NT};
+  const int total = units.total(), tiles_k = args.tiles_k;
+  int pair, step;
+  // the first weights that this CTA will load, into L2 while the launch in front still runs
+  if (warp == 0 && lane == 0 && cluster < total) {
+    units.at(cluster, pair, step);
+    const int tile = NT == 2 ? 2 * step + static_cast<int>(rank) : step, n = tiles_k < 8 ? tiles_k : 8;
+    if (tile < args.tiles_n) {
+      const int64_t at = static_cast<int64_t>(tile) * tiles_k;
+      for (int kt = 0; kt < n; ++kt) l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
+      l2_prefetch_bulk(args.atoms + at * kAtomBytes, static_cast<uint32_t>(n) * kAtomBytes);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before anything signals across the pair
@@ -157,16 +171,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   launder(a.bias);
   launder(a.residual);
 
-  const int n_clusters = static_cast<int>(gridDim.x >> 1), cluster = static_cast<int>(blockIdx.x >> 1);
-  const LinearUnits units = {static_cast<int>((a.m + 255) / 256), (a.tiles_n + NT - 1) / NT};
-  const int total = units.total(), tiles_k = a.tiles_k;
-  int pair, step;
-
   // The issuing warpgroup and the two epilogue warpgroups do not meet again before the kernel's last lines.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
       // ---------------------------------------------------------------- code producer (both CTAs)
+      if (cluster < total) scales_first_wait();
       if (lane == 0) {
         const uint32_t full0 = map_to_cta(smem_u32(&bar_full[0]), 0);  // the leader's barriers, as seen from this CTA
         uint32_t it = 0, s = 0, ph = 1u;
@@ -194,36 +204,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       // l + 32, l + 64 and l + 96. A group's bytes are asked for two groups ahead.
       const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
       const RowScales scales(a.scales, a.m, a.k);
-      uint4 even[4], odd[4];
+      uint32_t even[4][5] = {}, odd[4][5] = {};
       int fu = cluster, fkt = 0;  // the group that is asked for next
-      const auto fetch = [&](uint4 (&v)[4]) {
+      const auto fetch = [&](uint32_t (&v)[4][5]) {
         if (fu >= total) return;
         units.at(fu, pair, step);
-        const int64_t row = static_cast<int64_t>(pair) * 256 + rank * 128 + lane;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = scales.at(row + 32 * i, fkt);
+        scales.load(static_cast<int64_t>(pair) * 256 + rank * 128 + lane, fkt, v);
         if ((fkt += kSfGroup) >= tiles_k) fkt = 0, fu += n_clusters;
       };
       uint32_t it = 0, slot = 0, ph = 1u;
       int u = cluster, kt = 0;  // the group that is stored next
       bool ok = true;
-      const auto group = [&](uint4 (&v)[4]) {
+      const auto group = [&](uint32_t (&v)[4][5]) {
         if (u >= total || !ok) return;
         // free once its previous contents are in tensor memory
         if (!warp_wait(smem_u32(&bar_sf[slot]), ph, abort_v, status)) { ok = false; return; }
         const uint32_t sfull = sfull0 + 8u * slot, at = C::kSfOff + slot * C::kSfSlotBytes;
+        units.at(u, pair, step);
         if (lane == 0) {
-          units.at(u, pair, step);
           const int atom = (NT * step * tiles_k + kt) * 4;  // the atoms seen as rows of 128 bytes
           if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 2 * NT * kSfGroup * kAtomBytes);
           // (a last group of fewer K-tiles brings the next tile's atoms or zeros along, which nothing reads)
           tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
           if (NT == 2) tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
         }
-        ++it;
+        if (it++ == 0) scales_first_arrive();
+        scales.tiles(static_cast<int64_t>(pair) * 256 + rank * 128 + lane, kt, v);
         uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at) + lane;
 #pragma unroll
-        for (int d = 0; d < kSfGroup; ++d) cells[d * 32] = make_uint4(word_of(v[0], d), word_of(v[1], d), word_of(v[2], d), word_of(v[3], d));
+        for (int d = 0; d < kSfGroup; ++d) cells[d * 32] = make_uint4(v[0][d], v[1][d], v[2][d], v[3][d]);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(leader ? smem_u32(&bar_sfull[slot]) : smem_u32(&bar_relay[slot]));
