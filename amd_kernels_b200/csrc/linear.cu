@@ -60,7 +60,9 @@ __global__ void __launch_bounds__(256) quant_mxfp8_kernel(const uint4* x, int64_
 
 // ------------------------------------------------------------------------------------------------ the call
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream);  // linear_tc.cu
-int linear_pair(const LinearArgs& a, int nt, int32_t* status, cudaStream_t stream);            // linear_pair.cu
+int linear_tc_resident(int bm, int log_splits);
+int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_pair.cu
+int linear_pair_resident();
 int set_wait_limit_linear_tc(unsigned long long ns);
 int set_wait_limit_linear_pair(unsigned long long ns);
 
@@ -98,14 +100,37 @@ int set_wait_limit_linear(unsigned long long ns) {
   return r ? r : set_wait_limit_linear_pair(ns);
 }
 
-// The kernel, its token block and its split of K for these sizes.
+// CTAs along K for `units` (weight tile, token block): the most of 1, 2 and 4 whose clusters are all resident at once (a second round of
+// clusters costs more than any split gives: 6144 -> 6144, one row, 10.4 us with 4, 16 with 6), and 8 where they do not fill the SMs
+// once (4096 -> 2048: 5.2 against 6.3 with 4; 6144 -> 4096, 256 CTAs of 8: 8.5 against 8.8 for a row, 16.1 against 14.7 for 128). 0: no one round.
+static int splits_for(const LinearArgs& a, int bm, int64_t units) {
+  for (int log = 3; log >= 0; --log) {
+    if ((1 << log) > a.tiles_k || (log == 3 && units * 8 > sm_count())) continue;
+    if (units <= linear_tc_resident(bm, log)) return 1 << log;
+  }
+  return 0;
+}
+
+// The kernel, its token block and its split of K. Measured, us, 6144 -> 6144 (4096; 12288) unless said otherwise:
+//   up to 128 rows the smallest block that holds them, so that the weights stream once; but two blocks of half the rows where these
+//   still split K by 4 (33 to 64 rows: 10.7 / 11.4 at 4096, 14.1 / 13.1 at 6144 with a split of 2) or by 2 (65 to 128 rows: 12.2 / 14.7 at
+//   4096, 16.3 / 16.4 at 6144, 25.7 / 22.7 at 12288 without a split).
+//   More rows: blocks of 128 on one CTA while they split K by 2 in one round, else CTA pairs: 256 rows 21.1 / 25.4, 384 21.1 / 25.7, 512
+//   34.3 / 26.2; 1024 rows 6144 -> 2048 20.5 / 24.3, 1536 33.4 / 25.7. Without a split too where they need one round and the pairs two
+//   (384 rows at 12288: 35.7 / 42.1).
 static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
-  if (a.m > 256) return linear_pair(a, 2, status, stream);
-  const int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : a.m <= 128 ? 128 : 256;
-  const int64_t units = (a.m + bm - 1) / bm * a.tiles_n;
-  int splits = 1;
-  while (splits < 8 && splits < a.tiles_k && units * (splits + 1) <= sm_count()) ++splits;
-  return linear_tc(a, bm, splits, status, stream);
+  const int64_t blocks = (a.m + 127) / 128;
+  int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+  int splits = splits_for(a, bm, blocks * a.tiles_n);
+  if (blocks == 1 && bm >= 64) {
+    const int half = splits_for(a, bm / 2, 2 * static_cast<int64_t>(a.tiles_n));
+    if (half >= (bm == 64 ? 4 : 2)) bm /= 2, splits = half;
+  }
+  if (blocks > 1) {
+    const int64_t pairs = (a.m + 255) / 256 * ((a.tiles_n + 1) / 2);
+    if (splits == 0 || (splits == 1 && pairs <= linear_pair_resident())) return linear_pair(a, status, stream);
+  }
+  return linear_tc(a, bm, splits ? splits : 1, status, stream);
 }
 
 }  // namespace b200moe

@@ -1,8 +1,8 @@
 // The MXFP8 product for many rows, on CTA pairs: tcgen05.mma.cta_group::2 kind::mxf8f6f4 with M = 256 token rows (two blocks of 128) x
-// N = 256 or 128 weight rows (NT = two tiles or one) x K = 32 per instruction, each CTA staging its own 128 token rows and half of the
+// N = 256 weight rows (two tiles) x K = 32 per instruction, each CTA staging its own 128 token rows and half of the
 // weight rows. No multicast.
 //
-// Unit = (pair of token blocks) x (NT weight tiles). Two rings: 6 stages of codes, and 3 slots of the scales of four K-tiles that travel
+// Unit = (pair of token blocks) x (pair of weight tiles). Two rings: 5 stages of codes, and 3 slots of the scales of four K-tiles that travel
 // ahead of them, so that the MMA warp waits for codes and, once in four K-tiles, for scales. The token scales come row-major, as every producer of this package writes them: the scale
 // warp turns them into atoms on the way, so no launch in front of the product re-lays them.
 //
@@ -10,7 +10,7 @@
 //   warp 1      tensor memory (both CTAs); in the leader it issues the MMAs for both, the whole warp around one elected lane
 //   warp 2      leader: copies the scales into tensor memory in both CTAs, in the same way; partner: tells the leader of its token scales
 //   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
-//   warps 4-11  epilogue (both CTAs): thread = one token row, 64 * NT columns. The sums are pulled into registers and the accumulator
+//   warps 4-11  epilogue (both CTAs): thread = one token row, 128 columns. The sums are pulled into registers and the accumulator
 //               is handed back; then bias, activation, residual and one rounding, 32 columns at a time. bf16 rows go through a strip of
 //               shared memory per warp, 32 rows x 64 columns: the residual arrives there by TMA, the result leaves there by TMA. (A
 //               thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the operands of
@@ -22,23 +22,19 @@
 
 namespace b200moe {
 
-template <int NT>
 struct LinearPairCfg {
-  static constexpr int kStages = NT == 2 ? 5 : 6;       // code ring (NT = 2: 6 stages and no strips were 0 to 1 % faster, 4 were 5 % slower)
-  static constexpr int kWRows = 64 * NT;                // weight rows of one CTA
-  static constexpr int kWOff = 128 * 128;               // behind the CTA's 128 token rows
-  static constexpr int kStageBytes = kWOff + kWRows * 128;
-  static constexpr int kSfSlots = 3;                    // groups of scales in shared memory
-  static constexpr int kStripBytes = 32 * 128;          // one epilogue warp's rows x 64 bf16 columns, 128-byte swizzle
+  static constexpr int kStages = 5;                // code ring (6 stages and no strips were 0 to 1 % faster, 4 were 5 % slower)
+  static constexpr int kSfSlots = 3;               // groups of scales in shared memory
+  static constexpr int kWOff = 128 * 128;          // the CTA's weight tile, behind its 128 token rows
+  static constexpr int kStageBytes = 2 * 128 * 128;
+  static constexpr int kStripBytes = 32 * 128;     // one epilogue warp's rows x 64 bf16 columns, 128-byte swizzle
   static constexpr int kStripOff = kStages * kStageBytes;
   static constexpr int kSfOff = kStripOff + 8 * kStripBytes;
-  static constexpr int kSfSlotBytes = kSfGroup * (1 + NT) * kAtomBytes;  // four token atoms, four atoms of each weight tile
+  static constexpr int kSfSlotBytes = kSfGroup * 3 * kAtomBytes;  // four token atoms, four atoms of each weight tile
   static constexpr int kBiasOff = kSfOff + kSfSlots * kSfSlotBytes;
-  static constexpr int kCols = 64 * NT;                 // accumulator columns of an epilogue thread
-  static constexpr int kSmemBytes = kBiasOff + 8 * kCols * 4 + 1024;
+  static constexpr int kSmemBytes = kBiasOff + 8 * 128 * 4 + 1024;
   static constexpr int kThreads = 32 * 12;
-  static constexpr int kAccs = NT == 1 ? 2 : 1;         // accumulators of 128 * NT columns
-  static constexpr int kSfCol = 256;                    // tensor memory: accumulators, then 2 sets of 4 x 16 columns
+  static constexpr int kSfCol = 256;               // tensor memory: the accumulator, then 2 sets of 4 x 16 columns
   static constexpr int kTmemCols = 512;
   static_assert(kSmemBytes <= 227 * 1024 && kSfCol + kSfSets * kSfGroup * 16 <= kTmemCols, "shared and tensor memory");
 };
@@ -90,12 +86,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-template <int KIND, bool MX, int NT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::kThreads, 1)
+template <int KIND, bool MX>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_wc,
                        const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_res,
                        const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LinearArgs args, int32_t* status) {
-  using C = LinearPairCfg<NT>;
+  using C = LinearPairCfg;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[C::kStages];     // leader: both CTAs' codes of the stage have landed
   __shared__ __align__(8) uint64_t bar_empty[C::kStages];    // in each CTA: the MMAs that read the stage have completed
@@ -103,8 +99,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   __shared__ __align__(8) uint64_t bar_sf[C::kSfSlots];         // in each CTA: they have been copied to tensor memory
   __shared__ __align__(8) uint64_t bar_relay[C::kSfSlots];   // partner: its token scales of the group are in its shared memory
   __shared__ __align__(8) uint64_t bar_set[kSfSets];         // leader: the MMAs that read the set have completed
-  __shared__ __align__(8) uint64_t bar_tfull[C::kAccs];      // in each CTA: the unit's accumulator is complete
-  __shared__ __align__(8) uint64_t bar_tempty[C::kAccs];     // leader: both CTAs' epilogues have read it
+  __shared__ __align__(8) uint64_t bar_tfull;                // in each CTA: the unit's accumulator is complete
+  __shared__ __align__(8) uint64_t bar_tempty;               // leader: both CTAs' epilogues have read it
   __shared__ __align__(8) uint64_t bar_res[8];               // an epilogue warp's residual has landed in its strip
   __shared__ __align__(8) uint64_t bar_drain[2];
   __shared__ uint32_t tmem_base_slot;
@@ -130,10 +126,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
       mbar_init(smem_u32(&bar_sf[j]), 1);
       mbar_init(smem_u32(&bar_relay[j]), 1);
     }
-    for (int i = 0; i < C::kAccs; ++i) {
-      mbar_init(smem_u32(&bar_tfull[i]), 1);
-      mbar_init(smem_u32(&bar_tempty[i]), 16);  // one arrival per epilogue warp of both CTAs
-    }
+    mbar_init(smem_u32(&bar_tfull), 1);
+    mbar_init(smem_u32(&bar_tempty), 16);  // one arrival per epilogue warp of both CTAs
     for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&bar_res[i]), 1);
     mbar_init(smem_u32(&bar_drain[0]), 1);
     mbar_init(smem_u32(&bar_drain[1]), 1);
@@ -147,13 +141,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   const int n_clusters = static_cast<int>(gridDim.x >> 1), cluster = static_cast<int>(blockIdx.x >> 1);
-  const LinearUnits units = {static_cast<int>((args.m + 255) / 256), (args.tiles_n + NT - 1) / NT};
+  const LinearUnits units = {static_cast<int>((args.m + 255) / 256), (args.tiles_n + 1) / 2};
   const int total = units.total(), tiles_k = args.tiles_k;
   int pair, step;
   // the first weights that this CTA will load, into L2 while the launch in front still runs
   if (warp == 0 && lane == 0 && cluster < total) {
     units.at(cluster, pair, step);
-    const int tile = NT == 2 ? 2 * step + static_cast<int>(rank) : step, n = tiles_k < 8 ? tiles_k : 8;
+    const int tile = 2 * step + static_cast<int>(rank), n = tiles_k < 8 ? tiles_k : 8;
     if (tile < args.tiles_n) {
       const int64_t at = static_cast<int64_t>(tile) * tiles_k;
       for (int kt = 0; kt < n; ++kt) l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
@@ -184,9 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
         for (int u = cluster; u < total && ok; u += n_clusters) {
           units.at(u, pair, step);
           const int row = pair * 256 + static_cast<int>(rank) * 128;
-          // NT = 2: the whole tile 2 step + rank; NT = 1: half of tile `step`
-          int rec = NT == 2 ? (2 * step + static_cast<int>(rank)) * tiles_k * 128
-                            : step * tiles_k * 128 + static_cast<int>(rank) * 64;
+          int rec = (2 * step + static_cast<int>(rank)) * tiles_k * 128;  // the images seen as rows of 128 bytes
           for (int kt = 0; kt < tiles_k; ++kt, ++it, rec += 128) {
             if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
             const uint32_t full = full0 + 8u * s, base = tiles + s * C::kStageBytes;
@@ -222,11 +214,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
         const uint32_t sfull = sfull0 + 8u * slot, at = C::kSfOff + slot * C::kSfSlotBytes;
         units.at(u, pair, step);
         if (lane == 0) {
-          const int atom = (NT * step * tiles_k + kt) * 4;  // the atoms seen as rows of 128 bytes
-          if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 2 * NT * kSfGroup * kAtomBytes);
+          const int atom = (2 * step * tiles_k + kt) * 4;  // the atoms seen as rows of 128 bytes
+          if (leader) mbar_arrive_expect_tx(smem_u32(&bar_sfull[slot]), 4 * kSfGroup * kAtomBytes);
           // (a last group of fewer K-tiles brings the next tile's atoms or zeros along, which nothing reads)
           tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
-          if (NT == 2) tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
+          tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
         }
         if (it++ == 0) scales_first_arrive();
         scales.tiles(static_cast<int64_t>(pair) * 256 + rank * 128 + lane, kt, v);
@@ -250,15 +242,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue (leader only)
       if (leader) {
-        // E4M3 x E4M3, UE8M0 scales, M = 256, N = 128 NT; scale byte k of a row's cell for MMA k
-        constexpr uint32_t kIdesc = (static_cast<uint32_t>(128 * NT >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24);
+        // E4M3 x E4M3, UE8M0 scales, M = 256, N = 256; scale byte k of a row's cell for MMA k
+        constexpr uint32_t kIdesc = (static_cast<uint32_t>(256 >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24);
         uint32_t ui = 0, s = 0, ph = 0, slot = 0, sph = 0, set = 0;
         bool ok = true, ready = false;
         for (int u = cluster; u < total && ok; u += n_clusters, ++ui) {
-          const uint32_t acc = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
-          if (!warp_wait(smem_u32(&bar_tempty[acc]), aph ^ 1u, abort_v, status)) break;
+          if (!warp_wait(smem_u32(&bar_tempty), (ui & 1u) ^ 1u, abort_v, status)) break;
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + acc * 128 * NT;
           for (int kt = 0; kt < tiles_k && ok; kt += kSfGroup) {
             if (!warp_wait(smem_u32(&bar_sf[slot]), sph, abort_v, status)) { ok = false; break; }
             if (++slot == C::kSfSlots) { slot = 0; sph ^= 1u; }
@@ -273,10 +263,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
               if (++s == C::kStages) { s = 0; ph ^= 1u; }
               ready = mbar_test(smem_u32(&bar_full[s]), ph);
               if (elect_one()) {
-                tc_mma_mxf8_two(d_tmem, x_lo, w_lo, kIdesc, t_sft, t_sfw, static_cast<uint32_t>(kt + d != 0));
-                tc_mma_mxf8_two(d_tmem, x_lo + 2, w_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sft, t_sfw, 1u);
-                tc_mma_mxf8_two(d_tmem, x_lo + 4, w_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sft, t_sfw, 1u);
-                tc_mma_mxf8_two(d_tmem, x_lo + 6, w_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sft, t_sfw, 1u);
+                tc_mma_mxf8_two(tmem_base, x_lo, w_lo, kIdesc, t_sft, t_sfw, static_cast<uint32_t>(kt + d != 0));
+                tc_mma_mxf8_two(tmem_base, x_lo + 2, w_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sft, t_sfw, 1u);
+                tc_mma_mxf8_two(tmem_base, x_lo + 4, w_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sft, t_sfw, 1u);
+                tc_mma_mxf8_two(tmem_base, x_lo + 6, w_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sft, t_sfw, 1u);
                 tc_commit_both(empty);  // the stage is free again, in both CTAs
                 if (d == n - 1) tc_commit_pair(smem_u32(&bar_set[set]));
               }
@@ -284,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
             }
             if (++set == kSfSets) set = 0;
           }
-          if (ok && elect_one()) tc_commit_both(smem_u32(&bar_tfull[acc]));
+          if (ok && elect_one()) tc_commit_both(smem_u32(&bar_tfull));
         }
         if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05_pair(smem_u32(&bar_drain[0]));
       }
@@ -309,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
                 const uint32_t from = lo + d * (kAtomBytes >> 4);
                 tc_cp_scales_pair(t_sft + 16 * d, from);                                         // each CTA its own token rows
                 tc_cp_scales_pair(t_sfw + 16 * d, from + (kSfGroup * kAtomBytes >> 4));          // weight rows 0..127 of N
-                if (NT == 2) tc_cp_scales_pair(t_sfw + 16 * d + 4, from + (2 * kSfGroup * kAtomBytes >> 4));  // 128..255
+                tc_cp_scales_pair(t_sfw + 16 * d + 4, from + (2 * kSfGroup * kAtomBytes >> 4));  // 128..255
               }
               tc_commit_both(smem_u32(&bar_sf[slot]));
             }
@@ -336,15 +326,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
   } else {
     // ---------------------------------------------------------------- epilogue (both CTAs, warps 4..11)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    constexpr int kParts = C::kCols / 32;                       // accumulator pieces of 32 columns
+    constexpr int kParts = 4;                                   // accumulator pieces of 32 columns
     constexpr int kOuts = KIND == kGated ? kParts / 2 : kParts; // pieces of 32 output columns
     const int q = warp & 3;                  // the TMEM lane quarter this warp may read
     const int half = (warp >> 2) - 1;        // which half of the unit's columns
-    const uint32_t tempty_leader = map_to_cta(smem_u32(&bar_tempty[0]), 0);
-    float* const bias = reinterpret_cast<float*>(tiles_ptr + C::kBiasOff) + (warp - 4) * C::kCols;
-    constexpr bool kStore = !MX && kOuts >= 2;  // bf16 rows leave through the strip (a lone piece of 32 columns: directly)
-    const bool wide = !MX ? (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (a.out_stride & 15) == 0
-                          : (reinterpret_cast<uintptr_t>(a.out_codes) & 31) == 0;
+    const uint32_t tempty_leader = map_to_cta(smem_u32(&bar_tempty), 0);
+    float* const bias = reinterpret_cast<float*>(tiles_ptr + C::kBiasOff) + (warp - 4) * 128;
+    const bool wide = (reinterpret_cast<uintptr_t>(a.out_codes) & 31) == 0;
     const bool scale_words = (a.n & 127) == 0 && (reinterpret_cast<uintptr_t>(a.out_scales) & 3) == 0;
     const uint32_t strip = tiles + C::kStripOff + (warp - 4) * C::kStripBytes;
     uint8_t* const strip_row = tiles_ptr + C::kStripOff + (warp - 4) * C::kStripBytes + lane * 128;
@@ -354,8 +342,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
     const auto place = [&](int v, int64_t& row, int& col) {
       units.at(v, pair, step);
       row = static_cast<int64_t>(pair) * 256 + rank * 128 + q * 32;
-      const int tile = NT == 2 ? 2 * step + half : step;
-      col = KIND == kGated ? tile * 64 + (NT == 1 ? 32 * half : 0) : tile * 128 + (NT == 1 ? 64 * half : 0);
+      col = (2 * step + half) * (KIND == kGated ? 64 : 128);
     };
     // The residual of 64 columns (rows and columns beyond the matrix arrive as zeros); lane 0, once the strip is free.
     const auto ask_residual = [&](int64_t row, int col) {
@@ -383,18 +370,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
         bias[32 * i + lane] = a.bias != nullptr && col < a.n ? __ldcg(a.bias + from) : 0.0f;
       }
       __syncwarp();
-      const uint32_t acc_i = ui % C::kAccs, aph = (ui / C::kAccs) & 1u;
       // the warp decides together: tcgen05.ld below needs all 32 lanes
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull[acc_i]), aph, abort_v, status))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull), ui & 1u, abort_v, status))) break;
       tc_fence_after();
-      const uint32_t t_acc = tmem_base + acc_i * 128 * NT + C::kCols * half + (static_cast<uint32_t>(q * 32) << 16);
+      const uint32_t t_acc = tmem_base + 128 * half + (static_cast<uint32_t>(q * 32) << 16);
       uint32_t acc[kParts][32];
 #pragma unroll
       for (int i = 0; i < kParts; ++i) tc_ld32_nowait(t_acc + 32 * i, acc[i]);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * acc_i);
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
       // (a loop of one piece whose registers move up: unrolled, the code of a unit does not stay in the instruction cache)
       uint32_t scale_bytes = 0;
       bool ok = true;
@@ -463,39 +449,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg<NT>::k
               if (i == 3) *reinterpret_cast<uint32_t*>(a.out_scales + row * (a.n / 32) + col / 32 - 3) = scale_bytes;
             }
           }
-        } else if (kStore) {
+        } else {
 #pragma unroll
           for (int p = 0; p < 4; ++p)
             *reinterpret_cast<uint4*>(strip_row + (((4 * (i & 1) + p) ^ (lane & 7)) << 4)) =
                 make_uint4(pack_bf16x2(y[4 * p].x, y[4 * p].y), pack_bf16x2(y[4 * p + 1].x, y[4 * p + 1].y),
                            pack_bf16x2(y[4 * p + 2].x, y[4 * p + 2].y), pack_bf16x2(y[4 * p + 3].x, y[4 * p + 3].y));
-        } else {
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            uint32_t w[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(y[8 * p + k].x, y[8 * p + k].y);
-            const int c = col + 16 * p;
-            if (in_row && c < a.n) {
-              __nv_bfloat16* o = a.out + row * a.out_stride + c;
-              if (wide && c + 8 < a.n) {
-                st_sector(o, w);
-              } else {
-                reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                if (c + 8 < a.n) reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-              }
-            }
-          }
         }
-        if ((i & 1) || i == kOuts - 1) {  // 64 columns are done
-          if (kStore) fence_proxy_async();
+        if (i & 1) {  // 64 columns are done
+          if (!MX) fence_proxy_async();
           __syncwarp();
           const bool more = i + 1 < kOuts || u + n_clusters < total;
           int64_t next_row = row0;
           int next_col = col + 32;
           if (residual && i + 1 >= kOuts && more) place(u + n_clusters, next_row, next_col);
           if (lane == 0) {
-            if (kStore) {
+            if (!MX) {
               // (what lies beyond the matrix is not written)
               if (row0 < a.m && col - 32 < a.n) tma_store_2d(&map_out, col - 32, static_cast<int>(row0), strip);
               tma_store_wait_read();
@@ -545,51 +514,49 @@ static int make_rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t 
   return r == CUDA_SUCCESS ? 0 : B200MOE_E_DRIVER;
 }
 
-template <int KIND, bool MX, int NT>
+template <int KIND, bool MX>
 static int linear_pairs() {
   static std::mutex mu;
   static int pairs[kMaxDevices] = {};
   static bool known[kMaxDevices] = {};
-  return resident_pairs_of(linear_pair_kernel<KIND, MX, NT>, LinearPairCfg<NT>::kThreads, LinearPairCfg<NT>::kSmemBytes, mu, known, pairs);
+  return resident_pairs_of(linear_pair_kernel<KIND, MX>, LinearPairCfg::kThreads, LinearPairCfg::kSmemBytes, mu, known, pairs);
 }
 
-template <int KIND, bool MX, int NT>
+template <int KIND, bool MX>
 static int launch_linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
-  using C = LinearPairCfg<NT>;
+  using C = LinearPairCfg;
   CUtensorMap mx, mwc, mws, mres = {}, mout = {};
   const uint64_t n_tiles = static_cast<uint64_t>(a.tiles_n) * a.tiles_k;
   int r;
   if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), 128))) return r;
-  if ((r = make_flat_map(&mwc, a.tiles, n_tiles * 128, C::kWRows))) return r;
+  if ((r = make_flat_map(&mwc, a.tiles, n_tiles * 128, 128))) return r;
   if ((r = make_flat_map(&mws, a.atoms, n_tiles * 4, kSfGroup * 4))) return r;
   if (a.residual && (r = make_rows_map(&mres, a.residual, a.n, a.m, a.residual_stride))) return r;
   if (a.out && (r = make_rows_map(&mout, a.out, a.n, a.m, a.out_stride))) return r;
-  const int64_t units = (a.m + 255) / 256 * ((a.tiles_n + NT - 1) / NT);
+  const int64_t units = (a.m + 255) / 256 * ((a.tiles_n + 1) / 2);
   if (units > 0x7fffffff) return B200MOE_E_ARG;
-  const int pairs = linear_pairs<KIND, MX, NT>();
+  const int pairs = linear_pairs<KIND, MX>();
   if (pairs <= 0) return B200MOE_E_DRIVER;
-  return launch_pairs(linear_pair_kernel<KIND, MX, NT>, units < pairs ? static_cast<int>(units) : pairs, C::kThreads, C::kSmemBytes, stream,
+  return launch_pairs(linear_pair_kernel<KIND, MX>, units < pairs ? static_cast<int>(units) : pairs, C::kThreads, C::kSmemBytes, stream,
                       mx, mwc, mws, mres, mout, a, status);
 }
 
-template <int KIND, int NT>
+template <int KIND>
 static int linear_pair_out(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
-  return a.out ? launch_linear_pair<KIND, false, NT>(a, status, stream) : launch_linear_pair<KIND, true, NT>(a, status, stream);
+  return a.out ? launch_linear_pair<KIND, false>(a, status, stream) : launch_linear_pair<KIND, true>(a, status, stream);
 }
 
-template <int NT>
-static int linear_pair_kind(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
+int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   switch (a.act.kind) {
-    case kLinear: return linear_pair_out<kLinear, NT>(a, status, stream);
-    case kSigmoid: return linear_pair_out<kSigmoid, NT>(a, status, stream);
-    case kGelu: return linear_pair_out<kGelu, NT>(a, status, stream);
+    case kLinear: return linear_pair_out<kLinear>(a, status, stream);
+    case kSigmoid: return linear_pair_out<kSigmoid>(a, status, stream);
+    case kGelu: return linear_pair_out<kGelu>(a, status, stream);
   }
-  return linear_pair_out<kGated, NT>(a, status, stream);
+  return linear_pair_out<kGated>(a, status, stream);
 }
 
-int linear_pair(const LinearArgs& a, int nt, int32_t* status, cudaStream_t stream) {
-  return nt == 2 ? linear_pair_kind<2>(a, status, stream) : linear_pair_kind<1>(a, status, stream);
-}
+// Pairs that are resident at once (the kinds do not differ in what they hold)
+int linear_pair_resident() { return linear_pairs<kLinear, false>(); }
 
 int set_wait_limit_linear_pair(unsigned long long ns) { return set_wait_limit_here(ns); }
 

@@ -18,100 +18,89 @@ namespace b200moe {
 
 template <int BM>
 struct LinearCfg {
-  static constexpr int kAtoms = BM > 128 ? 2 : 1;                            // token scale atoms of a K-tile
-  static constexpr int kTokOff = kLinearImageBytes;                          // token rows behind the weight image
+  static constexpr int kTokOff = kLinearImageBytes;               // token rows behind the weight image
   static constexpr int kStageBytes = kTokOff + BM * 128;
-  static constexpr int kCtasPerSm = BM > 128 ? 1 : 2;                        // two: one's start and end under the other's stream
-  static constexpr int kStages = BM > 128 ? 4 : BM > 64 ? 3 : BM > 32 ? 4 : 5;
-  static constexpr int kSfSlots = BM == 32 ? 2 : 3;                          // groups of scales in shared memory
+  static constexpr int kCtasPerSm = 2;                            // one's start and end under the other's stream
+  static constexpr int kStages = BM > 64 ? 3 : BM > 32 ? 4 : 5;
+  static constexpr int kSfSlots = BM == 32 ? 2 : 3;               // groups of scales in shared memory
   static constexpr int kSfOff = kStages * kStageBytes;
-  static constexpr int kSfTileBytes = (1 + kAtoms) * kAtomBytes;             // a K-tile's scales in a slot: see below
-  static constexpr int kSfSlotBytes = kSfGroup * kSfTileBytes;               // weight atoms of the group, then token atoms by K-tile
-  static constexpr int kSumRow = 132;                                        // floats of a token's 128 columns in the parts (alias the ring)
+  static constexpr int kSfSlotBytes = kSfGroup * 2 * kAtomBytes;  // weight atoms of the group, then token atoms
+  static constexpr int kSumRow = 132;                             // floats of a token's 128 columns in the parts (alias the ring)
   static constexpr int kSmemBytes = kSfOff + kSfSlots * kSfSlotBytes + 1024;
-  static constexpr int kSfCols = kAtoms > 1 ? 16 : 8;                        // tensor memory columns of a K-tile's scales: weights, tokens
+  static constexpr int kSfCols = 8;                               // tensor memory columns of a K-tile's scales: 4 weights, 4 tokens
   static constexpr int kColsUsed = BM + kSfSets * kSfGroup * kSfCols;
-  static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+  static constexpr int kTmemCols = kColsUsed <= 128 ? 128 : 256;
   static_assert(BM * kSumRow * 4 <= kSfOff, "the parts fit the ring");
   static_assert(kSmemBytes <= 227 * 1024 / kCtasPerSm - 1024 && kTmemCols * kCtasPerSm <= 512, "shared and tensor memory");
 };
 
+// (neither volatile nor ordered by a memory clobber: the loads of a row's parts have to be in flight together; what orders them is the
+// cluster barrier in front, whose address register they are made to depend on)
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  asm("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
-// one token row of a tile: four columns a lane (gated: two columns a lane). `at`: this row's sums in this CTA's shared memory
-__device__ __forceinline__ void finish_row(const LinearArgs& a, int64_t row, int tile, uint32_t at, int splits, int lane) {
-  float y[4];
-  int col, cols;
-  if (a.act.kind == kGated) {
-    const int g = lane >> 4, j = (lane & 15) * 2;
-    col = tile * 64 + 32 * g + j;
-    cols = 2;
-    float2 p = make_float2(0.0f, 0.0f), u = p;
-    for (int r = 0; r < splits; ++r) {
-      const uint32_t from = splits > 1 ? map_to_cta(at, r) : at;
-      const float2 pr = ld_cluster_f2(from + (64 * g + j) * 4), ur = ld_cluster_f2(from + (64 * g + 32 + j) * 4);
-      p.x += pr.x, p.y += pr.y, u.x += ur.x, u.y += ur.y;
+constexpr int kMaxSplits = 8;
+
+// The rows of the block that fall to this warp (every `step`-th from `first` on): the parts of a row are added in the order of K, then bias,
+// activation, residual and the only rounding. A lane has four of the tile's 128 columns; gated, lanes 0-7 and 16-23 have the gates of
+// four output columns and take the ups from the lanes 8 above. `parts`: the sums in this CTA's shared memory, kSumRow floats a row.
+template <int SUM_ROW>
+__device__ __forceinline__ void finish_rows(const LinearArgs& a, int64_t row0, int rows, int first, int step, int tile, uint32_t parts,
+                                            int splits, int lane) {
+  const bool gated = a.act.kind == kGated;
+  const int col = gated ? tile * 64 + 32 * (lane >> 4) + (lane & 7) * 4 : tile * 128 + lane * 4;
+  const bool up = gated && (lane & 8);
+  const bool in = col < a.n && !up;  // (n is a multiple of 8: a lane's columns are all inside or all outside)
+  float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (a.bias != nullptr && col < a.n) bias = __ldcg(reinterpret_cast<const float4*>(a.bias + (up ? a.n : 0) + col));
+  uint32_t from[kMaxSplits];
+#pragma unroll
+  for (int r = 0; r < kMaxSplits; ++r) from[r] = r < splits ? (splits > 1 ? map_to_cta(parts, r) : parts) + lane * 16 : 0u;
+  for (int t = first; t < rows; t += step) {
+    const int64_t row = row0 + t;
+    float4 part[kMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < splits) part[r] = ld_cluster_f4(from[r] + t * SUM_ROW * 4);
+    uint2 res = make_uint2(0u, 0u);
+    if (a.residual != nullptr && in) res = __ldcg(reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col));
+    float4 p = part[0];
+#pragma unroll
+    for (int r = 1; r < kMaxSplits; ++r)
+      if (r < splits) p.x += part[r].x, p.y += part[r].y, p.z += part[r].z, p.w += part[r].w;
+    F2 lo = F2{p.x, p.y} + F2{bias.x, bias.y}, hi = F2{p.z, p.w} + F2{bias.z, bias.w};
+    if (gated) {
+      const F2 ulo = {__shfl_down_sync(0xffffffffu, lo.x, 8), __shfl_down_sync(0xffffffffu, lo.y, 8)};
+      const F2 uhi = {__shfl_down_sync(0xffffffffu, hi.x, 8), __shfl_down_sync(0xffffffffu, hi.y, 8)};
+      lo = act_gated(lo, ulo, a.act), hi = act_gated(hi, uhi, a.act);
+    } else if (a.act.kind == kLinear) {
+      lo = act_of<kLinear>(lo, a.act), hi = act_of<kLinear>(hi, a.act);
+    } else if (a.act.kind == kSigmoid) {
+      lo = act_of<kSigmoid>(lo, a.act), hi = act_of<kSigmoid>(hi, a.act);
+    } else {
+      lo = act_of<kGelu>(lo, a.act), hi = act_of<kGelu>(hi, a.act);
     }
-    if (a.bias != nullptr && col < a.n) {
-      const float2 bp = __ldcg(reinterpret_cast<const float2*>(a.bias + col)), bu = __ldcg(reinterpret_cast<const float2*>(a.bias + a.n + col));
-      p.x += bp.x, p.y += bp.y, u.x += bu.x, u.y += bu.y;
+    if (a.residual != nullptr) {
+      lo = lo + F2{__uint_as_float(res.x << 16), __uint_as_float(res.x & 0xffff0000u)};
+      hi = hi + F2{__uint_as_float(res.y << 16), __uint_as_float(res.y & 0xffff0000u)};
     }
-    const F2 v = act_gated(F2{p.x, p.y}, F2{u.x, u.y}, a.act);
-    y[0] = v.x, y[1] = v.y, y[2] = y[3] = 0.0f;
-  } else {
-    col = tile * 128 + lane * 4;
-    cols = 4;
-    float4 p = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int r = 0; r < splits; ++r) {
-      const float4 pr = ld_cluster_f4((splits > 1 ? map_to_cta(at, r) : at) + lane * 16);
-      p.x += pr.x, p.y += pr.y, p.z += pr.z, p.w += pr.w;
+    if (a.out != nullptr) {
+      if (in) *reinterpret_cast<uint2*>(a.out + row * a.out_stride + col) = make_uint2(pack_bf16x2(lo.x, lo.y), pack_bf16x2(hi.x, hi.y));
+    } else {  // a block of 32 columns is 8 neighbouring lanes
+      float amax = fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(hi.x), fabsf(hi.y)));
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      const int e = linear_scale(amax);
+      const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+      if (in) {
+        *reinterpret_cast<uint32_t*>(a.out_codes + row * a.n + col) = pack_e4m3x4(lo.x * inv, lo.y * inv, hi.x * inv, hi.y * inv);
+        if ((lane & 7) == 0) a.out_scales[row * (a.n / 32) + col / 32] = static_cast<uint8_t>(e);
+      }
     }
-    if (a.bias != nullptr && col < a.n) {
-      const float4 b = __ldcg(reinterpret_cast<const float4*>(a.bias + col));
-      p.x += b.x, p.y += b.y, p.z += b.z, p.w += b.w;
-    }
-    F2 lo = {p.x, p.y}, hi = {p.z, p.w};
-    if (a.act.kind == kLinear) lo = act_of<kLinear>(lo, a.act), hi = act_of<kLinear>(hi, a.act);
-    else if (a.act.kind == kSigmoid) lo = act_of<kSigmoid>(lo, a.act), hi = act_of<kSigmoid>(hi, a.act);
-    else lo = act_of<kGelu>(lo, a.act), hi = act_of<kGelu>(hi, a.act);
-    y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
   }
-  const bool in = col < a.n;  // (n is a multiple of 8: a lane's columns are all inside or all outside)
-  if (a.residual != nullptr && in) {
-    const __nv_bfloat16* r = a.residual + row * a.residual_stride + col;
-    const uint32_t r0 = __ldcg(reinterpret_cast<const uint32_t*>(r));
-    y[0] += __uint_as_float(r0 << 16), y[1] += __uint_as_float(r0 & 0xffff0000u);
-    if (cols == 4) {
-      const uint32_t r1 = __ldcg(reinterpret_cast<const uint32_t*>(r) + 1);
-      y[2] += __uint_as_float(r1 << 16), y[3] += __uint_as_float(r1 & 0xffff0000u);
-    }
-  }
-  if (a.out != nullptr) {
-    if (!in) return;
-    __nv_bfloat16* o = a.out + row * a.out_stride + col;
-    if (cols == 4) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-    else *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(y[0], y[1]);
-    return;
-  }
-  // a block of 32 columns is 8 lanes (gated: 16)
-  float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
-  for (int off = 1; off < 32 / cols; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  const int e = linear_scale(amax);
-  const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
-  if (!in) return;
-  uint8_t* o = a.out_codes + row * a.n + col;
-  if (cols == 4) *reinterpret_cast<uint32_t*>(o) = pack_e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-  else *reinterpret_cast<uint16_t*>(o) = static_cast<uint16_t>(cvt_e4m3x2(y[0] * inv, y[1] * inv));
-  if ((col & 31) == 0) a.out_scales[row * (a.n / 32) + col / 32] = static_cast<uint8_t>(e);
 }
 
 template <int BM>
@@ -245,8 +234,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       if (elect_one()) {
         for (int d = 0; d < n; ++d) {
           tc_cp_scales_lo(t_sfw + d * C::kSfCols, w_atom + d * (kAtomBytes >> 4));
-#pragma unroll
-          for (int h = 0; h < C::kAtoms; ++h) tc_cp_scales_lo(t_sfx + d * C::kSfCols + 4 * h, x_atom + (d * C::kAtoms + h) * (kAtomBytes >> 4));
+          tc_cp_scales_lo(t_sfx + d * C::kSfCols, x_atom + d * (kAtomBytes >> 4));
         }
         tc_commit(smem_u32(&bar_sf[slot]));
       }
@@ -281,10 +269,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at + kSfGroup * kAtomBytes) + lane;
 #pragma unroll
       for (int d = 0; d < kSfGroup; ++d)
-#pragma unroll
-        for (int h = 0; h < C::kAtoms; ++h)
-          cells[(d * C::kAtoms + h) * 32] = make_uint4(v[4 * h][d], kRows > 1 ? v[(4 * h + 1) % kRows][d] : 0u,
-                                                       kRows > 2 ? v[(4 * h + 2) % kRows][d] : 0u, kRows > 2 ? v[(4 * h + 3) % kRows][d] : 0u);
+        cells[d * 32] = make_uint4(v[0][d], kRows > 1 ? v[1 % kRows][d] : 0u, kRows > 2 ? v[2 % kRows][d] : 0u, kRows > 2 ? v[3 % kRows][d] : 0u);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(sfull);
@@ -306,12 +291,24 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     if (__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull), 0, abort_v, status))) {
       tc_fence_after();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-#pragma unroll 1
-      for (int c0 = 0; c0 < BM && row0 + c0 < a.m; c0 += 16) {
+      if (BM == 16) {
         uint32_t v[16];
-        tc_ld16(t_acc + c0, v);
+        tc_ld16(t_acc, v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mine[(c0 + j) * C::kSumRow] = __uint_as_float(v[j]);
+        for (int j = 0; j < 16; ++j) mine[j * C::kSumRow] = __uint_as_float(v[j]);
+      } else {
+        constexpr int kAtOnce = BM >= 64 ? 2 : 1;
+#pragma unroll 1
+        for (int c0 = 0; c0 < BM && row0 + c0 < a.m; c0 += 32 * kAtOnce) {
+          uint32_t v[kAtOnce][32];
+#pragma unroll
+          for (int h = 0; h < kAtOnce; ++h) tc_ld32_nowait(t_acc + c0 + 32 * h, v[h]);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int h = 0; h < kAtOnce; ++h)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) mine[(c0 + 32 * h + j) * C::kSumRow] = __uint_as_float(v[h][j]);
+        }
       }
     }
   }
@@ -321,10 +318,12 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   __syncthreads();
   if (splits > 1) cluster_sync_all();
   const int rows = static_cast<int>(a.m - row0 < BM ? a.m - row0 : BM);
-  if (!abort_flag)
-    for (int t = rank * 8 + warp; t < rows; t += 8 * splits) finish_row(a, row0 + t, tile, tiles + t * C::kSumRow * 4, splits, lane);
+  uint32_t parts = tiles;
+  asm volatile("" : "+r"(parts)::"memory");
+  if (!abort_flag) finish_rows<C::kSumRow>(a, row0, rows, rank * 8 + warp, 8 * splits, tile, parts, splits, lane);
   __syncwarp();
-  if (splits > 1) cluster_sync_all();  // nobody leaves while its parts are read
+  // Nobody leaves while its parts are read. (Relaxed: what has been loaded is in registers, and a release would wait for the stores.)
+  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
@@ -334,23 +333,20 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
 }
 
 template <int BM>
-static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cudaStream_t stream) {
-  using C = LinearCfg<BM>;
+static int configure_linear_tc() {
   static PerDeviceOnce once;
-  int r = once.run([] {
-    return static_cast<int>(cudaFuncSetAttribute(linear_tc_kernel<BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+  return once.run([] {
+    return static_cast<int>(cudaFuncSetAttribute(linear_tc_kernel<BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinearCfg<BM>::kSmemBytes));
   });
-  if (r) return r;
-  CUtensorMap mx;
-  if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), BM))) return r;
-  const int64_t n_blocks = (a.m + BM - 1) / BM, ctas = n_blocks * a.tiles_n * splits;
-  if (ctas > 0x7fffffff) return B200MOE_E_ARG;
+}
+
+template <int BM>
+static cudaLaunchConfig_t linear_tc_config(int64_t clusters, int splits, cudaLaunchAttribute (&attr)[2], cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * splits));
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.dynamicSmemBytes = LinearCfg<BM>::kSmemBytes;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -359,18 +355,62 @@ static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cu
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
+  return cfg;
+}
+
+template <int BM>
+static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cudaStream_t stream) {
+  int r = configure_linear_tc<BM>();
+  if (r) return r;
+  CUtensorMap mx;
+  if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), BM))) return r;
+  const int64_t n_blocks = (a.m + BM - 1) / BM, units = n_blocks * a.tiles_n;
+  if (units * splits > 0x7fffffff) return B200MOE_E_ARG;
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = linear_tc_config<BM>(units, splits, attr, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM>, mx, a, splits, static_cast<int>(n_blocks), status));
 }
 
-// bm: 16, 32, 64, 128 or 256 token rows a block; splits: CTAs along K, 1 to 8 and at most the K-tiles
+// Clusters of `1 << log_splits` CTAs that are resident at once on the current device; asked once per device.
+template <int BM>
+static int resident_clusters(int log_splits) {
+  static std::mutex mu;
+  static int known[kMaxDevices][4] = {};  // 1 + the number
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || configure_linear_tc<BM>()) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[dev][log_splits];
+  if (n == 0) {
+    int got = 0;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = linear_tc_config<BM>(sm_count(), 1 << log_splits, attr, nullptr);
+    if (log_splits == 0) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, linear_tc_kernel<BM>, 256, LinearCfg<BM>::kSmemBytes) != cudaSuccess) got = 1;
+      got *= sm_count();
+    } else if (cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM>, &cfg) != cudaSuccess) {
+      got = 0;
+    }
+    (void)cudaGetLastError();
+    n = 1 + got;
+  }
+  return n - 1;
+}
+
+int linear_tc_resident(int bm, int log_splits) {
+  return bm == 16   ? resident_clusters<16>(log_splits)
+         : bm == 32 ? resident_clusters<32>(log_splits)
+         : bm == 64 ? resident_clusters<64>(log_splits)
+                    : resident_clusters<128>(log_splits);
+}
+
+// bm: 16, 32, 64 or 128 token rows a block; splits: 1, 2, 4 or 8 CTAs along K, at most the K-tiles
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream) {
   switch (bm) {
     case 16: return launch_linear_tc<16>(a, splits, status, stream);
     case 32: return launch_linear_tc<32>(a, splits, status, stream);
     case 64: return launch_linear_tc<64>(a, splits, status, stream);
-    case 128: return launch_linear_tc<128>(a, splits, status, stream);
   }
-  return launch_linear_tc<256>(a, splits, status, stream);
+  return launch_linear_tc<128>(a, splits, status, stream);
 }
 
 int set_wait_limit_linear_tc(unsigned long long ns) { return set_wait_limit_here(ns); }
