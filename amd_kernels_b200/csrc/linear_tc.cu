@@ -371,7 +371,9 @@ static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cu
   return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM>, mx, a, splits, static_cast<int>(n_blocks), status));
 }
 
-// Clusters of `1 << log_splits` CTAs that are resident at once on the current device; asked once per device.
+// Clusters of `1 << log_splits` CTAs that run at once on the current device; asked once per device. The occupancy calculation counts one CTA
+// an SM for kernels that use tensor memory, whatever their shared memory (it says one at 60 KB too); two run (288 CTAs in clusters of two
+// take the time of 192), so its number is doubled.
 template <int BM>
 static int resident_clusters(int log_splits) {
   static std::mutex mu;
@@ -381,17 +383,12 @@ static int resident_clusters(int log_splits) {
   std::lock_guard<std::mutex> lock(mu);
   int& n = known[dev][log_splits];
   if (n == 0) {
-    int got = 0;
+    int got = sm_count();
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = linear_tc_config<BM>(sm_count(), 1 << log_splits, attr, nullptr);
-    if (log_splits == 0) {
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, linear_tc_kernel<BM>, 256, LinearCfg<BM>::kSmemBytes) != cudaSuccess) got = 1;
-      got *= sm_count();
-    } else if (cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM>, &cfg) != cudaSuccess) {
-      got = 0;
-    }
+    const cudaLaunchConfig_t cfg = linear_tc_config<BM>(sm_count(), 1 << log_splits, attr, nullptr);
+    if (log_splits > 0 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM>, &cfg) != cudaSuccess) got = 0;
     (void)cudaGetLastError();
-    n = 1 + got;
+    n = 1 + LinearCfg<BM>::kCtasPerSm * got;
   }
   return n - 1;
 }
