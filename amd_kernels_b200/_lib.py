@@ -40,10 +40,9 @@ class Prepared(Structure):
 
 
 # Calls that a decode step makes many times hand their arguments over as one packed struct (a tenth of the host time of as many ctypes
-# arguments): struct b200moe_norm_call, b200moe_linear_weights, b200moe_linear_call in the machine's alignment; 0 is a null pointer.
+# arguments): struct b200moe_norm_call and b200moe_linear_call in the machine's alignment; 0 is a null pointer.
 NORM_CALL = struct.Struct("@PqPqPPqPqPPqqff")
-LINEAR_WEIGHTS = struct.Struct("@PPqqi")
-LINEAR_CALL = struct.Struct("@PqPPqPqPqPPi")
+LINEAR_CALL = struct.Struct("@PPqqi4xPqPPqPqPqPPi")
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5, "swiglu_oai": 6}  # from 5 on gated
 LAYER_ROUTER, LAYER_SHARED, LAYER_OWN_SLOTS, LAYER_OWN_SHARED_OUT, LAYER_COMPACT = 1, 2, 4, 8, 16
 
@@ -118,7 +117,7 @@ SIGNATURES = {
     "b200moe_linear_weight_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "b200moe_preshuffle_linear": (c_int, [_P, _P, c_int64, c_int64, c_int, _P, _P]),
     "b200moe_quant_mxfp8": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P, _P]),
-    "b200moe_linear": (c_int, [c_char_p, c_char_p, _P, _P]),  # LINEAR_WEIGHTS.pack(...), LINEAR_CALL.pack(...)
+    "b200moe_linear": (c_int, [c_char_p, _P, _P]),  # LINEAR_CALL.pack(...)
     "b200moe_forward": (c_int, [POINTER(Weights), _P, _P, c_int64, _P, c_size_t, _P, _P, _P, _P]),
     "b200moe_forward_host": (c_int, [POINTER(Weights), _P, _P, c_int64, _P, _P, _P, c_size_t, _P, _P, _P, _P, _P]),
 }

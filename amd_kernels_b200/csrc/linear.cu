@@ -170,10 +170,11 @@ extern "C" int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t
 
 namespace b200moe {
 // Checks a call and fills the kernels' arguments; a.m is 0 where there is nothing to do.
-static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const b200moe_linear_call* call, const int32_t* status) {
+static int linear_args(LinearArgs& a, const b200moe_linear_call* call, const int32_t* status) {
   a.m = 0;
-  if (!w || !call) return B200MOE_E_ARG;
+  if (!call) return B200MOE_E_ARG;
   const b200moe_linear_call& c = *call;
+  const b200moe_linear_weights* w = &c.w;
   const int64_t m = c.m;
   if (m < 0 || m > B200MOE_LINEAR_MAX_ROWS || !linear_dims(w->rows, w->k, w->gated)) return B200MOE_E_ARG;
   if (c.activation < B200MOE_ACT_NONE || c.activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
@@ -221,11 +222,11 @@ static int linear_args(LinearArgs& a, const b200moe_linear_weights* w, const b20
 }
 }  // namespace b200moe
 
-extern "C" int b200moe_linear(const b200moe_linear_weights* w, const b200moe_linear_call* call, int32_t* status, void* stream) {
+extern "C" int b200moe_linear(const b200moe_linear_call* call, int32_t* status, void* stream) {
   using namespace b200moe;
   LinearArgs a;
-  int r = linear_args(a, w, call, status);
+  int r = linear_args(a, call, status);
   if (r || a.m == 0) return r;
-  if (call->x && (r = b200moe_quant_mxfp8(call->x, call->x_stride, call->m, w->k, call->codes8, call->scales8, stream))) return r;
+  if (call->x && (r = b200moe_quant_mxfp8(call->x, call->x_stride, call->m, call->w.k, call->codes8, call->scales8, stream))) return r;
   return dispatch_linear(a, status, static_cast<cudaStream_t>(stream));
 }

@@ -97,6 +97,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {  // max(|a|, |b|, |c|); a NaN is skipped
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 constexpr float kLog2e = 1.4426950409f;
 // p * sigmoid(v), v given as -v log2(e)
 __device__ __forceinline__ F2 f2_times_sigmoid(F2 p, F2 w) { return p * f2_rcp(f2_exp2(w) + f2_dup(1.0f)); }
@@ -106,23 +112,23 @@ __device__ __forceinline__ F2 act_sigmoid(F2 p, const LinearAct& a) {
   if (a.c3 == 0.0f) return f2_times_sigmoid(p, p * f2_dup(-kLog2e * a.c1));
   return f2_times_sigmoid(p, p * f2_fma(p * p, f2_dup(-kLog2e * a.c3), f2_dup(-kLog2e * a.c1)));
 }
-// Phi(p) = erfc(-p / sqrt(2)) / 2. erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0: the Chebyshev fit of Numerical Recipes
-// (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision.
+// p Phi(p) = max(p, 0) - |p| erfc(|p| / sqrt(2)) / 2. erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2): the Chebyshev fit of Numerical
+// Recipes (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision. Here s = -t (the
+// odd coefficients change sign), the exponent is to base 2 and takes the half with it.
 __device__ __forceinline__ F2 act_gelu(F2 p) {
-  const F2 z = F2{fabsf(p.x), fabsf(p.y)} * f2_dup(0.70710678f), t = f2_rcp(f2_fma(z, f2_dup(0.5f), f2_dup(1.0f)));
-  F2 q = f2_fma(t, f2_dup(0.17087277f), f2_dup(-0.82215223f));
-  q = f2_fma(q, t, f2_dup(1.48851587f));
-  q = f2_fma(q, t, f2_dup(-1.13520398f));
-  q = f2_fma(q, t, f2_dup(0.27886807f));
-  q = f2_fma(q, t, f2_dup(-0.18628806f));
-  q = f2_fma(q, t, f2_dup(0.09678418f));
-  q = f2_fma(q, t, f2_dup(0.37409196f));
-  q = f2_fma(q, t, f2_dup(1.00002368f));
-  q = f2_fma(q, t, f2_dup(-1.26551223f));
-  const F2 w = f2_fma(z * f2_dup(-1.0f), z, q) * f2_dup(kLog2e);
-  const F2 half = t * f2_dup(0.5f) * f2_exp2(w);  // erfc(z) / 2
-  const F2 other = f2_fma(half, f2_dup(-1.0f), f2_dup(1.0f));
-  return p * F2{p.x < 0.0f ? half.x : other.x, p.y < 0.0f ? half.y : other.y};
+  const F2 m = {fminf(fabsf(p.x), 64.0f), fminf(fabsf(p.y), 64.0f)};  // (erfc is 0 there; infinity times 0 is not)
+  const F2 s = f2_rcp(f2_fma(m, f2_dup(-0.35355339f), f2_dup(-1.0f)));
+  F2 q = f2_fma(s, f2_dup(-0.17087277f * kLog2e), f2_dup(-0.82215223f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-1.48851587f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-1.13520398f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-0.27886807f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-0.18628806f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-0.09678418f * kLog2e));
+  q = f2_fma(q, s, f2_dup(0.37409196f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-1.00002368f * kLog2e));
+  q = f2_fma(q, s, f2_dup(-1.26551223f * kLog2e - 1.0f));
+  const F2 half = s * f2_exp2(f2_fma(m * m, f2_dup(-0.5f * kLog2e), q));  // -erfc / 2
+  return f2_fma(m, half, F2{max_nan(p.x, 0.0f), max_nan(p.y, 0.0f)});
 }
 __device__ __forceinline__ F2 act_gated(F2 g, F2 u, const LinearAct& a) {
   g = {min_nan(g.x, a.top), min_nan(g.y, a.top)};

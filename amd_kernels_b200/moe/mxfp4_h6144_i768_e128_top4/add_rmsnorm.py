@@ -9,40 +9,46 @@ from ... import _lib
 from .tail import TailOutput
 
 MAX_H = 65536
-_BF16 = torch.bfloat16
+_BF16, _U8 = torch.bfloat16, torch.uint8
 
 
-def rows_of(name, t, m, h, dev, shared_row=False):
-    """Checks bf16 rows [m, h] with unit column stride, a multiple of 8 elements apart; that distance."""
-    if t.dtype is not _BF16 or t.shape != (m, h) or t.device != dev:
-        raise ValueError(f"{name}: expected BF16 [{m}, {h}] on {dev}")
+def row_stride(name, t, m, h, one_row=False):
+    """The distance in elements of the rows of a [m, h] tensor that is not contiguous: unit stride along the row, a multiple of 8."""
     stride, unit = t.stride()
     if unit != 1:
         raise ValueError(f"{name}: expected unit stride along the row")
-    if m > 1 and (stride & 7 or (stride < h and not (shared_row and stride == 0))):
+    if m > 1 and (stride & 7 or (stride < h and not (one_row and stride == 0))):
         raise ValueError(f"{name}: rows {stride} elements apart (needs a multiple of 8, at least {h})")
     return stride
 
 
-def check_mxfp8(name, codes, scales, m, width, dev):
+def check_rows(name, t, shape, device):
+    """bf16 [m, h] on CUDA device number ``device``; the distance of its rows in elements."""
+    if t.dtype is not _BF16 or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"{name}: expected BF16 {list(shape)} on device {device}")
+    return shape[1] if t.is_contiguous() else row_stride(name, t, *shape)
+
+
+def check_mxfp8(name, codes, scales, m, width, device):
     """Contiguous [m, width] and [m, width / 32] of one byte each (uint8, or float8 of the two formats)."""
     if codes is None or scales is None:
         raise ValueError(f"{name}: codes and scales come together")
-    if (codes.element_size() != 1 or codes.shape != (m, width) or not codes.is_contiguous() or codes.device != dev
-            or scales.element_size() != 1 or scales.shape != (m, width // 32) or not scales.is_contiguous() or scales.device != dev):
-        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] and scales [{m}, {width // 32}] of one byte each on {dev}")
+    if ((codes.dtype is not _U8 and codes.element_size() != 1) or codes.shape != (m, width) or not codes.is_contiguous()
+            or (scales.dtype is not _U8 and scales.element_size() != 1) or scales.shape != (m, width // 32)
+            or not scales.is_contiguous() or codes.get_device() != device or scales.get_device() != device):
+        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] and scales [{m}, {width // 32}] of one byte each on "
+                         f"device {device}")
 
 
-def launch_on(dev, call, *args):
-    """``call(*args, stream)`` on the current stream of ``dev``, which is made the current device where it is not. A device that is no
-    CUDA device is a ValueError."""
-    if dev.type != "cuda":
-        raise ValueError(f"expected tensors on a CUDA device, got {dev}")
-    if dev.index == torch._C._cuda_getDevice():
-        code = call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def launch_on(device, call, *args):
+    """``call(*args, stream)`` on the current stream of CUDA device number ``device``, which is made the current one where it is not."""
+    if device < 0:
+        raise ValueError("nothing is launched on tensors that are not on a CUDA device")
+    if device == torch._C._cuda_getDevice():
+        code = call(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(dev):
-            code = call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with torch.cuda.device(device):
+            code = call(*args, torch._C._cuda_getCurrentRawStream(device))
     if code:
         _lib.check(code, call.__name__)
 
@@ -58,39 +64,41 @@ def add_rmsnorm_mxfp8(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     comes back. A residual expanded from one row (stride 0) is added to every row. ``out``: where the results go; its tensors
     that are not None say what is computed (``mxfp8`` and ``bf16_out`` are not read). Its ``residual`` and ``normed`` may be ``x`` or
     ``residual`` itself; codes and scales are contiguous. A row's bits depend on nothing but the row."""
-    if x.ndim != 2 or weight.ndim != 1:
-        raise ValueError("expected BF16 [M, H] rows and a [H] weight")
-    m, h = x.shape
-    dev = x.device
+    shape, device = x.shape, x.get_device()
+    if x.dtype is not _BF16 or len(shape) != 2:
+        raise ValueError("expected BF16 [M, H] rows")
+    m, h = shape
     if h < 32 or h % 32 or h > MAX_H:
         raise ValueError(f"rows of {h} columns (needs a multiple of 32, up to {MAX_H})")
-    xs = rows_of("x", x, m, h, dev)
-    rs = 0 if residual is None else rows_of("residual", residual, m, h, dev, True)
-    if weight.dtype is not _BF16 or weight.shape != (h,) or not weight.is_contiguous() or weight.device != dev:
-        raise ValueError(f"weight: expected contiguous BF16 [{h}] on {dev}")
+    xs = h if x.is_contiguous() else row_stride("x", x, m, h)
+    r_at = rs = ro_at = n_at = c_at = s_at = 0
     ros = ns = h
+    if residual is not None:
+        if residual.dtype is not _BF16 or residual.shape != shape or residual.get_device() != device:
+            raise ValueError(f"residual: expected BF16 [{m}, {h}] on device {device}")
+        rs = h if residual.is_contiguous() else row_stride("residual", residual, m, h, True)
+        r_at = residual.data_ptr()
+    if weight.dtype is not _BF16 or weight.shape != (h,) or not weight.is_contiguous() or weight.get_device() != device:
+        raise ValueError(f"weight: expected contiguous BF16 [{h}] on device {device}")
     if out is None:
-        empty = torch.empty
-        out = TailOutput(None if residual is None else empty((m, h), dtype=_BF16, device=dev),
-                         empty((m, h), dtype=torch.uint8, device=dev) if mxfp8 else None,
-                         empty((m, h // 32), dtype=torch.uint8, device=dev) if mxfp8 else None,
-                         empty((m, h), dtype=_BF16, device=dev) if bf16_out else None)
-        ro, codes, scales, normed = out.residual, out.codes, out.scales, out.normed
-    else:
-        ro, codes, scales, normed = out.residual, out.codes, out.scales, out.normed
-        if ro is not None:
-            if residual is None:
-                raise ValueError("out.residual without a residual")
-            ros = rows_of("out.residual", ro, m, h, dev)
-        if normed is not None:
-            ns = rows_of("out.normed", normed, m, h, dev)
-        if codes is not None or scales is not None:
-            check_mxfp8("out", codes, scales, m, h, dev)
-    if ro is None and normed is None and codes is None:
+        out = TailOutput(None if residual is None else torch.empty(shape, dtype=_BF16, device=x.device),
+                         torch.empty(shape, dtype=_U8, device=x.device) if mxfp8 else None,
+                         torch.empty((m, h // 32), dtype=_U8, device=x.device) if mxfp8 else None,
+                         torch.empty(shape, dtype=_BF16, device=x.device) if bf16_out else None)
+    ro, codes, scales, normed = out.residual, out.codes, out.scales, out.normed
+    if ro is not None:
+        if residual is None:
+            raise ValueError("out.residual without a residual")
+        ros = check_rows("out.residual", ro, shape, device)
+        ro_at = ro.data_ptr()
+    if normed is not None:
+        ns = check_rows("out.normed", normed, shape, device)
+        n_at = normed.data_ptr()
+    if codes is not None or scales is not None:
+        check_mxfp8("out", codes, scales, m, h, device)
+        c_at, s_at = codes.data_ptr(), scales.data_ptr()
+    elif ro is None and normed is None:
         raise ValueError("no output asked for")
-    call = _lib.NORM_CALL.pack(x.data_ptr(), xs, 0 if residual is None else residual.data_ptr(), rs, weight.data_ptr(),
-                               0 if ro is None else ro.data_ptr(), ros, 0 if normed is None else normed.data_ptr(), ns,
-                               0 if codes is None else codes.data_ptr(), 0 if scales is None else scales.data_ptr(), m, h,
-                               weight_offset, eps)
-    launch_on(dev, _lib.load().b200moe_add_rmsnorm_quant, call)
+    launch_on(device, _lib.load().b200moe_add_rmsnorm_quant, _lib.NORM_CALL.pack(
+        x.data_ptr(), xs, r_at, rs, weight.data_ptr(), ro_at, ros, n_at, ns, c_at, s_at, m, h, weight_offset, eps))
     return out

@@ -9,7 +9,7 @@ from dataclasses import dataclass
 import torch
 
 from ... import _lib
-from .add_rmsnorm import check_mxfp8, launch_on, rows_of
+from .add_rmsnorm import check_mxfp8, check_rows, launch_on, row_stride
 from .chain import status_word
 
 MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
@@ -30,10 +30,6 @@ class LinearWeights:
     def n(self) -> int:
         """Output columns."""
         return self.rows // 2 if self.gated else self.rows
-
-    def abi(self) -> bytes:
-        """``struct b200moe_linear_weights`` over this object's tensors as they are now."""
-        return _lib.LINEAR_WEIGHTS.pack(self.tiles.data_ptr(), 0 if self.bias is None else self.bias.data_ptr(), self.rows, self.k, self.gated)
 
     @classmethod
     def from_row_major(cls, w, scale, bias=None, *, gated: bool = False):
@@ -60,7 +56,7 @@ class LinearWeights:
         if codes.data_ptr() & 15:
             codes = codes.clone()
         tiles = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-        launch_on(w.device, _lib.load().b200moe_preshuffle_linear, codes.data_ptr(), scales.data_ptr(), rows, k, int(gated),
+        launch_on(w.get_device(), _lib.load().b200moe_preshuffle_linear, codes.data_ptr(), scales.data_ptr(), rows, k, int(gated),
                   tiles.data_ptr())
         return cls(tiles, bias, rows, k, bool(gated))
 
@@ -68,18 +64,18 @@ class LinearWeights:
 def mxfp8_quant(x: torch.Tensor, *, out=None):
     """bf16 [M, K] -> (E4M3 codes u8 [M, K], E8M0 scales u8 [M, K / 32]): ``shared_quant_rows`` at any width that is a multiple of 32
     (the same bits at 6144; an infinite value saturates and keeps its block's scale finite). Rows any multiple of 8 elements apart."""
-    if x.ndim != 2:
+    if x.ndim != 2 or x.dtype is not torch.bfloat16:
         raise ValueError("expected BF16 [M, K]")
     m, k = x.shape
-    dev = x.device
+    device = x.get_device()
     if k < 32 or k % 32 or k > MAX_DIM or m > MAX_ROWS:
         raise ValueError(f"rows of {k} columns (needs a multiple of 32, up to {MAX_DIM}; up to {MAX_ROWS} rows)")
-    stride = rows_of("x", x, m, k, dev, True)
+    stride = k if x.is_contiguous() else row_stride("x", x, m, k, True)
     if out is None:
-        out = torch.empty((m, k), dtype=torch.uint8, device=dev), torch.empty((m, k // 32), dtype=torch.uint8, device=dev)
+        out = torch.empty((m, k), dtype=torch.uint8, device=x.device), torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
     else:
-        check_mxfp8("out", *out, m, k, dev)
-    launch_on(dev, _lib.load().b200moe_quant_mxfp8, x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr())
+        check_mxfp8("out", *out, m, k, device)
+    launch_on(device, _lib.load().b200moe_quant_mxfp8, x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr())
     return out
 
 
@@ -98,39 +94,41 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
         raise ValueError(f"unknown activation {activation!r}")
     if (act >= 5) != w.gated:
         raise ValueError(f"activation {activation!r} on {'gated' if w.gated else 'plain'} weights")
-    k, n, dev = w.k, w.n, w.tiles.device
-    if dev.type != "cuda":
-        raise ValueError(f"expected weights on a CUDA device, got {dev}")
-    xs = x_at = 0
+    tiles, bias, rows, k, gated = w.tiles, w.bias, w.rows, w.k, w.gated
+    n, device = rows // 2 if gated else rows, tiles.get_device()
+    x_at = xs = r_at = rs = y_at = oc_at = os_at = 0
+    ys = n
     if isinstance(x, torch.Tensor):
-        if x.ndim != 2:
-            raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
+        if x.dtype is not torch.bfloat16 or x.ndim != 2 or x.shape[1] != k or x.get_device() != device:
+            raise ValueError(f"x: expected BF16 [M, {k}] (or a pair of codes and scales) on device {device}")
         m = x.shape[0]
-        xs, x_at = rows_of("x", x, m, k, dev, True), x.data_ptr()
-        rows8 = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=dev)  # the quantised rows
-        c_at = rows8.data_ptr()
+        xs, x_at = k if x.is_contiguous() else row_stride("x", x, m, k, True), x.data_ptr()
+        quantised = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=x.device)
+        c_at = quantised.data_ptr()
         s_at = c_at + m * k
-    elif isinstance(x, (tuple, list)) and len(x) == 2 and x[0] is not None and x[0].ndim == 2:
+    elif isinstance(x, (tuple, list)) and len(x) == 2 and x[0] is not None:
         codes, scales = x
-        m = codes.shape[0]
-        check_mxfp8("x", codes, scales, m, k, dev)
+        m = codes.shape[0] if codes.ndim else 0
+        check_mxfp8("x", codes, scales, m, k, device)
         c_at, s_at = codes.data_ptr(), scales.data_ptr()
     else:
         raise ValueError("expected BF16 [M, K] rows or a pair of codes and scales")
-    rs = 0 if residual is None else rows_of("residual", residual, m, n, dev)
-    os, y, oc, osc = n, 0, 0, 0
+    if residual is not None:
+        rs, r_at = check_rows("residual", residual, (m, n), device), residual.data_ptr()
     if out is None:
         if mxfp8_out:
-            out = torch.empty((m, n), dtype=torch.uint8, device=dev), torch.empty((m, n // 32), dtype=torch.uint8, device=dev)
+            out = torch.empty((m, n), dtype=torch.uint8, device=tiles.device), torch.empty((m, n // 32), dtype=torch.uint8, device=tiles.device)
         else:
-            out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+            out = torch.empty((m, n), dtype=torch.bfloat16, device=tiles.device)
     if isinstance(out, torch.Tensor):
-        os, y = rows_of("out", out, m, n, dev), out.data_ptr()
+        ys, y_at = check_rows("out", out, (m, n), device), out.data_ptr()
     else:
         if n % 32:
             raise ValueError(f"MXFP8 output of {n} columns (needs a multiple of 32)")
-        check_mxfp8("out", *out, m, n, dev)
-        oc, osc = out[0].data_ptr(), out[1].data_ptr()
-    call = _lib.LINEAR_CALL.pack(x_at, xs, c_at, s_at, m, 0 if residual is None else residual.data_ptr(), rs, y, os, oc, osc, act)
-    launch_on(dev, _lib.load().b200moe_linear, w.abi(), call, status_word(dev).data_ptr())
+        check_mxfp8("out", *out, m, n, device)
+        oc_at, os_at = out[0].data_ptr(), out[1].data_ptr()
+    status = status_word(tiles.device).data_ptr() if device >= 0 else 0
+    launch_on(device, _lib.load().b200moe_linear, _lib.LINEAR_CALL.pack(
+        tiles.data_ptr(), 0 if bias is None else bias.data_ptr(), rows, k, gated, x_at, xs, c_at, s_at, m, r_at, rs, y_at, ys, oc_at,
+        os_at, act), status)
     return out

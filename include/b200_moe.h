@@ -478,6 +478,7 @@ typedef struct b200moe_linear_weights {
  * of x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
  * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG. m may be 0. */
 typedef struct b200moe_linear_call {
+  b200moe_linear_weights w;
   const void* x; /* or null */
   int64_t x_stride;
   uint8_t* codes8;
@@ -491,7 +492,7 @@ typedef struct b200moe_linear_call {
   uint8_t* out_scales8;
   int activation;
 } b200moe_linear_call;
-int b200moe_linear(const b200moe_linear_weights* w, const b200moe_linear_call* call, int32_t* status, void* stream);
+int b200moe_linear(const b200moe_linear_call* call, int32_t* status, void* stream);
 
 /* The whole layer in one call, with or without the shared expert (MOE/chain.py:127-197 mxfp4_moe; the shared expert runs
  * beside the routed experts inside the same launches up to 512 tokens; above, its two GEMMs are launches of their own, on

@@ -21,6 +21,13 @@ def test_both_packages_have_them():
         assert name in P.__all__ and name in P2.__all__ and getattr(P, name) is getattr(P2, name)
 
 
+def refused(call, *args, why=None, **kw):
+    """A ValueError; for another reason than that nothing is launched on host tensors, unless ``why`` says so."""
+    with pytest.raises(ValueError) as e:
+        call(*args, **kw)
+    assert ("nothing is launched" in str(e.value)) == (why == "nothing is launched"), str(e.value)
+
+
 # ------------------------------------------------------------------------------------------------ the norm
 def norm_call(lib, x=4096, xs=64, r=1 << 20, rs=64, w=256, rows=4, h=64, ro=2 << 20, ros=64, n=3 << 20, ns=64, c=4 << 20, s=5 << 20):
     p = [0 if a is None else a for a in (x, r, w, ro, n, c, s)]
@@ -60,9 +67,10 @@ def test_norm_refuses_bad_tensors():
                      ((x, r, w), dict(out=out(codes=torch.zeros((4, 64), dtype=U8), scales=torch.zeros((4, 3), dtype=U8)))),
                      ((x, r, w), dict(out=out(codes=torch.zeros((4, 64), dtype=torch.int16), scales=torch.zeros((4, 2), dtype=U8)))),
                      ((x, r, w), dict(out=out(normed=torch.zeros((4, 64))))),
-                     ((x, r.to("meta"), w), {}), ((x, r, w.to("meta")), {}), ((x, r, w), {})]:  # (the last: host tensors)
-        with pytest.raises(ValueError):
-            P.add_rmsnorm_mxfp8(*args, **kw)
+                     ((x, r[::2], w), {}), ((x, r, torch.zeros(128, dtype=BF16)[::2]), {})]:
+        refused(P.add_rmsnorm_mxfp8, *args, **kw)
+    refused(P.add_rmsnorm_mxfp8, x, r, w, why="nothing is launched")  # all is well but that the tensors are the host's
+    refused(P.add_rmsnorm_mxfp8, x, None, w, out=out(normed=x), why="nothing is launched")
 
 
 # ------------------------------------------------------------------------------------------------ the product
@@ -74,8 +82,8 @@ def weights(rows=64, k=96, gated=False, bias=False):
 def linear_call(lib, rows=64, k=96, gated=0, tiles=256, bias=None, c=1 << 20, s=2 << 20, m=4, act=0, r=None, rs=64, o=3 << 20, os=64,
                 oc=None, osc=None, status=256, x=None, xs=96):
     p = [0 if a is None else a for a in (tiles, bias, c, s, r, o, oc, osc)]
-    return lib.b200moe_linear(_lib.LINEAR_WEIGHTS.pack(p[0], p[1], rows, k, gated),
-                              _lib.LINEAR_CALL.pack(0 if x is None else x, xs, p[2], p[3], m, p[4], rs, p[5], os, p[6], p[7], act), at(status), None)
+    return lib.b200moe_linear(_lib.LINEAR_CALL.pack(p[0], p[1], rows, k, gated, 0 if x is None else x, xs, p[2], p[3], m, p[4], rs, p[5], os,
+                                                    p[6], p[7], act), at(status), None)
 
 
 @pytest.mark.parametrize("inter", [768, 1536])
@@ -124,13 +132,13 @@ def test_product_refuses_bad_tensors():
                      ((x, w), dict(residual=bf(4, 68)[:, :64])), ((x, w), dict(residual=bf(1, 64).expand(4, 64))), ((x, w), dict(out=bf(4, 72))), ((x, w), dict(out=torch.zeros((4, 64)))),
                      ((x, w), dict(out=bf(1, 64).expand(4, 64))), ((x, w), dict(out=(u8(4, 64), u8(4, 3)))), ((x, w), dict(out=(u8(4, 64), None))),
                      ((x, w), dict(out=(None, None))), ((x, weights(rows=40)), dict(mxfp8_out=True)),
-                     ((x, w), dict(residual=bf(4, 64).to("meta"))), (((u8(4, 96).to("meta"), u8(4, 3).to("meta")), w), {}),
-                     ((x, w), {}), ((bf(4, 96), w), {})]:  # (the last two: host tensors)
-        with pytest.raises(ValueError):
-            P.mxfp8_linear(*args, **kw)
+                     ((x, g), dict(activation="swiglu", residual=bf(4, 64))), ((bf(4, 100)[:, :96], w), {})]:
+        refused(P.mxfp8_linear, *args, **kw)
     for bad in (bf(4, 40), bf(96), u8(4, 96), torch.zeros((4, 96)), bf(4, 200)[:, ::2], bf(4, 100)[:, :96]):
-        with pytest.raises(ValueError):
-            P.mxfp8_quant(bad)
+        refused(P.mxfp8_quant, bad)
+    for args, kw in [((x, w), {}), ((bf(4, 96), w), dict(residual=bf(4, 64))), ((x, g), dict(activation="swiglu_oai", mxfp8_out=True))]:
+        refused(P.mxfp8_linear, *args, **kw, why="nothing is launched")
+    refused(P.mxfp8_quant, bf(4, 96), why="nothing is launched")
 
 
 def test_weights_refuse_bad_tensors():
@@ -140,9 +148,5 @@ def test_weights_refuse_bad_tensors():
             P.LinearWeights.from_row_major(*args)  # host tensors, types, ranks
 
 
-def test_layout_and_struct():
-    w = weights(bias=True)
-    assert w.abi() == _lib.LINEAR_WEIGHTS.pack(w.tiles.data_ptr(), w.bias.data_ptr(), 64, 96, 0)
-    w.bias = None
-    assert w.abi() == _lib.LINEAR_WEIGHTS.pack(w.tiles.data_ptr(), 0, 64, 96, 0)
-    assert weights(gated=True).n == 32 and L.MAX_DIM == 1 << 20
+def test_output_columns():
+    assert weights(gated=True).n == 32 and weights().n == 64 and L.MAX_DIM == 1 << 20
