@@ -8,7 +8,7 @@ import torch
 from ... import _lib
 from .tail import TailOutput
 
-MAX_H = 65536
+MAX_H = 32768
 _BF16, _U8 = torch.bfloat16, torch.uint8
 
 
@@ -58,7 +58,7 @@ def add_rmsnorm_mxfp8(x: torch.Tensor, residual: torch.Tensor | None, weight: to
                       out: TailOutput | None = None) -> TailOutput:
     """``s = x + residual`` in fp32 (residual out ``bf16(s)``), ``y = s * rstd * (weight + weight_offset)``, MXFP8 of the fp32 ``y``
     and / or ``bf16(y)``: steps 2-4 of ``amd_kernels/norm/gemma_add_rmsnorm_h6144/reference.py`` (whose weight offset is 1; 0 is
-    the plain RMS norm) at any width H that is a multiple of 32, up to 65536.
+    the plain RMS norm) at any width H that is a multiple of 32, up to 32768.
 
     ``x`` and ``residual`` bf16 [M, H], rows any multiple of 8 elements apart; M may be 0. ``residual`` None: ``s = x``, and no residual
     comes back. A residual expanded from one row (stride 0) is added to every row. ``out``: where the results go; its tensors

@@ -419,7 +419,7 @@ int b200moe_forward_x(const b200moe_weights* w, const void* x_bf16, int64_t toke
  * stride of 0 is one row for all), weight bf16 [h]; 16-byte aligned, codes8 8-byte. h: a multiple of 32, up to
  * B200MOE_NORM_MAX_H. residual_out or normed may be x or residual (the same address and stride); any other overlap of an output is
  * B200MOE_E_ARG. The bits of a row do not depend on the other rows. rows may be 0. */
-#define B200MOE_NORM_MAX_H 65536
+#define B200MOE_NORM_MAX_H 32768
 typedef struct b200moe_norm_call {
   const void* x;
   int64_t x_stride;

@@ -53,7 +53,7 @@ def check_codes(codes, scales, y, lowest, delta, slack=0.0):
     assert bool(((v - y).abs() <= (2.0 ** -4 + 2 * delta) * y.abs() + 2.0 ** -10 * got_scale + 2 * slack).all())
 
 
-WIDTHS = [32, 64, 96, 256, 288, 544, 1024, 1056, 2080, 4064, 4096, 6144, 6176, 8192, 16384, 16416]
+WIDTHS = [32, 64, 96, 256, 288, 544, 1024, 1056, 2080, 4064, 4096, 6144, 6176, 8192, 16384, 16416, 32768]
 
 
 @pytest.mark.parametrize("h", WIDTHS)
