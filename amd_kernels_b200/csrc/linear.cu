@@ -180,22 +180,25 @@ static int linear_args(LinearArgs& a, const b200moe_linear_call* call, const int
   if (c.activation < B200MOE_ACT_NONE || c.activation > B200MOE_ACT_SWIGLU_OAI) return B200MOE_E_ARG;
   if ((w->gated != 0) != (c.activation >= B200MOE_ACT_SWIGLU)) return B200MOE_E_ARG;
   if (m == 0) return 0;
-  if (!w->tiles || !c.codes8 || !c.scales8 || !status) return B200MOE_E_ARG;
+  const bool inside = c.x && m <= B200MOE_LINEAR_ROWS_INSIDE;
+  if (!w->tiles || !status || (!inside && (!c.codes8 || !c.scales8))) return B200MOE_E_ARG;
   if ((c.out != nullptr) == (c.out_codes8 != nullptr) || (c.out_codes8 != nullptr) != (c.out_scales8 != nullptr)) return B200MOE_E_ARG;
   const int64_t n = w->gated ? w->rows / 2 : w->rows;
   if (c.out_codes8 && n % 32) return B200MOE_E_ARG;
+  if (c.x && m > 1 && c.x_stride < w->k && c.x_stride != 0) return B200MOE_E_ARG;
   if (m > 1 && ((c.out && c.out_stride < n) || (c.residual && c.residual_stride < n))) return B200MOE_E_ARG;
   const auto bad_rows = [m](const void* p, int64_t stride) { return misaligned(p, 16) || (p && m > 1 && (stride & 7)); };
-  if (misaligned(w->tiles, 128) || misaligned(w->bias, 16) || misaligned(c.codes8, 16) || misaligned(c.out_codes8, 16) ||
+  if (misaligned(w->tiles, 128) || misaligned(w->bias, 16) || bad_rows(c.x, c.x_stride) || misaligned(c.codes8, 16) || misaligned(c.out_codes8, 16) ||
       bad_rows(c.out, c.out_stride) || bad_rows(c.residual, c.residual_stride))
     return B200MOE_E_ALIGN;
   // the rows of out may be those of the residual (a thread stores where it has loaded); any other overlap with an input is refused
   const void* outs[3] = {c.out, c.out_codes8, c.out_scales8};
   const size_t rows = static_cast<size_t>(m);
   const size_t out_bytes[3] = {((rows - 1) * c.out_stride + n) * 2, rows * n, rows * (n / 32)};
-  const size_t res_bytes = ((rows - 1) * c.residual_stride + n) * 2;
+  const size_t res_bytes = ((rows - 1) * c.residual_stride + n) * 2, x_bytes = ((rows - 1) * c.x_stride + w->k) * 2;
   for (int i = 0; i < 3; ++i) {
-    if (overlap(outs[i], out_bytes[i], c.codes8, rows * w->k) || overlap(outs[i], out_bytes[i], c.scales8, rows * (w->k / 32)))
+    if (inside && overlap(outs[i], out_bytes[i], c.x, x_bytes)) return B200MOE_E_ARG;
+    if (!inside && (overlap(outs[i], out_bytes[i], c.codes8, rows * w->k) || overlap(outs[i], out_bytes[i], c.scales8, rows * (w->k / 32))))
       return B200MOE_E_ARG;
     const bool same = i == 0 && c.out == c.residual && (m == 1 || c.out_stride == c.residual_stride);
     if (!same && overlap(outs[i], out_bytes[i], c.residual, res_bytes)) return B200MOE_E_ARG;
@@ -203,6 +206,8 @@ static int linear_args(LinearArgs& a, const b200moe_linear_call* call, const int
   if (overlap(c.out_codes8, out_bytes[1], c.out_scales8, out_bytes[2])) return B200MOE_E_ARG;
   a.tiles = w->tiles;
   a.bias = w->bias;
+  a.x = inside ? static_cast<const __nv_bfloat16*>(c.x) : nullptr;
+  a.x_stride = c.x_stride;
   a.codes = c.codes8;
   a.scales = c.scales8;
   a.residual = static_cast<const __nv_bfloat16*>(c.residual);
@@ -227,6 +232,6 @@ extern "C" int b200moe_linear(const b200moe_linear_call* call, int32_t* status, 
   LinearArgs a;
   int r = linear_args(a, call, status);
   if (r || a.m == 0) return r;
-  if (call->x && (r = b200moe_quant_mxfp8(call->x, call->x_stride, call->m, call->w.k, call->codes8, call->scales8, stream))) return r;
+  if (call->x && !a.x && (r = b200moe_quant_mxfp8(call->x, call->x_stride, call->m, call->w.k, call->codes8, call->scales8, stream))) return r;
   return dispatch_linear(a, status, static_cast<cudaStream_t>(stream));
 }

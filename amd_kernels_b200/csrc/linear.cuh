@@ -33,11 +33,12 @@ struct LinearArgs {
   const float* bias;              // [weight rows] or null
   const uint8_t* codes;           // [m][k]
   const uint8_t* scales;          // [m][k / 32]
+  const __nv_bfloat16* x;         // where the kernel quantises the rows itself: rows x_stride apart, in place of codes and scales
   const __nv_bfloat16* residual;  // rows residual_stride apart, or null
   __nv_bfloat16* out;             // rows out_stride apart; or null:
   uint8_t* out_codes;             // [m][n]
   uint8_t* out_scales;            // [m][n / 32]
-  int64_t m, residual_stride, out_stride;
+  int64_t m, x_stride, residual_stride, out_stride;
   int k, n;  // n: output columns
   int tiles_n, tiles_k;
   LinearAct act;

@@ -11,22 +11,26 @@
 //   warp 2     scales: shared memory -> tensor memory
 //   warp 3     scale producer: the weights' atoms (bulk copy); the tokens' from row-major global memory through registers
 //   warps 4-7  the sum out of tensor memory; all warps take part in what follows
+//
+// QUANT, for a few bf16 rows: there is no launch that quantises them. Warps 4-7, idle until the sum is there, quantise the block's rows
+// K-tile by K-tile into the stage, codes and scale atom, while the weights stream; every CTA does it again for its weight tile (the
+// rows are a few hundred KB in L2). A stage is then one barrier: image, weight atom and tokens.
 #include "linear.cuh"
 #include "tc_pair.cuh"
 
 namespace b200moe {
 
-template <int BM>
+template <int BM, bool QUANT = false>
 struct LinearCfg {
   static constexpr int kTokOff = kLinearImageBytes;               // token rows behind the weight image
   static constexpr int kStageBytes = kTokOff + BM * 128;
   static constexpr int kCtasPerSm = 2;                            // one's start and end under the other's stream
   static constexpr int kStages = BM > 64 ? 3 : BM > 32 ? 4 : 5;
-  static constexpr int kSfSlots = BM == 32 ? 2 : 3;               // groups of scales in shared memory
+  static constexpr int kSfSlots = BM == 32 ? 2 : 3;               // groups of scales in shared memory; QUANT: a slot a stage
   static constexpr int kSfOff = kStages * kStageBytes;
   static constexpr int kSfSlotBytes = kSfGroup * 2 * kAtomBytes;  // weight atoms of the group, then token atoms
   static constexpr int kSumRow = 132;                             // floats of a token's 128 columns in the parts (alias the ring)
-  static constexpr int kSmemBytes = kSfOff + kSfSlots * kSfSlotBytes + 1024;
+  static constexpr int kSmemBytes = kSfOff + (QUANT ? kStages * 2 * kAtomBytes : kSfSlots * kSfSlotBytes) + 1024;
   static constexpr int kSfCols = 8;                               // tensor memory columns of a K-tile's scales: 4 weights, 4 tokens
   static constexpr int kColsUsed = BM + kSfSets * kSfGroup * kSfCols;
   static constexpr int kTmemCols = kColsUsed <= 128 ? 128 : 256;
@@ -103,16 +107,16 @@ __device__ __forceinline__ void finish_rows(const LinearArgs& a, int64_t row0, i
   }
 }
 
-template <int BM>
+template <int BM, bool QUANT>
 __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     linear_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs args, int splits, int n_blocks,
                      int32_t* status) {
-  using C = LinearCfg<BM>;
+  using C = LinearCfg<BM, QUANT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[C::kStages];   // weight image and token rows of the stage have landed
   __shared__ __align__(8) uint64_t bar_empty[C::kStages];  // the MMAs that read it have completed
   __shared__ __align__(8) uint64_t bar_sfull[C::kSfSlots];    // the scales of the group are in shared memory
-  __shared__ __align__(8) uint64_t bar_sf[C::kSfSlots];       // they are in tensor memory
+  __shared__ __align__(8) uint64_t bar_sf[QUANT ? C::kStages : C::kSfSlots];  // they (QUANT: the stage's) are in tensor memory
   __shared__ __align__(8) uint64_t bar_set[kSfSets];       // the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull;
   __shared__ __align__(8) uint64_t bar_drain[2];
@@ -127,12 +131,13 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_full[s]), QUANT ? 5 : 1);  // the byte count; QUANT: four warps' tokens too
       mbar_init(smem_u32(&bar_empty[s]), 1);
+      if (QUANT) mbar_init(smem_u32(&bar_sf[s]), 1);
     }
     for (int j = 0; j < C::kSfSlots; ++j) {
       mbar_init(smem_u32(&bar_sfull[j]), 2);  // the byte count of the weights' atoms, the tokens' atoms
-      mbar_init(smem_u32(&bar_sf[j]), 1);
+      if (!QUANT) mbar_init(smem_u32(&bar_sf[j]), 1);
     }
     for (int j = 0; j < kSfSets; ++j) mbar_init(smem_u32(&bar_set[j]), 1);
     mbar_init(smem_u32(&bar_tfull), 1);
@@ -169,10 +174,65 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   launder(a.tiles);
   launder(a.atoms);
   launder(a.scales);
+  launder(a.x);
   launder(a.bias);
   launder(a.residual);
 
-  if (warp == 0) {
+  if (QUANT && warp == 0) {
+    if (lane == 0) {  // ------------------------------------------------ QUANT: weights, images and atoms
+      const int64_t at = static_cast<int64_t>(tile) * a.tiles_k;
+      uint32_t it = 0, s = 0, ph = 1u;
+      bool ok = true;
+      for (int kt = kt0; kt < kt1; ++kt, ++it) {
+        if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
+        const uint32_t full = smem_u32(&bar_full[s]);
+        mbar_arrive_expect_tx(full, kLinearTileBytes);
+        bulk_load(tiles + s * C::kStageBytes, a.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes, full);
+        bulk_load(tiles + C::kSfOff + s * 2 * kAtomBytes, a.atoms + (at + kt) * kAtomBytes, kAtomBytes, full);
+        if (++s == C::kStages) { s = 0; ph ^= 1u; }
+      }
+      if (!ok) drain_copies(bar_full, it, C::kStages);
+    }
+  } else if (QUANT && warp == 1) {
+    // ------------------------------------------------ QUANT: MMA issue
+    constexpr uint32_t kIdesc = (static_cast<uint32_t>(BM >> 3) << 17) | (1u << 23) | (8u << 24);
+    uint32_t s = 0, ph = 0;
+    bool ok = true;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      if (!warp_wait(smem_u32(&bar_sf[s]), ph, abort_v, status)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t w_lo = (tiles + s * C::kStageBytes) >> 4, x_lo = w_lo + (C::kTokOff >> 4);
+      const uint32_t t_sfw = tmem_base + BM + s * C::kSfCols, t_sfx = t_sfw + C::kSfCols / 2;
+      if (elect_one()) {
+        tc_mma_mxf8_lo<2>(tmem_base, w_lo, x_lo, kIdesc, t_sfw, t_sfx, static_cast<uint32_t>(kt != kt0));
+        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 2, x_lo + 2, kIdesc | (1u << 29) | (1u << 4), t_sfw, t_sfx);
+        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 4, x_lo + 4, kIdesc | (2u << 29) | (2u << 4), t_sfw, t_sfx);
+        tc_mma_mxf8_lo<1>(tmem_base, w_lo + 6, x_lo + 6, kIdesc | (3u << 29) | (3u << 4), t_sfw, t_sfx);
+        tc_commit(smem_u32(&bar_empty[s]));
+      }
+      __syncwarp();
+      if (++s == C::kStages) { s = 0; ph ^= 1u; }
+    }
+    if (ok && elect_one()) tc_commit(smem_u32(&bar_tfull));
+    if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[0]));
+  } else if (QUANT && warp == 2) {
+    // ------------------------------------------------ QUANT: scale copies (the set of a stage is free once the stage is)
+    uint32_t s = 0, ph = 0;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      if (!warp_wait(smem_u32(&bar_full[s]), ph, abort_v, status)) break;
+      tc_fence_after();
+      const uint32_t atoms = (tiles + C::kSfOff + s * 2 * kAtomBytes) >> 4, t_sfw = tmem_base + BM + s * C::kSfCols;
+      if (elect_one()) {
+        tc_cp_scales_lo(t_sfw, atoms);
+        tc_cp_scales_lo(t_sfw + C::kSfCols / 2, atoms + (kAtomBytes >> 4));
+        tc_commit(smem_u32(&bar_sf[s]));
+      }
+      __syncwarp();
+      if (++s == C::kStages) { s = 0; ph ^= 1u; }
+    }
+    if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[1]));
+  } else if (QUANT && warp == 3) {
+  } else if (!QUANT && warp == 0) {
     scales_first_wait();
     if (lane == 0) {  // ------------------------------------------------ code producer
       const uint8_t* w_src = a.tiles + (static_cast<int64_t>(tile) * a.tiles_k + kt0) * kLinearImageBytes;
@@ -188,7 +248,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       }
       if (!ok) drain_copies(bar_full, it, C::kStages);
     }
-  } else if (warp == 1) {
+  } else if (!QUANT && warp == 1) {
     // ------------------------------------------------ MMA issue: E4M3 x E4M3, UE8M0 scales, M = 128, N = BM
     constexpr uint32_t kIdesc = (static_cast<uint32_t>(BM >> 3) << 17) | (1u << 23) | (8u << 24);
     uint32_t s = 0, ph = 0, slot = 0, sph = 0, set = 0;
@@ -220,7 +280,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     }
     if (ok && elect_one()) tc_commit(smem_u32(&bar_tfull));
     if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[0]));
-  } else if (warp == 2) {
+  } else if (!QUANT && warp == 2) {
     // ------------------------------------------------ scale copies into tensor memory
     uint32_t slot = 0, ph = 0, set = 0, set_ph = 1u;
     for (int kt = kt0; kt < kt1; kt += kSfGroup) {
@@ -243,7 +303,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       if (++set == kSfSets) { set = 0; set_ph ^= 1u; }
     }
     if (__any_sync(0xffffffffu, *abort_v != 0) && elect_one()) drain_tcgen05(smem_u32(&bar_drain[1]));
-  } else if (warp == 3) {
+  } else if (!QUANT && warp == 3) {
     // ------------------------------------------------ scale producer: lane l writes an atom's 16 bytes of rows l, l + 32, l + 64, l + 96.
     // A group's bytes are asked for two groups ahead.
     constexpr int kRows = (BM + 31) / 32;
@@ -284,6 +344,52 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     }
     if (!ok && lane == 0) drain_copies(bar_sfull, it, C::kSfSlots);
   } else {
+    if (QUANT) {
+      // ---------------------------------------------- the block's rows: 16 lanes to a row's 256 bytes of a K-tile, four lanes to a scale
+      constexpr int kItems = BM * 16 / 128;
+      const int et = threadIdx.x - 128, c = et & 15;
+      uint4 next[kItems];
+      const auto fetch = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const int64_t row = row0 + (i * 128 + et) / 16;
+          const int col = kt * 128 + c * 8;
+          next[i] = kt < kt1 && row < a.m && col < a.k ? __ldcg(reinterpret_cast<const uint4*>(a.x + row * a.x_stride + col)) : uint4{};
+        }
+      };
+      uint32_t s = 0, ph = 1u;
+      fetch(kt0);
+      for (int kt = kt0; kt < kt1; ++kt) {
+        uint4 now[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) now[i] = next[i];
+        fetch(kt + 1);
+        if (!warp_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) break;
+        uint8_t* const codes = tiles_ptr + s * C::kStageBytes + C::kTokOff;
+        uint8_t* const atom = tiles_ptr + C::kSfOff + s * 2 * kAtomBytes + kAtomBytes;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const int r = (i * 128 + et) / 16;
+          float v[8];
+          unpack_bf16x8(now[i], v);
+          float amax = max3_abs(max3_abs(v[0], v[1], v[2]), max3_abs(v[3], v[4], v[5]), max3_abs(v[6], v[7], 0.0f));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int e = linear_scale(amax);
+          const float inv = e8m0_value(static_cast<uint32_t>(254 - e));
+          *reinterpret_cast<uint2*>(codes + r * 128 + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8) =
+              make_uint2(pack_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), pack_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+          uint32_t sc = static_cast<uint32_t>(e);
+          sc |= __shfl_down_sync(0xffffffffu, sc, 4) << 8;
+          sc |= __shfl_down_sync(0xffffffffu, sc, 8) << 16;
+          if (c == 0) *reinterpret_cast<uint32_t*>(atom + atom_offset(r, 0)) = sc;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_full[s]));
+        if (++s == C::kStages) { s = 0; ph ^= 1u; }
+      }
+    }
     // ------------------------------------------------ the part: lane = weight row, column = token. All copies have landed and all MMAs have
     // read them (the last commit), so the ring's memory is free.
     const int q = warp & 3;
@@ -332,20 +438,21 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   }
 }
 
-template <int BM>
+template <int BM, bool QUANT>
 static int configure_linear_tc() {
   static PerDeviceOnce once;
   return once.run([] {
-    return static_cast<int>(cudaFuncSetAttribute(linear_tc_kernel<BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinearCfg<BM>::kSmemBytes));
+    return static_cast<int>(
+        cudaFuncSetAttribute(linear_tc_kernel<BM, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinearCfg<BM, QUANT>::kSmemBytes));
   });
 }
 
-template <int BM>
+template <int BM, bool QUANT>
 static cudaLaunchConfig_t linear_tc_config(int64_t clusters, int splits, cudaLaunchAttribute (&attr)[2], cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * splits));
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = LinearCfg<BM>::kSmemBytes;
+  cfg.dynamicSmemBytes = LinearCfg<BM, QUANT>::kSmemBytes;
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -358,17 +465,17 @@ static cudaLaunchConfig_t linear_tc_config(int64_t clusters, int splits, cudaLau
   return cfg;
 }
 
-template <int BM>
+template <int BM, bool QUANT>
 static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cudaStream_t stream) {
-  int r = configure_linear_tc<BM>();
+  int r = configure_linear_tc<BM, QUANT>();
   if (r) return r;
-  CUtensorMap mx;
-  if ((r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), BM))) return r;
+  CUtensorMap mx = {};
+  if (!QUANT && (r = make_map(&mx, a.codes, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), BM))) return r;
   const int64_t n_blocks = (a.m + BM - 1) / BM, units = n_blocks * a.tiles_n;
   if (units * splits > 0x7fffffff) return B200MOE_E_ARG;
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = linear_tc_config<BM>(units, splits, attr, stream);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM>, mx, a, splits, static_cast<int>(n_blocks), status));
+  const cudaLaunchConfig_t cfg = linear_tc_config<BM, QUANT>(units, splits, attr, stream);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM, QUANT>, mx, a, splits, static_cast<int>(n_blocks), status));
 }
 
 // Clusters of `1 << log_splits` CTAs that run at once on the current device; asked once per device. The occupancy calculation counts one CTA
@@ -379,14 +486,14 @@ static int resident_clusters(int log_splits) {
   static std::mutex mu;
   static int known[kMaxDevices][4] = {};  // 1 + the number
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || configure_linear_tc<BM>()) return 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || configure_linear_tc<BM, false>()) return 0;
   std::lock_guard<std::mutex> lock(mu);
   int& n = known[dev][log_splits];
   if (n == 0) {
     int got = sm_count();
     cudaLaunchAttribute attr[2];
-    const cudaLaunchConfig_t cfg = linear_tc_config<BM>(sm_count(), 1 << log_splits, attr, nullptr);
-    if (log_splits > 0 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM>, &cfg) != cudaSuccess) got = 0;
+    const cudaLaunchConfig_t cfg = linear_tc_config<BM, false>(sm_count(), 1 << log_splits, attr, nullptr);
+    if (log_splits > 0 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM, false>, &cfg) != cudaSuccess) got = 0;
     (void)cudaGetLastError();
     n = 1 + LinearCfg<BM>::kCtasPerSm * got;
   }
@@ -400,14 +507,14 @@ int linear_tc_resident(int bm, int log_splits) {
                     : resident_clusters<128>(log_splits);
 }
 
-// bm: 16, 32, 64 or 128 token rows a block; splits: 1, 2, 4 or 8 CTAs along K, at most the K-tiles
+// bm: 16, 32, 64 or 128 token rows a block (a.x given: 16, 32 or 64); splits: 1, 2, 4 or 8 CTAs along K, at most the K-tiles
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream) {
   switch (bm) {
-    case 16: return launch_linear_tc<16>(a, splits, status, stream);
-    case 32: return launch_linear_tc<32>(a, splits, status, stream);
-    case 64: return launch_linear_tc<64>(a, splits, status, stream);
+    case 16: return a.x ? launch_linear_tc<16, true>(a, splits, status, stream) : launch_linear_tc<16, false>(a, splits, status, stream);
+    case 32: return a.x ? launch_linear_tc<32, true>(a, splits, status, stream) : launch_linear_tc<32, false>(a, splits, status, stream);
+    case 64: return a.x ? launch_linear_tc<64, true>(a, splits, status, stream) : launch_linear_tc<64, false>(a, splits, status, stream);
   }
-  return launch_linear_tc<128>(a, splits, status, stream);
+  return launch_linear_tc<128, false>(a, splits, status, stream);
 }
 
 int set_wait_limit_linear_tc(unsigned long long ns) { return set_wait_limit_here(ns); }

@@ -13,6 +13,7 @@ from .add_rmsnorm import check_mxfp8, check_rows, launch_on, row_stride
 from .chain import status_word
 
 MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
+ROWS_INSIDE = 64  # up to so many bf16 rows are quantised inside the product's launch
 
 
 @dataclass
@@ -83,7 +84,8 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
                  mxfp8_out: bool = False, out=None):
     """``y = activation(x @ w.T + bias) + residual``, fp32 until one rounding at the end.
 
-    ``x``: MXFP8 rows as a pair (codes [M, K], scales [M, K / 32]), or bf16 [M, K], which ``mxfp8_quant`` quantises first. M may be 0.
+    ``x``: MXFP8 rows as a pair (codes [M, K], scales [M, K / 32]), or bf16 [M, K], quantised as by
+    ``mxfp8_quant`` (up to 64 rows inside the product's launch, more in one in front of it; the same bits). M may be 0.
     ``activation``: None, "relu", "silu", "gelu" (exact), "gelu_tanh"; for gated weights "swiglu" (silu(gate) * up) or "swiglu_oai"
     (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart.
     Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.
@@ -103,9 +105,11 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
             raise ValueError(f"x: expected BF16 [M, {k}] (or a pair of codes and scales) on device {device}")
         m = x.shape[0]
         xs, x_at = k if x.is_contiguous() else row_stride("x", x, m, k, True), x.data_ptr()
-        quantised = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=x.device)
-        c_at = quantised.data_ptr()
-        s_at = c_at + m * k
+        c_at = s_at = 0
+        if m > ROWS_INSIDE:
+            quantised = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=x.device)
+            c_at = quantised.data_ptr()
+            s_at = c_at + m * k
     elif isinstance(x, (tuple, list)) and len(x) == 2 and x[0] is not None:
         codes, scales = x
         m = codes.shape[0] if codes.ndim else 0

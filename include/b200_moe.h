@@ -447,6 +447,7 @@ int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* stream);
  * k: a multiple of 32. Weight rows: a multiple of 8, with MXFP8 output of 32, gated of 64. */
 #define B200MOE_LINEAR_MAX_DIM (1 << 20)
 #define B200MOE_LINEAR_MAX_ROWS (1 << 24)
+#define B200MOE_LINEAR_ROWS_INSIDE 64
 #define B200MOE_ACT_NONE 0
 #define B200MOE_ACT_RELU 1
 #define B200MOE_ACT_SILU 2
@@ -473,10 +474,12 @@ typedef struct b200moe_linear_weights {
   int gated;
 } b200moe_linear_weights;
 
-/* x: codes8 (16-byte aligned) and scales8; or bf16 rows x (16-byte aligned), which are first quantised into codes8 and scales8 by a launch
+/* x: codes8 (16-byte aligned) and scales8; or bf16 rows x (16-byte aligned), quantised by the rule above: up to
+ * B200MOE_LINEAR_ROWS_INSIDE rows inside the product (codes8 and scales8 are not used), more of them into codes8 and scales8 by a launch
  * in front (b200moe_quant_mxfp8). residual, out and x are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a stride of 0
  * of x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
- * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG. m may be 0. */
+ * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG (bf16
+ * rows that a launch in front quantises may be overwritten). m may be 0. */
 typedef struct b200moe_linear_call {
   b200moe_linear_weights w;
   const void* x; /* or null */

@@ -154,7 +154,7 @@ def test_gated_against_the_formula(P, m, k, n, act):
     assert bool(((got - y).abs() <= 2.0 ** -8 * y.abs() + 1.01 * slack).all())
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 96, 40), (60, 2048, 264), (300, 544, 136), (1300, 160, 520)])
+@pytest.mark.parametrize("m,k,n", [(1, 96, 40), (2, 6144, 1024), (13, 800, 136), (31, 1056, 640), (60, 2048, 264), (64, 512, 4096), (65, 512, 96), (300, 544, 136), (1300, 160, 520)])
 def test_bf16_rows_strides_and_in_place(P, m, k, n):
     gen = gen_of(m, k, n)
     wide = torch.randn((m, k + 40), generator=gen, device="cuda").bfloat16()
@@ -168,6 +168,11 @@ def test_bf16_rows_strides_and_in_place(P, m, k, n):
                        (x.double() / torch.exp2(byte - 127).repeat_interleave(32, -1)).float().to(torch.float8_e4m3fn).float())
     plain = P.mxfp8_linear(q, weights)
     assert torch.equal(P.mxfp8_linear(x, weights), plain)
+    # infinities and NaN are quantised alike inside the product and in front of it
+    odd = x.clone()
+    odd[0, 3], odd[m - 1, k - 1], odd[m // 2, 40] = float("inf"), float("-inf"), float("nan")
+    got, want = P.mxfp8_linear(odd, weights), P.mxfp8_linear(P.mxfp8_quant(odd), weights)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
     # residual rows and result rows inside wider buffers; what is beside them stays as it was
     stream = torch.randn((m + 1, n + 64), generator=gen, device="cuda").bfloat16()
     keep, view = stream.clone(), stream[:m, 16:n + 16]

@@ -105,6 +105,9 @@ def test_c_abi_refuses_product_arguments(inter):
                 dict(o=None, oc=4 << 20, osc=5 << 20, r=4 << 20)):
         assert linear_call(lib, **bad) == A, bad
     assert linear_call(lib, x=(6 << 20) + 8) == L_ and linear_call(lib, x=6 << 20, xs=100) == L_ and linear_call(lib, x=6 << 20, xs=88) == A
+    # bf16 rows: up to 64 need no room for their codes, and then may not be the result's
+    assert linear_call(lib, m=65, x=6 << 20, c=None) == A and linear_call(lib, x=6 << 20, o=(6 << 20) + 128, c=None, s=None) == A
+    assert linear_call(lib, x=6 << 20, c=None, s=None, status=None) == A
     assert linear_call(lib, m=0, c=None, s=None, o=None) == 0
     for rows, k, gated, want in ((64, 96, 0, 16896), (136, 160, 0, 4 * 16896), (64, 32, 1, 16896), (192, 128, 1, 2 * 16896), (64, 40, 0, 0),
                                  (60, 96, 0, 0), (96, 96, 1, 0), (1 << 20, 1 << 20, 0, 0)):
