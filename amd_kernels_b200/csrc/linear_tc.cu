@@ -2,9 +2,10 @@
 // BM token rows as N, so that one pass over the weights serves the whole block.
 //
 // What bounds it: the weight stream (HBM). One CTA = (weight tile, token block, part of K). K is split over the CTAs of a cluster until
-// there are enough of them to keep every SM loading; each adds its part in tensor memory, writes it to its shared memory, and after a cluster barrier
-// the CTAs share out the block's rows: the parts of a row are added in the order of K through distributed shared memory, then
-// bias, activation, residual and the only rounding. No workspace, no atomics, one launch, sums in a fixed order.
+// there are enough of them to keep every SM loading; each adds its part in tensor memory and writes it to its shared memory; after a
+// cluster barrier the CTAs share out the block's rows: the parts of a row are fetched and added in the order of K, then bias, activation,
+// residual and the only rounding. No workspace, no atomics, one launch, sums in a fixed order. What bounds the end of a call is distributed
+// shared memory: 48 KB into a CTA (128 rows split by 4) take 8000 cycles, fetched by 16 bytes a lane or sent by 4 alike.
 //
 //   warp 0     code producer: the weight image (one bulk copy of consecutive HBM bytes) and the token rows (TMA)
 //   warp 1     tensor memory; issues the MMAs, the whole warp around one elected lane
@@ -39,42 +40,41 @@ struct LinearCfg {
 };
 
 // (neither volatile nor ordered by a memory clobber: the loads of a row's parts have to be in flight together; what orders them is the
-// cluster barrier in front, whose address register they are made to depend on)
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+// barrier in front, behind which their address is laundered)
+template <bool CLUSTER>
+__device__ __forceinline__ float4 ld_part(uint32_t addr) {
   float4 v;
-  asm("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  if (CLUSTER) asm("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  else asm("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
-constexpr int kMaxSplits = 8;
-
 // The rows of the block that fall to this warp (every `step`-th from `first` on): the parts of a row are added in the order of K, then bias,
 // activation, residual and the only rounding. A lane has four of the tile's 128 columns; gated, lanes 0-7 and 16-23 have the gates of
-// four output columns and take the ups from the lanes 8 above. `parts`: the sums in this CTA's shared memory, kSumRow floats a row.
-template <int SUM_ROW>
-__device__ __forceinline__ void finish_rows(const LinearArgs& a, int64_t row0, int rows, int first, int step, int tile, uint32_t parts,
-                                            int splits, int lane) {
+// four output columns and take the ups from the lanes 8 above. `parts`: the sums in this CTA's shared memory, SUM_ROW floats a row. (The
+// splits are a template's: with a branch around each load the loads of a row wait for one another, 450 cycles each.)
+template <int SUM_ROW, int SPLITS>
+__device__ __forceinline__ void finish_rows(const LinearArgs& a, int64_t row0, int rows, int first, int tile, uint32_t parts, int lane) {
   const bool gated = a.act.kind == kGated;
   const int col = gated ? tile * 64 + 32 * (lane >> 4) + (lane & 7) * 4 : tile * 128 + lane * 4;
   const bool up = gated && (lane & 8);
   const bool in = col < a.n && !up;  // (n is a multiple of 8: a lane's columns are all inside or all outside)
   float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (a.bias != nullptr && col < a.n) bias = __ldcg(reinterpret_cast<const float4*>(a.bias + (up ? a.n : 0) + col));
-  uint32_t from[kMaxSplits];
+  uint32_t from[SPLITS];
 #pragma unroll
-  for (int r = 0; r < kMaxSplits; ++r) from[r] = r < splits ? (splits > 1 ? map_to_cta(parts, r) : parts) + lane * 16 : 0u;
-  for (int t = first; t < rows; t += step) {
+  for (int r = 0; r < SPLITS; ++r) from[r] = (SPLITS > 1 ? map_to_cta(parts, r) : parts) + lane * 16;
+#pragma unroll 2
+  for (int t = first; t < rows; t += 8 * SPLITS) {
     const int64_t row = row0 + t;
-    float4 part[kMaxSplits];
+    float4 part[SPLITS];
 #pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r)
-      if (r < splits) part[r] = ld_cluster_f4(from[r] + t * SUM_ROW * 4);
+    for (int r = 0; r < SPLITS; ++r) part[r] = ld_part<(SPLITS > 1)>(from[r] + t * SUM_ROW * 4);
     uint2 res = make_uint2(0u, 0u);
     if (a.residual != nullptr && in) res = __ldcg(reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col));
     float4 p = part[0];
 #pragma unroll
-    for (int r = 1; r < kMaxSplits; ++r)
-      if (r < splits) p.x += part[r].x, p.y += part[r].y, p.z += part[r].z, p.w += part[r].w;
+    for (int r = 1; r < SPLITS; ++r) p.x += part[r].x, p.y += part[r].y, p.z += part[r].z, p.w += part[r].w;
     F2 lo = F2{p.x, p.y} + F2{bias.x, bias.y}, hi = F2{p.z, p.w} + F2{bias.z, bias.w};
     if (gated) {
       const F2 ulo = {__shfl_down_sync(0xffffffffu, lo.x, 8), __shfl_down_sync(0xffffffffu, lo.y, 8)};
@@ -397,24 +397,14 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     if (__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_tfull), 0, abort_v, status))) {
       tc_fence_after();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-      if (BM == 16) {
-        uint32_t v[16];
-        tc_ld16(t_acc, v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mine[j * C::kSumRow] = __uint_as_float(v[j]);
-      } else {
-        constexpr int kAtOnce = BM >= 64 ? 2 : 1;
+      constexpr int kAtOnce = BM < 32 ? BM : 32;
 #pragma unroll 1
-        for (int c0 = 0; c0 < BM && row0 + c0 < a.m; c0 += 32 * kAtOnce) {
-          uint32_t v[kAtOnce][32];
+      for (int c0 = 0; c0 < BM && row0 + c0 < a.m; c0 += kAtOnce) {
+        uint32_t v[kAtOnce];
+        if constexpr (BM < 32) tc_ld16(t_acc + c0, v);
+        else tc_ld32(t_acc + c0, v);
 #pragma unroll
-          for (int h = 0; h < kAtOnce; ++h) tc_ld32_nowait(t_acc + c0 + 32 * h, v[h]);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int h = 0; h < kAtOnce; ++h)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) mine[(c0 + 32 * h + j) * C::kSumRow] = __uint_as_float(v[h][j]);
-        }
+        for (int j = 0; j < kAtOnce; ++j) mine[(c0 + j) * C::kSumRow] = __uint_as_float(v[j]);
       }
     }
   }
@@ -426,7 +416,13 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
   const int rows = static_cast<int>(a.m - row0 < BM ? a.m - row0 : BM);
   uint32_t parts = tiles;
   asm volatile("" : "+r"(parts)::"memory");
-  if (!abort_flag) finish_rows<C::kSumRow>(a, row0, rows, rank * 8 + warp, 8 * splits, tile, parts, splits, lane);
+  if (!abort_flag) {
+    const int first = rank * 8 + warp;
+    if (splits == 4) finish_rows<C::kSumRow, 4>(a, row0, rows, first, tile, parts, lane);
+    else if (splits == 2) finish_rows<C::kSumRow, 2>(a, row0, rows, first, tile, parts, lane);
+    else if (splits == 1) finish_rows<C::kSumRow, 1>(a, row0, rows, first, tile, parts, lane);
+    else finish_rows<C::kSumRow, 8>(a, row0, rows, first, tile, parts, lane);
+  }
   __syncwarp();
   // Nobody leaves while its parts are read. (Relaxed: what has been loaded is in registers, and a release would wait for the stores.)
   if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
