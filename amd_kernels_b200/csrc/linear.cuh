@@ -105,41 +105,74 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {  // max(|
 }
 
 constexpr float kLog2e = 1.4426950409f;
-// p * sigmoid(v), v given as -v log2(e)
-__device__ __forceinline__ F2 f2_times_sigmoid(F2 p, F2 w) { return p * f2_rcp(f2_exp2(w) + f2_dup(1.0f)); }
+// The activations take N pairs a step at a time: a pair's own chain (an exponential, a reciprocal, GELU's polynomial) is far longer than what
+// one instruction issues, and the compiler keeps the order that it is given.
+#define FOR_PAIRS _Pragma("unroll") for (int k = 0; k < N; ++k)
 
-__device__ __forceinline__ F2 act_linear(F2 p, const LinearAct& a) { return {max_nan(p.x, a.floor), max_nan(p.y, a.floor)}; }
-__device__ __forceinline__ F2 act_sigmoid(F2 p, const LinearAct& a) {
-  if (a.c3 == 0.0f) return f2_times_sigmoid(p, p * f2_dup(-kLog2e * a.c1));
-  return f2_times_sigmoid(p, p * f2_fma(p * p, f2_dup(-kLog2e * a.c3), f2_dup(-kLog2e * a.c1)));
+template <int N>
+__device__ __forceinline__ void act_linear(F2 (&p)[N], const LinearAct& a) {
+  FOR_PAIRS p[k] = {max_nan(p[k].x, a.floor), max_nan(p[k].y, a.floor)};
 }
-// p Phi(p) = max(p, 0) - |p| erfc(|p| / sqrt(2)) / 2. erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2): the Chebyshev fit of Numerical
-// Recipes (erfcc), off by at most 1.2e-7 of its value everywhere, so that the negative tail keeps its relative precision. Here s = -t (the
-// odd coefficients change sign), the exponent is to base 2 and takes the half with it.
-__device__ __forceinline__ F2 act_gelu(F2 p) {
-  const F2 m = {fminf(fabsf(p.x), 64.0f), fminf(fabsf(p.y), 64.0f)};  // (erfc is 0 there; infinity times 0 is not)
-  const F2 s = f2_rcp(f2_fma(m, f2_dup(-0.35355339f), f2_dup(-1.0f)));
-  F2 q = f2_fma(s, f2_dup(-0.17087277f * kLog2e), f2_dup(-0.82215223f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-1.48851587f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-1.13520398f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-0.27886807f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-0.18628806f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-0.09678418f * kLog2e));
-  q = f2_fma(q, s, f2_dup(0.37409196f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-1.00002368f * kLog2e));
-  q = f2_fma(q, s, f2_dup(-1.26551223f * kLog2e - 1.0f));
-  const F2 half = s * f2_exp2(f2_fma(m * m, f2_dup(-0.5f * kLog2e), q));  // -erfc / 2
-  return f2_fma(m, half, F2{max_nan(p.x, 0.0f), max_nan(p.y, 0.0f)});
+// p *= sigmoid(v), w = -v log2(e)
+template <int N>
+__device__ __forceinline__ void times_sigmoid(F2 (&p)[N], F2 (&w)[N]) {
+  FOR_PAIRS w[k] = f2_exp2(w[k]);
+  FOR_PAIRS w[k] = w[k] + f2_dup(1.0f);
+  FOR_PAIRS w[k] = f2_rcp(w[k]);
+  FOR_PAIRS p[k] = p[k] * w[k];
 }
-__device__ __forceinline__ F2 act_gated(F2 g, F2 u, const LinearAct& a) {
-  g = {min_nan(g.x, a.top), min_nan(g.y, a.top)};
-  u = {max_nan(min_nan(u.x, a.top), -a.top), max_nan(min_nan(u.y, a.top), -a.top)};
-  return f2_times_sigmoid(g, g * f2_dup(-kLog2e * a.c1)) * (u + f2_dup(a.beta));
+template <int N>
+__device__ __forceinline__ void act_sigmoid(F2 (&p)[N], const LinearAct& a) {
+  F2 w[N];
+  const F2 c1 = f2_dup(-kLog2e * a.c1);
+  if (a.c3 == 0.0f) {
+    FOR_PAIRS w[k] = p[k] * c1;
+  } else {
+    const F2 c3 = f2_dup(-kLog2e * a.c3);
+    FOR_PAIRS w[k] = p[k] * p[k];
+    FOR_PAIRS w[k] = f2_fma(w[k], c3, c1);
+    FOR_PAIRS w[k] = p[k] * w[k];
+  }
+  times_sigmoid(p, w);
 }
-template <int KIND>
-__device__ __forceinline__ F2 act_of(F2 p, const LinearAct& a) {
-  return KIND == kLinear ? act_linear(p, a) : KIND == kSigmoid ? act_sigmoid(p, a) : act_gelu(p);
+// p Phi(p) = max(p, 0) - |p| erfc(z) / 2, z = |p| / sqrt(2), and erfc(z) = exp(-z^2) t Q(t) with t = 1 / (1 + 0.425 z): Q of degree 5 is a
+// fit of this file's (least squares, weighted until the largest relative error up to z = 7 is least: 2.9e-6), so that the negative tail
+// keeps its relative precision. The coefficients carry the minus sign, the exponent (to base 2) the half. A fit of degree 9 (1.2e-7), which no
+// result of 8 or 4 bits of mantissa shows, made a product of K = 800 8 % slower: the multiply-adds bound this one.
+template <int N>
+__device__ __forceinline__ void act_gelu(F2 (&p)[N]) {
+  F2 m[N], s[N], q[N];
+  FOR_PAIRS m[k] = {fminf(fabsf(p[k].x), 64.0f), fminf(fabsf(p[k].y), 64.0f)};  // (erfc is 0 there; infinity times 0 is not)
+  FOR_PAIRS s[k] = f2_fma(m[k], f2_dup(0.300520382f), f2_dup(1.0f));
+  FOR_PAIRS s[k] = f2_rcp(s[k]);
+  FOR_PAIRS q[k] = f2_fma(s[k], f2_dup(0.1613505f), f2_dup(-0.45090797f));
+  FOR_PAIRS q[k] = f2_fma(q[k], s[k], f2_dup(0.05656477f));
+  FOR_PAIRS q[k] = f2_fma(q[k], s[k], f2_dup(-0.30168103f));
+  FOR_PAIRS q[k] = f2_fma(q[k], s[k], f2_dup(-0.22441523f));
+  FOR_PAIRS q[k] = f2_fma(q[k], s[k], f2_dup(-0.24091359f));
+  FOR_PAIRS q[k] = q[k] * s[k];
+  FOR_PAIRS s[k] = f2_fma(m[k] * m[k], f2_dup(-0.5f * kLog2e), f2_dup(-1.0f));
+  FOR_PAIRS s[k] = f2_exp2(s[k]);
+  FOR_PAIRS q[k] = q[k] * s[k];  // -erfc / 2
+  FOR_PAIRS p[k] = f2_fma(m[k], q[k], F2{max_nan(p[k].x, 0.0f), max_nan(p[k].y, 0.0f)});
 }
+// g becomes min(g, top) sigmoid(c1 min(g, top)) (clamp(u) + beta)
+template <int N>
+__device__ __forceinline__ void act_gated(F2 (&g)[N], const F2 (&u)[N], const LinearAct& a) {
+  F2 w[N];
+  const F2 c1 = f2_dup(-kLog2e * a.c1);
+  FOR_PAIRS g[k] = {min_nan(g[k].x, a.top), min_nan(g[k].y, a.top)};
+  FOR_PAIRS w[k] = g[k] * c1;
+  times_sigmoid(g, w);
+  FOR_PAIRS g[k] = g[k] * (F2{max_nan(min_nan(u[k].x, a.top), -a.top), max_nan(min_nan(u[k].y, a.top), -a.top)} + f2_dup(a.beta));
+}
+template <int KIND, int N>
+__device__ __forceinline__ void act_of(F2 (&p)[N], const LinearAct& a) {
+  if (KIND == kLinear) act_linear(p, a);
+  else if (KIND == kSigmoid) act_sigmoid(p, a);
+  else act_gelu(p);
+}
+#undef FOR_PAIRS
 
 // E8M0 byte of an MXFP8 block, the shared expert's rule (ceil_pow2(amax / 448), at least 1); an infinite block keeps a finite scale
 __device__ __forceinline__ int linear_scale(float amax) {

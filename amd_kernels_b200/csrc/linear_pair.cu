@@ -381,29 +381,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty_leader);
-      // (a loop of one piece whose registers move up: unrolled, the code of a unit does not stay in the instruction cache)
+      // A loop of one piece: unrolled, the code of a unit does not stay in the instruction cache. The piece is picked from the accumulator's
+      // registers, or they move up behind it (GELU, gated); an activation takes 16 columns at a time. Measured, 2048 x 800 -> 5984: SiLU
+      // 27.4 us in this order, 32.5 with the registers moving up and pair behind pair; GELU 30.6, 31.7 picked and 16 columns at a time.
       uint32_t scale_bytes = 0;
       bool ok = true;
 #pragma unroll 1
       for (int i = 0; i < kOuts; ++i) {
         const int col = col0 + 32 * i;
         F2 y[16];
+        const float* b_at = bias + 32 * (KIND == kGated ? 2 * i : i);
+        constexpr int kTake = KIND == kLinear ? 16 : KIND == kGelu ? 2 : 8;  // pairs of columns at a time
+        if (KIND == kGated) {
 #pragma unroll
-        for (int k4 = 0; k4 < 8; ++k4) {
-          const float4 b = *reinterpret_cast<const float4*>(bias + 32 * (KIND == kGated ? 2 * i : i) + 4 * k4);
-          const F2 p0 = F2{__uint_as_float(acc[0][4 * k4]), __uint_as_float(acc[0][4 * k4 + 1])} + F2{b.x, b.y};
-          const F2 p1 = F2{__uint_as_float(acc[0][4 * k4 + 2]), __uint_as_float(acc[0][4 * k4 + 3])} + F2{b.z, b.w};
-          if (KIND == kGated) {
+          for (int g = 0; g < 16; g += kTake) {
             constexpr int kUp = KIND == kGated ? 1 : 0;
-            const float4 bu = *reinterpret_cast<const float4*>(bias + 32 * (2 * i + 1) + 4 * k4);
-            const F2 u0 = F2{__uint_as_float(acc[kUp][4 * k4]), __uint_as_float(acc[kUp][4 * k4 + 1])} + F2{bu.x, bu.y};
-            const F2 u1 = F2{__uint_as_float(acc[kUp][4 * k4 + 2]), __uint_as_float(acc[kUp][4 * k4 + 3])} + F2{bu.z, bu.w};
-            y[2 * k4] = act_gated(p0, u0, a.act);
-            y[2 * k4 + 1] = act_gated(p1, u1, a.act);
-          } else {
-            y[2 * k4] = act_of<KIND>(p0, a.act);
-            y[2 * k4 + 1] = act_of<KIND>(p1, a.act);
+            F2 gate[kTake], up[kTake];
+#pragma unroll
+            for (int k = 0; k < kTake; k += 2) {
+              const float4 b = *reinterpret_cast<const float4*>(b_at + 2 * (g + k)), bu = *reinterpret_cast<const float4*>(b_at + 32 + 2 * (g + k));
+              const int c = 2 * (g + k);
+              gate[k] = F2{__uint_as_float(acc[0][c]), __uint_as_float(acc[0][c + 1])} + F2{b.x, b.y};
+              gate[k + 1] = F2{__uint_as_float(acc[0][c + 2]), __uint_as_float(acc[0][c + 3])} + F2{b.z, b.w};
+              up[k] = F2{__uint_as_float(acc[kUp][c]), __uint_as_float(acc[kUp][c + 1])} + F2{bu.x, bu.y};
+              up[k + 1] = F2{__uint_as_float(acc[kUp][c + 2]), __uint_as_float(acc[kUp][c + 3])} + F2{bu.z, bu.w};
+            }
+            act_gated(gate, up, a.act);
+#pragma unroll
+            for (int k = 0; k < kTake; ++k) y[g + k] = gate[k];
           }
+          if (i == 0) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[0][k] = acc[2][k], acc[1][k] = acc[3][k];
+          }
+        } else {
+          const auto pick = [&](const uint32_t (&from)[32]) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = F2{__uint_as_float(from[2 * k]), __uint_as_float(from[2 * k + 1])};
+          };
+          if (KIND == kGelu || i == 0) pick(acc[0]);
+          else if (i == 1) pick(acc[1]);
+          else if (i == 2) pick(acc[2]);
+          else pick(acc[3]);
+#pragma unroll
+          for (int g = 0; g < 16; g += kTake) {
+            F2 r[kTake];
+#pragma unroll
+            for (int k = 0; k < kTake; k += 2) {
+              const float4 b = *reinterpret_cast<const float4*>(b_at + 2 * (g + k));
+              r[k] = y[g + k] + F2{b.x, b.y};
+              r[k + 1] = y[g + k + 1] + F2{b.z, b.w};
+            }
+            act_of<KIND>(r, a.act);
+#pragma unroll
+            for (int k = 0; k < kTake; ++k) y[g + k] = r[k];
+          }
+        }
+        if (KIND == kGelu) {
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[j][k] = acc[j + 1][k];
         }
         if (residual) {
           if ((i & 1) == 0) {  // the next 64 columns
@@ -424,7 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
         if (MX) {
           float amax = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fmaxf(fabsf(y[k].x), fabsf(y[k].y)));
+          for (int k = 0; k < 16; ++k) amax = max3_abs(amax, y[k].x, y[k].y);
           const int e = linear_scale(amax);
           const F2 inv = f2_dup(e8m0_value(static_cast<uint32_t>(254 - e)));
           uint32_t w[8];
@@ -474,11 +512,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
           asked = residual && more;
           __syncwarp();  // the strip is free
         }
-        constexpr int kMove = KIND == kGated ? 2 : 1;
-#pragma unroll
-        for (int j = 0; j + kMove < kParts; ++j)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) acc[j][k] = acc[j + kMove][k];
       }
       if (!ok) break;
       __syncwarp();  // all lanes have read this unit's bias

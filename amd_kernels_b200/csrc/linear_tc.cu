@@ -75,18 +75,19 @@ __device__ __forceinline__ void finish_rows(const LinearArgs& a, int64_t row0, i
     float4 p = part[0];
 #pragma unroll
     for (int r = 1; r < SPLITS; ++r) p.x += part[r].x, p.y += part[r].y, p.z += part[r].z, p.w += part[r].w;
-    F2 lo = F2{p.x, p.y} + F2{bias.x, bias.y}, hi = F2{p.z, p.w} + F2{bias.z, bias.w};
+    F2 y[2] = {F2{p.x, p.y} + F2{bias.x, bias.y}, F2{p.z, p.w} + F2{bias.z, bias.w}};
     if (gated) {
-      const F2 ulo = {__shfl_down_sync(0xffffffffu, lo.x, 8), __shfl_down_sync(0xffffffffu, lo.y, 8)};
-      const F2 uhi = {__shfl_down_sync(0xffffffffu, hi.x, 8), __shfl_down_sync(0xffffffffu, hi.y, 8)};
-      lo = act_gated(lo, ulo, a.act), hi = act_gated(hi, uhi, a.act);
+      const F2 u[2] = {{__shfl_down_sync(0xffffffffu, y[0].x, 8), __shfl_down_sync(0xffffffffu, y[0].y, 8)},
+                       {__shfl_down_sync(0xffffffffu, y[1].x, 8), __shfl_down_sync(0xffffffffu, y[1].y, 8)}};
+      act_gated(y, u, a.act);
     } else if (a.act.kind == kLinear) {
-      lo = act_of<kLinear>(lo, a.act), hi = act_of<kLinear>(hi, a.act);
+      act_of<kLinear>(y, a.act);
     } else if (a.act.kind == kSigmoid) {
-      lo = act_of<kSigmoid>(lo, a.act), hi = act_of<kSigmoid>(hi, a.act);
+      act_of<kSigmoid>(y, a.act);
     } else {
-      lo = act_of<kGelu>(lo, a.act), hi = act_of<kGelu>(hi, a.act);
+      act_of<kGelu>(y, a.act);
     }
+    F2 lo = y[0], hi = y[1];
     if (a.residual != nullptr) {
       lo = lo + F2{__uint_as_float(res.x << 16), __uint_as_float(res.x & 0xffff0000u)};
       hi = hi + F2{__uint_as_float(res.y << 16), __uint_as_float(res.y & 0xffff0000u)};

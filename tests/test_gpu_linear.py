@@ -189,6 +189,24 @@ def test_bf16_rows_strides_and_in_place(P, m, k, n):
     assert torch.equal(P.mxfp8_linear(one, weights), P.mxfp8_linear(one.contiguous(), weights))
 
 
+@pytest.mark.parametrize("m,k", [(1, 32), (9, 96), (300, 160), (33, 6144), (5, 8224), (3, 32800), (2, 70016)])
+def test_quantised_rows_of_any_width(P, m, k):
+    """Exact in 64 bits: the scale's power of two and the code's rounding; rows inside wider rows; scales that begin at any byte."""
+    gen = gen_of("quant", m, k)
+    x = torch.randn((m, k + 8), generator=gen, device="cuda") * torch.exp(2 * torch.randn((m, k + 8), generator=gen, device="cuda"))
+    x = x.bfloat16()[:, :k]
+    x[0, :32] = 0
+    byte = mxfp8_of(x.double(), 1)
+    byte[0, 0] = 1
+    want = (x.double() / torch.exp2(byte - 127).repeat_interleave(32, -1)).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    room = torch.full((m * (k // 32) + 9,), 93, dtype=torch.uint8, device="cuda")
+    scales = room[1:m * (k // 32) + 1].view(m, k // 32)
+    codes, s = P.mxfp8_quant(x)
+    assert torch.equal(s.double(), byte) and torch.equal(codes & 127, want & 127) and torch.equal(codes, want)
+    P.mxfp8_quant(x, out=(codes.zero_(), scales))
+    assert torch.equal(scales, s) and torch.equal(codes, want) and int(room[0]) == 93 and bool((room[m * (k // 32) + 1:] == 93).all())
+
+
 @pytest.mark.parametrize("m,k", [(40, 800), (700, 6144), (130, 160)])
 def test_rows_of_a_larger_batch_and_unaligned_scales(P, m, k):
     """A slice of the rows: its scales begin at any byte. Same bits as the rows copied out."""
