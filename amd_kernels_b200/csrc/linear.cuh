@@ -200,6 +200,13 @@ struct RowScales {
     const uintptr_t at = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(per_row);
     alignment = (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
   }
+  // asks L2 for the line in which those bytes begin (before the launch in front has ended: L2 is where its stores go)
+  template <int ROWS>
+  __device__ __forceinline__ void prefetch(int64_t row, int kt) const {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      if (row + 32 * i < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (row + 32 * i) * per_row + kt * 4));
+  }
   template <int ROWS>
   __device__ __forceinline__ void load(int64_t row, int kt, uint32_t (&w)[ROWS][5]) const {
     const uint8_t* p = base + row * per_row + kt * 4;
@@ -269,6 +276,11 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
 // took 5000 cycles to come.
 __device__ __forceinline__ void scales_first_wait() { asm volatile("bar.sync 3, 64;" ::: "memory"); }
 __device__ __forceinline__ void scales_first_arrive() { asm volatile("bar.arrive 3, 64;" ::: "memory"); }
+
+// the same for a tile of codes, through its tensor map
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
+}
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -144,14 +144,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
   const LinearUnits units = {static_cast<int>((args.m + 255) / 256), (args.tiles_n + 1) / 2};
   const int total = units.total(), tiles_k = args.tiles_k;
   int pair, step;
-  // the first weights that this CTA will load, into L2 while the launch in front still runs
-  if (warp == 0 && lane == 0 && cluster < total) {
+  // what this CTA will load first, into L2 while the launch in front still runs
+  if (cluster < total && (warp == 0 || warp == 3)) {
     units.at(cluster, pair, step);
-    const int tile = 2 * step + static_cast<int>(rank), n = tiles_k < 8 ? tiles_k : 8;
-    if (tile < args.tiles_n) {
+    const int row = pair * 256 + static_cast<int>(rank) * 128, tile = 2 * step + static_cast<int>(rank), n = tiles_k < 8 ? tiles_k : 8;
+    if (warp == 3) {
+      RowScales(args.scales, args.m, args.k).prefetch<4>(row + lane, 0);
+    } else if (lane == 0) {
       const int64_t at = static_cast<int64_t>(tile) * tiles_k;
-      for (int kt = 0; kt < n; ++kt) l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
-      l2_prefetch_bulk(args.atoms + at * kAtomBytes, static_cast<uint32_t>(n) * kAtomBytes);
+      if (tile < args.tiles_n) l2_prefetch_bulk(args.atoms + at * kAtomBytes, static_cast<uint32_t>(n) * kAtomBytes);
+      for (int kt = 0; kt < n; ++kt) {
+        if (tile < args.tiles_n) l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
+        if (row < args.m) tma_prefetch_2d(&map_x, kt * 128, row);
+      }
     }
   }
   tc_fence_before();
@@ -524,7 +529,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // neither CTA frees tensor memory or leaves while the partner may still signal or read it
+  // Neither CTA frees tensor memory or leaves while the partner may still signal or read it. (Relaxed: a release would wait for the stores.)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),

@@ -164,8 +164,12 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     const int64_t at = static_cast<int64_t>(tile) * args.tiles_k + kt0;
     const int n = kt1 - kt0 < C::kStages ? kt1 - kt0 : C::kStages;
     l2_prefetch_bulk(args.atoms + at * kAtomBytes, static_cast<uint32_t>(n) * kAtomBytes);
-    for (int kt = 0; kt < n; ++kt) l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
+    for (int kt = 0; kt < n; ++kt) {
+      l2_prefetch_bulk(args.tiles + (at + kt) * kLinearImageBytes, kLinearImageBytes);
+      if (!QUANT) tma_prefetch_2d(&map_x, (kt0 + kt) * 128, static_cast<int>(row0));
+    }
   }
+  if (!QUANT && warp == 3) RowScales(args.scales, args.m, args.k).prefetch<(BM + 31) / 32>(row0 + lane, kt0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
