@@ -277,7 +277,11 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
 __device__ __forceinline__ void scales_first_wait() { asm volatile("bar.sync 3, 64;" ::: "memory"); }
 __device__ __forceinline__ void scales_first_arrive() { asm volatile("bar.arrive 3, 64;" ::: "memory"); }
 
-// the same for a tile of codes, through its tensor map
+// a tensor map into the cache that the copies read it from
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+// a tile of codes into L2, through its tensor map
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }

@@ -2,7 +2,7 @@
 // N = 256 weight rows (two tiles) x K = 32 per instruction, each CTA staging its own 128 token rows and half of the
 // weight rows. No multicast.
 //
-// Unit = (pair of token blocks) x (pair of weight tiles). Two rings: 5 stages of codes, and 3 slots of the scales of four K-tiles that travel
+// Unit = (pair of token blocks) x (pair of weight tiles). Two rings: 5 stages of codes, and 2 slots of the scales of four K-tiles that travel
 // ahead of them, so that the MMA warp waits for codes and, once in four K-tiles, for scales. The token scales come row-major, as every producer of this package writes them: the scale
 // warp turns them into atoms on the way, so no launch in front of the product re-lays them.
 //
@@ -12,7 +12,7 @@
 //   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
 //   warps 4-11  epilogue (both CTAs): thread = one token row, 128 columns. The sums are pulled into registers and the accumulator
 //               is handed back; then bias, activation, residual and one rounding, 32 columns at a time. bf16 rows go through a strip of
-//               shared memory per warp, 32 rows x 64 columns: the residual arrives there by TMA, the result leaves there by TMA. (A
+//               shared memory per warp, pieces of 32 rows x 32 columns: the residual arrives by TMA, two pieces ahead, the result leaves by TMA. (A
 //               thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the operands of
 //               the MMAs wait: with them a residual made 16384 x 6144 -> 6144 28 % slower.)
 // 12 warps start with 168 registers; the issuing warpgroup drops to 88, the epilogue's rise to 208 (4 x 88 + 8 x 208 = 12 x 168: the
@@ -24,10 +24,11 @@ namespace b200moe {
 
 struct LinearPairCfg {
   static constexpr int kStages = 5;                // code ring (6 stages and no strips were 0 to 1 % faster, 4 were 5 % slower)
-  static constexpr int kSfSlots = 3;               // groups of scales in shared memory
+  static constexpr int kSfSlots = 2;               // groups of scales in shared memory
   static constexpr int kWOff = 128 * 128;          // the CTA's weight tile, behind its 128 token rows
   static constexpr int kStageBytes = 2 * 128 * 128;
-  static constexpr int kStripBytes = 32 * 128;     // one epilogue warp's rows x 64 bf16 columns, 128-byte swizzle
+  static constexpr int kPieceBytes = 32 * 64;      // an epilogue warp's 32 rows x 32 bf16 columns, 64-byte swizzle
+  static constexpr int kStripBytes = 3 * kPieceBytes;  // a warp's: two pieces of residual, one of results
   static constexpr int kStripOff = kStages * kStageBytes;
   static constexpr int kSfOff = kStripOff + 8 * kStripBytes;
   static constexpr int kSfSlotBytes = kSfGroup * 3 * kAtomBytes;  // four token atoms, four atoms of each weight tile
@@ -84,6 +85,7 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
                "r"(src), "r"(x), "r"(y)
                : "memory");
 }
+// until the thread's stores have read their shared memory
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 template <int KIND, bool MX>
@@ -101,7 +103,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
   __shared__ __align__(8) uint64_t bar_set[kSfSets];         // leader: the MMAs that read the set have completed
   __shared__ __align__(8) uint64_t bar_tfull;                // in each CTA: the unit's accumulator is complete
   __shared__ __align__(8) uint64_t bar_tempty;               // leader: both CTAs' epilogues have read it
-  __shared__ __align__(8) uint64_t bar_res[8];               // an epilogue warp's residual has landed in its strip
+  __shared__ __align__(8) uint64_t bar_res[8][2];            // the residual of a piece has landed in half 0 or 1 of the warp's strip
   __shared__ __align__(8) uint64_t bar_drain[2];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
@@ -128,7 +130,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
     }
     mbar_init(smem_u32(&bar_tfull), 1);
     mbar_init(smem_u32(&bar_tempty), 16);  // one arrival per epilogue warp of both CTAs
-    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&bar_res[i]), 1);
+    for (int i = 0; i < 16; ++i) mbar_init(smem_u32(&bar_res[i >> 1][i & 1]), 1);
     mbar_init(smem_u32(&bar_drain[0]), 1);
     mbar_init(smem_u32(&bar_drain[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -145,6 +147,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
   const int total = units.total(), tiles_k = args.tiles_k;
   int pair, step;
   // what this CTA will load first, into L2 while the launch in front still runs
+  if (threadIdx.x == 32) {
+    prefetch_map(&map_x);
+    prefetch_map(&map_wc);
+    prefetch_map(&map_ws);
+    if (args.residual != nullptr) prefetch_map(&map_res);
+    if (!MX) prefetch_map(&map_out);
+  }
   if (cluster < total && (warp == 0 || warp == 3)) {
     units.at(cluster, pair, step);
     const int row = pair * 256 + static_cast<int>(rank) * 128, tile = 2 * step + static_cast<int>(rank), n = tiles_k < 8 ? tiles_k : 8;
@@ -164,17 +173,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
   cluster_sync_all();  // both CTAs' barriers exist before anything signals across the pair
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
-  pdl_wait();
+  // Every role waits for the launch in front itself, after what it can do before (its code comes into the instruction cache meanwhile).
   LinearArgs a = args;
-  launder(a.scales);
-  launder(a.bias);
-  launder(a.residual);
 
   // The issuing warpgroup and the two epilogue warpgroups do not meet again before the kernel's last lines.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
       // ---------------------------------------------------------------- code producer (both CTAs)
+      pdl_wait();
       if (cluster < total) scales_first_wait();
       if (lane == 0) {
         const uint32_t full0 = map_to_cta(smem_u32(&bar_full[0]), 0);  // the leader's barriers, as seen from this CTA
@@ -200,7 +207,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
       // ---------------------------------------------------------------- scales (both CTAs): lane l writes 16 bytes of a token atom, rows l,
       // l + 32, l + 64 and l + 96. A group's bytes are asked for two groups ahead.
       const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
-      const RowScales scales(a.scales, a.m, a.k);
+      RowScales scales(a.scales, a.m, a.k);
       uint32_t even[4][5] = {}, odd[4][5] = {};
       int fu = cluster, fkt = 0;  // the group that is asked for next
       const auto fetch = [&](uint32_t (&v)[4][5]) {
@@ -225,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
           tma_load_2d_pair(tiles + at + kSfGroup * kAtomBytes, &map_ws, 0, atom, sfull);
           tma_load_2d_pair(tiles + at + 2 * kSfGroup * kAtomBytes, &map_ws, 0, atom + tiles_k * 4, sfull);
         }
-        if (it++ == 0) scales_first_arrive();
+        ++it;
         scales.tiles(static_cast<int64_t>(pair) * 256 + rank * 128 + lane, kt, v);
         uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at) + lane;
 #pragma unroll
@@ -237,7 +244,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
         if ((kt += kSfGroup) >= tiles_k) kt = 0, u += n_clusters;
         if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
       };
+      pdl_wait();
+      launder(scales.base);
       fetch(even);
+      if (cluster < total) scales_first_arrive();
       fetch(odd);
       while (u < total && ok) {
         group(even);
@@ -251,6 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
         constexpr uint32_t kIdesc = (static_cast<uint32_t>(256 >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24);
         uint32_t ui = 0, s = 0, ph = 0, slot = 0, sph = 0, set = 0;
         bool ok = true, ready = false;
+        pdl_wait();
         for (int u = cluster; u < total && ok; u += n_clusters, ++ui) {
           if (!warp_wait(smem_u32(&bar_tempty), (ui & 1u) ^ 1u, abort_v, status)) break;
           tc_fence_after();
@@ -288,6 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
       if (leader) {
         uint32_t slot = 0, ph = 0, set = 0, set_ph = 1u;
         bool ok = true;
+        pdl_wait();
         for (int u = cluster; u < total && ok; u += n_clusters) {
           for (int kt = 0; kt < tiles_k; kt += kSfGroup) {
             if (!__all_sync(0xffffffffu, mbar_wait_acquire_cluster(smem_u32(&bar_sfull[slot]), ph, abort_v, status) &&
@@ -319,6 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
         const uint32_t sfull0 = map_to_cta(smem_u32(&bar_sfull[0]), 0);
         uint32_t slot = 0, ph = 0;
         bool ok = true;
+        pdl_wait();
         for (int u = cluster; u < total && ok; u += n_clusters) {
           for (int kt = 0; kt < tiles_k; kt += kSfGroup) {
             if (!mbar_wait(smem_u32(&bar_relay[slot]), ph, abort_v, status)) { ok = false; break; }
@@ -339,9 +352,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
     float* const bias = reinterpret_cast<float*>(tiles_ptr + C::kBiasOff) + (warp - 4) * 128;
     const bool wide = (reinterpret_cast<uintptr_t>(a.out_codes) & 31) == 0;
     const bool scale_words = (a.n & 127) == 0 && (reinterpret_cast<uintptr_t>(a.out_scales) & 3) == 0;
+    // the residual of piece i of a unit is in part i & 1 of the strip, the result in part 2
     const uint32_t strip = tiles + C::kStripOff + (warp - 4) * C::kStripBytes;
-    uint8_t* const strip_row = tiles_ptr + C::kStripOff + (warp - 4) * C::kStripBytes + lane * 128;
-    const uint32_t res_bar = smem_u32(&bar_res[warp - 4]);
+    uint8_t* const strip_row = tiles_ptr + C::kStripOff + (warp - 4) * C::kStripBytes + lane * 64;
+    const uint32_t turn = (lane >> 1) & 3;                                     // the swizzle of a row's four 16-byte chunks
+    const uint32_t res_bar = smem_u32(&bar_res[warp - 4][0]);
     const bool residual = a.residual != nullptr;
     // first token row and first output column of this warp's part of a unit
     const auto place = [&](int v, int64_t& row, int& col) {
@@ -349,19 +364,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
       row = static_cast<int64_t>(pair) * 256 + rank * 128 + q * 32;
       col = (2 * step + half) * (KIND == kGated ? 64 : 128);
     };
-    // The residual of 64 columns (rows and columns beyond the matrix arrive as zeros); lane 0, once the strip is free.
-    const auto ask_residual = [&](int64_t row, int col) {
-      mbar_arrive_expect_tx(res_bar, C::kStripBytes);
-      tma_load_2d(strip, &map_res, col, static_cast<int>(row), res_bar);
+    // The residual of a piece (rows and columns beyond the matrix arrive as zeros); lane 0, once that part has been read.
+    const auto ask_residual = [&](int64_t row, int col, int part) {
+      mbar_arrive_expect_tx(res_bar + 8u * part, C::kPieceBytes);
+      tma_load_2d(strip + part * C::kPieceBytes, &map_res, col, static_cast<int>(row), res_bar + 8u * part);
     };
-    uint32_t ui = 0, res_ph = 0;
+    uint32_t ui = 0, res_ph = 0;  // res_ph: the phases of both parts (bit 0, bit 1)
     int64_t row0;
     int col0;
-    bool asked = false;
+    int asked = 0;                // pieces asked for and not yet waited for
+    pdl_wait();
+    launder(a.bias);
     if (residual && cluster < total) {
       place(cluster, row0, col0);
-      if (lane == 0) ask_residual(row0, col0);
-      asked = true;
+      if (lane == 0) {
+        ask_residual(row0, col0, 0);
+        ask_residual(row0, col0 + 32, 1);
+      }
+      asked = 2;
     }
     for (int u = cluster; u < total; u += n_clusters, ++ui) {
       place(u, row0, col0);
@@ -449,20 +469,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
             for (int k = 0; k < 32; ++k) acc[j][k] = acc[j + 1][k];
         }
         if (residual) {
-          if ((i & 1) == 0) {  // the next 64 columns
-            ok = __all_sync(0xffffffffu, mbar_wait(res_bar, res_ph, abort_v, status));
-            if (!ok) break;
-            res_ph ^= 1u;
-            asked = false;
-          }
+          ok = __all_sync(0xffffffffu, mbar_wait(res_bar + 8u * (i & 1), (res_ph >> (i & 1)) & 1u, abort_v, status));
+          if (!ok) break;
+          res_ph ^= 1u << (i & 1);
+          --asked;
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            const uint4 r = *reinterpret_cast<const uint4*>(strip_row + (((4 * (i & 1) + p) ^ (lane & 7)) << 4));
+            const uint4 r = *reinterpret_cast<const uint4*>(strip_row + (i & 1) * C::kPieceBytes + ((p ^ turn) << 4));
             const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               y[4 * p + k] = y[4 * p + k] + F2{__uint_as_float(rr[k] << 16), __uint_as_float(rr[k] & 0xffff0000u)};
           }
+          // piece i + 2 goes where piece i was
+          const bool here = i + 2 < kOuts;
+          if (here || u + n_clusters < total) {
+            int64_t next_row = row0;
+            int next_col = col + 64;
+            if (!here) {
+              place(u + n_clusters, next_row, next_col);
+              next_col += 32 * (i + 2 - kOuts);
+            }
+            __syncwarp();
+            if (lane == 0) ask_residual(next_row, next_col, i & 1);
+            ++asked;
+          }
+        }
+        if (!MX) {  // the piece before has left
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
         }
         if (MX) {
           float amax = 0.0f;
@@ -495,35 +530,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
         } else {
 #pragma unroll
           for (int p = 0; p < 4; ++p)
-            *reinterpret_cast<uint4*>(strip_row + (((4 * (i & 1) + p) ^ (lane & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(strip_row + 2 * C::kPieceBytes + ((p ^ turn) << 4)) =
                 make_uint4(pack_bf16x2(y[4 * p].x, y[4 * p].y), pack_bf16x2(y[4 * p + 1].x, y[4 * p + 1].y),
                            pack_bf16x2(y[4 * p + 2].x, y[4 * p + 2].y), pack_bf16x2(y[4 * p + 3].x, y[4 * p + 3].y));
         }
-        if (i & 1) {  // 64 columns are done
-          if (!MX) fence_proxy_async();
+        if (!MX) {
+          fence_proxy_async();
           __syncwarp();
-          const bool more = i + 1 < kOuts || u + n_clusters < total;
-          int64_t next_row = row0;
-          int next_col = col + 32;
-          if (residual && i + 1 >= kOuts && more) place(u + n_clusters, next_row, next_col);
-          if (lane == 0) {
-            if (!MX) {
-              // (what lies beyond the matrix is not written)
-              if (row0 < a.m && col - 32 < a.n) tma_store_2d(&map_out, col - 32, static_cast<int>(row0), strip);
-              tma_store_wait_read();
-            }
-            if (residual && more) ask_residual(next_row, next_col);
-          }
-          asked = residual && more;
-          __syncwarp();  // the strip is free
+          // (what lies beyond the matrix is not written)
+          if (lane == 0 && row0 < a.m && col < a.n) tma_store_2d(&map_out, col, static_cast<int>(row0), strip + 2 * C::kPieceBytes);
         }
       }
       if (!ok) break;
       __syncwarp();  // all lanes have read this unit's bias
     }
-    if (asked && lane == 0) {  // after an abort: the copy lands before the CTA gives up its shared memory
-      const uint64_t t0 = global_timer(), limit = wait_limit_ns();
-      while (!mbar_try_wait(res_bar, res_ph) && global_timer() - t0 < limit) {}
+    if (lane == 0) {
+      if (!MX) tma_store_wait_read();
+      if (asked > 0) {  // after an abort: the copies land before the CTA gives up its shared memory
+        const uint64_t t0 = global_timer(), limit = wait_limit_ns();
+        for (int h = 0; h < 2; ++h)
+          while (!mbar_try_wait(res_bar + 8u * h, (res_ph >> h) & 1u) && global_timer() - t0 < limit) {}
+      }
     }
   }
 
@@ -540,15 +567,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// bf16 rows [m][n], `stride` elements apart, boxes of 64 columns x 32 rows, 128-byte swizzle; columns and rows beyond are zeros / unwritten
+// bf16 rows [m][n], `stride` elements apart, boxes of 32 columns x 32 rows, 64-byte swizzle; columns and rows beyond are zeros / unwritten
 static int make_rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t m, int64_t stride) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return B200MOE_E_DRIVER;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(m)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(m > 1 ? stride : n) * 2};
-  const cuuint32_t box[2] = {64, 32}, estr[2] = {1, 1};
+  const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : B200MOE_E_DRIVER;
 }

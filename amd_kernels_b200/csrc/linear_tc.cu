@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       if (!QUANT) tma_prefetch_2d(&map_x, (kt0 + kt) * 128, static_cast<int>(row0));
     }
   }
+  if (!QUANT && threadIdx.x == 32) prefetch_map(&map_x);
   if (!QUANT && warp == 3) RowScales(args.scales, args.m, args.k).prefetch<(BM + 31) / 32>(row0 + lane, kt0);
   tc_fence_before();
   __syncthreads();
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
         mbar_arrive_expect_tx(sfull, bytes);
         bulk_load(tiles + at, a.atoms + (static_cast<int64_t>(tile) * a.tiles_k + kt) * kAtomBytes, bytes, sfull);
       }
-      if (it++ == 0) scales_first_arrive();
+      ++it;
       scales.tiles(row, kt, v);
       uint4* cells = reinterpret_cast<uint4*>(tiles_ptr + at + kSfGroup * kAtomBytes) + lane;
 #pragma unroll
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
       if (++slot == C::kSfSlots) { slot = 0; ph ^= 1u; }
     };
     fetch(kt0, even);
+    scales_first_arrive();
     fetch(kt0 + kSfGroup, odd);
     for (int kt = kt0; kt < kt1 && ok; kt += 2 * kSfGroup) {
       group(kt, even);
