@@ -108,11 +108,6 @@ static int launch_norm(const NormArgs& a, int threads, int rows_per_cta, cudaStr
   return 0;
 }
 
-// rows [n][width] elements of `size` bytes, `stride` elements apart: the bytes they span
-static size_t span_bytes(int64_t n, int64_t width, int64_t stride, int size) {
-  return (static_cast<size_t>(n - 1) * stride + width) * size;
-}
-
 }  // namespace b200moe
 
 extern "C" int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* stream) {
@@ -145,11 +140,12 @@ extern "C" int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* st
     if (!all[i].p || !all[i].out) continue;
     for (int j = 0; j < kAll; ++j) {
       if (!all[j].p || j == i || (all[j].out && j < i)) continue;
-      const uintptr_t pi = reinterpret_cast<uintptr_t>(all[i].p), pj = reinterpret_cast<uintptr_t>(all[j].p);
-      const size_t bi = span_bytes(rows, all[i].width, all[i].stride, all[i].size);
-      const size_t bj = j == 6 ? 2 * h : span_bytes(rows, all[j].width, all[j].stride, all[j].size);
-      const bool same = j < 2 && pi == pj && all[i].size == 2 && (rows <= 1 || all[i].stride == all[j].stride);
-      if (!same && pi < pj + bj && pj < pi + bi) return B200MOE_E_ARG;
+      const bool same = j < 2 && all[i].p == all[j].p && all[i].size == 2 && (rows <= 1 || all[i].stride == all[j].stride);
+      const auto span = [&](int k) {
+        const Rows& r = all[k];
+        return RowSpan{r.p, k == 6 ? 1 : rows, r.width * r.size, rows > 1 ? r.stride * r.size : r.width * r.size};
+      };
+      if (!same && rows_overlap(span(i), span(j))) return B200MOE_E_ARG;
     }
   }
   NormArgs a;

@@ -117,11 +117,6 @@ static bool linear_dims(int64_t rows, int64_t k, int gated) {
   return linear_row_tiles(rows) * linear_k_tiles(k) <= INT32_MAX / 128;
 }
 
-static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-  return a && b && pa < pb + nb && pb < pa + na;
-}
-
 int set_wait_limit_linear(unsigned long long ns) {
   const int r = set_wait_limit_linear_tc(ns);
   return r ? r : set_wait_limit_linear_pair(ns);
@@ -187,6 +182,8 @@ extern "C" int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t
   if (!x_bf16 || !codes8 || !scales8) return B200MOE_E_ARG;
   if (rows > 1 && x_stride < k && x_stride != 0) return B200MOE_E_ARG;
   if (misaligned(x_bf16, 16) || misaligned(codes8, 8) || (rows > 1 && (x_stride & 7))) return B200MOE_E_ALIGN;
+  const RowSpan x = {x_bf16, rows, 2 * k, rows > 1 ? 2 * x_stride : 2 * k}, codes = {codes8, rows, k, k}, scales = {scales8, rows, k / 32, k / 32};
+  if (rows_overlap(x, codes) || rows_overlap(x, scales) || rows_overlap(codes, scales)) return B200MOE_E_ARG;
   const int v = static_cast<int>(k / 8);
   return (v <= 1024 ? launch_quant<3> : launch_quant<8>)(static_cast<const uint4*>(x_bf16), x_stride / 8, rows, v,
                                                          reinterpret_cast<uint2*>(codes8), scales8, static_cast<cudaStream_t>(stream));
@@ -216,18 +213,19 @@ static int linear_args(LinearArgs& a, const b200moe_linear_call* call, const int
       bad_rows(c.out, c.out_stride) || bad_rows(c.residual, c.residual_stride))
     return B200MOE_E_ALIGN;
   // the rows of out may be those of the residual (a thread stores where it has loaded); any other overlap with an input is refused
-  const void* outs[3] = {c.out, c.out_codes8, c.out_scales8};
-  const size_t rows = static_cast<size_t>(m);
-  const size_t out_bytes[3] = {((rows - 1) * c.out_stride + n) * 2, rows * n, rows * (n / 32)};
-  const size_t res_bytes = ((rows - 1) * c.residual_stride + n) * 2, x_bytes = ((rows - 1) * c.x_stride + w->k) * 2;
-  for (int i = 0; i < 3; ++i) {
-    if (inside && overlap(outs[i], out_bytes[i], c.x, x_bytes)) return B200MOE_E_ARG;
-    if (!inside && (overlap(outs[i], out_bytes[i], c.codes8, rows * w->k) || overlap(outs[i], out_bytes[i], c.scales8, rows * (w->k / 32))))
-      return B200MOE_E_ARG;
-    const bool same = i == 0 && c.out == c.residual && (m == 1 || c.out_stride == c.residual_stride);
-    if (!same && overlap(outs[i], out_bytes[i], c.residual, res_bytes)) return B200MOE_E_ARG;
+  const int64_t k = w->k, weight_bytes = linear_row_tiles(w->rows) * linear_k_tiles(k) * kLinearTileBytes;
+  const auto bf16_rows = [m](const void* p, int64_t width, int64_t stride) { return RowSpan{p, m, 2 * width, m > 1 ? 2 * stride : 2 * width}; };
+  const RowSpan outs[] = {bf16_rows(c.out, n, c.out_stride), {c.out_codes8, m, n, n}, {c.out_scales8, m, n / 32, n / 32}};
+  const RowSpan residual = bf16_rows(c.residual, n, c.residual_stride);
+  const RowSpan ins[] = {bf16_rows(c.x, k, c.x_stride), {inside ? nullptr : c.codes8, m, k, k}, {inside ? nullptr : c.scales8, m, k / 32, k / 32},
+                         {w->tiles, 1, weight_bytes, weight_bytes}, {w->bias, 1, 4 * w->rows, 4 * w->rows}};
+  const bool in_place = c.out && c.out == c.residual && (m == 1 || c.out_stride == c.residual_stride);
+  for (const RowSpan& o : outs) {
+    for (const RowSpan& i : ins)
+      if (rows_overlap(o, i)) return B200MOE_E_ARG;
+    if (!in_place && rows_overlap(o, residual)) return B200MOE_E_ARG;
   }
-  if (overlap(c.out_codes8, out_bytes[1], c.out_scales8, out_bytes[2])) return B200MOE_E_ARG;
+  if (rows_overlap(outs[1], outs[2])) return B200MOE_E_ARG;
   a.tiles = w->tiles;
   a.bias = w->bias;
   a.x = inside ? static_cast<const __nv_bfloat16*>(c.x) : nullptr;

@@ -37,6 +37,9 @@ struct LinearCfg {
   static constexpr int kTmemCols = kColsUsed <= 128 ? 128 : 256;
   static_assert(BM * kSumRow * 4 <= kSfOff, "the parts fit the ring");
   static_assert(kSmemBytes <= 227 * 1024 / kCtasPerSm - 1024 && kTmemCols * kCtasPerSm <= 512, "shared and tensor memory");
+  // A CTA of the next launch may be there early. It must not hold tensor memory that one of this launch has yet to get: no third one of these
+  // fits an SM (nor any of the layer's kernels, which take more shared memory) until one of the two has left.
+  static_assert(3 * kSmemBytes > 227 * 1024, "three CTAs on an SM");
 };
 
 // (neither volatile nor ordered by a memory clobber: the loads of a row's parts have to be in flight together; what orders them is the

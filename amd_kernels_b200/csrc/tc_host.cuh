@@ -77,4 +77,20 @@ struct PerDeviceOnce {
 
 static inline bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+// n rows of `width` bytes, `stride` bytes apart (null: none)
+struct RowSpan {
+  const void* p;
+  int64_t n, width, stride;
+};
+// Do they share a byte? Rows of one stride may lie between one another (column ranges of one tensor).
+static inline bool rows_overlap(const RowSpan& a, const RowSpan& b) {
+  if (!a.p || !b.p || a.n == 0 || b.n == 0) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  const uintptr_t ea = pa + (a.n - 1) * a.stride + a.width, eb = pb + (b.n - 1) * b.stride + b.width;
+  if (pa >= eb || pb >= ea) return false;
+  if (a.n == 1 || b.n == 1 || a.stride != b.stride || a.stride == 0) return true;
+  const int64_t s = a.stride, d = pb >= pa ? static_cast<int64_t>(pb - pa) % s : (s - static_cast<int64_t>(pa - pb) % s) % s;
+  return d < a.width || d + b.width > s;
+}
+
 }  // namespace b200moe

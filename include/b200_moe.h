@@ -418,7 +418,7 @@ int b200moe_forward_x(const b200moe_weights* w, const void* x_bf16, int64_t toke
  * x, residual, residual_out and normed are bf16 rows with a stride of their own in elements (a multiple of 8, at least h; a residual
  * stride of 0 is one row for all), weight bf16 [h]; 16-byte aligned, codes8 8-byte. h: a multiple of 32, up to
  * B200MOE_NORM_MAX_H. residual_out or normed may be x or residual (the same address and stride); any other overlap of an output is
- * B200MOE_E_ARG. The bits of a row do not depend on the other rows. rows may be 0. */
+ * B200MOE_E_ARG (column ranges of one tensor do not overlap). The bits of a row do not depend on the other rows. rows may be 0. */
 #define B200MOE_NORM_MAX_H 32768
 typedef struct b200moe_norm_call {
   const void* x;
@@ -463,7 +463,7 @@ size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated);
 int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated, uint8_t* tiles,
                               void* stream);
 
-/* bf16 rows (x_stride elements apart, a multiple of 8, or 0) -> codes8 [rows][k], scales8 [rows][k/32], the rule above. */
+/* bf16 rows (x_stride elements apart, a multiple of 8, or 0) -> codes8 [rows][k], scales8 [rows][k/32], the rule above; they may not overlap. */
 int b200moe_quant_mxfp8(const void* x_bf16, int64_t x_stride, int64_t rows, int64_t k, uint8_t* codes8, uint8_t* scales8,
                         void* stream);
 
@@ -478,8 +478,8 @@ typedef struct b200moe_linear_weights {
  * B200MOE_LINEAR_ROWS_INSIDE rows inside the product (codes8 and scales8 are not used), more of them into codes8 and scales8 by a launch
  * in front (b200moe_quant_mxfp8). residual, out and x are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a stride of 0
  * of x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
- * residual (same address and stride); any other overlap of an output with what the product reads is B200MOE_E_ARG (bf16
- * rows that a launch in front quantises may be overwritten). m may be 0. */
+ * residual (same address and stride); any other overlap of an output with what the call reads is B200MOE_E_ARG (column ranges of one
+ * tensor do not overlap). m may be 0. */
 typedef struct b200moe_linear_call {
   b200moe_linear_weights w;
   const void* x; /* or null */

@@ -109,6 +109,24 @@ def test_in_place_and_shared_residual(P):
     assert torch.equal(P.add_rmsnorm_mxfp8(x, one, weight).codes, P.add_rmsnorm_mxfp8(x, one.contiguous(), weight).codes)
 
 
+def test_columns_of_one_tensor(P):
+    """Input and results side by side in one tensor; a result that reaches into an input is refused."""
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    m, h = 37, 1056
+    weight = (0.1 * torch.randn(h, generator=gen, device="cuda")).bfloat16()
+    buf = rows(gen, m, 4 * h)
+    x, res, res_out, normed = buf.split(h, 1)
+    want = P.add_rmsnorm_mxfp8(x.contiguous(), res.contiguous(), weight, mxfp8=False, bf16_out=True)
+    keep = buf.clone()
+    P.add_rmsnorm_mxfp8(x, res, weight, out=P.TailOutput(res_out, None, None, normed))
+    assert torch.equal(res_out, want.residual) and torch.equal(normed, want.normed) and torch.equal(buf[:, :2 * h], keep[:, :2 * h])
+    for bad in (buf[:, h - 8:2 * h - 8], buf[:, 8:h + 8], buf[:, 2 * h - 8:3 * h - 8]):
+        with pytest.raises(ValueError):
+            P.add_rmsnorm_mxfp8(x, res, weight, out=P.TailOutput(None, None, None, bad))
+    with pytest.raises(ValueError):
+        P.add_rmsnorm_mxfp8(x, res, weight, out=P.TailOutput(res_out, None, None, buf[:, 2 * h + 8:3 * h + 8]))
+
+
 def test_bits_of_the_tail_and_of_a_row_alone(P):
     """With one slot that is not zero the tail's sum is that slot, and its other steps are these; a row alone has the bits it has among others."""
     gen = torch.Generator(device="cuda").manual_seed(6)

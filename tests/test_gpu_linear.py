@@ -282,6 +282,88 @@ def test_sums_repeat_and_two_calls_at_once(P):
     assert all(torch.equal(y, w) for g, w in zip(got, want) for y in g)
 
 
+def test_two_captured_graphs_at_once(P):
+    """Graphs of bf16 calls (the rows' codes are the call's own) replayed on two streams, with inputs that change between replays."""
+    gen = gen_of(11)
+    weights = P.LinearWeights.from_row_major(*real(gen, 1032, 1056, 0.03), torch.randn(1032, generator=gen, device="cuda"))
+    ms = (30, 130, 700)
+    held = [torch.randn((m, 1056), generator=gen, device="cuda").bfloat16() for m in ms]
+    graphs, outs = [], []
+    for x in held:
+        P.mxfp8_linear(x, weights, activation="silu")
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            outs.append(P.mxfp8_linear(x, weights, activation="silu"))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for x in held:
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for graph, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, P.mxfp8_linear(x, weights, activation="silu")) for x, y in zip(held, outs))
+
+
+@pytest.mark.parametrize("m", [1, 6, 64, 65, 300, 1100])
+def test_columns_of_one_tensor(P, m):
+    """Rows, residual and result side by side in one tensor, the result beside and in the residual; what reaches into the rows is refused."""
+    gen = gen_of(12, m)
+    k, n = 544, 520
+    weights = P.LinearWeights.from_row_major(*real(gen, n, k, 0.05))
+    buf = torch.randn((m, k + 2 * n), generator=gen, device="cuda").bfloat16()
+    x, res, out = buf[:, :k], buf[:, k:k + n], buf[:, k + n:]
+    want = P.mxfp8_linear(x.contiguous(), weights, residual=res.contiguous())
+    keep = buf.clone()
+    assert P.mxfp8_linear(x, weights, residual=res, out=out) is out
+    assert torch.equal(out, want) and torch.equal(buf[:, :k + n], keep[:, :k + n])
+    P.mxfp8_linear(x, weights, residual=res, out=res)
+    assert torch.equal(res, want) and torch.equal(x, keep[:, :k])
+    for bad in (buf[:, k - 8:k - 8 + n], buf[:, :n], buf[:, 8:8 + n]):
+        with pytest.raises(ValueError):
+            P.mxfp8_linear(x, weights, out=bad)
+    with pytest.raises(ValueError):
+        P.mxfp8_linear(x, weights, residual=res, out=buf[:, k + 8:k + 8 + n])
+    torch.cuda.synchronize()
+    assert torch.equal(x, keep[:, :k])
+
+
+@pytest.mark.parametrize("m,stride", [(40, 1 << 26), (300, 1 << 23), (1100, 1 << 21)])
+def test_rows_beyond_32_bits(P, m, stride):
+    """bf16 rows, residual and result so far apart that the last begin behind 2^31 elements."""
+    gen = gen_of(13, m)
+    k, n = 544, 264
+    weights = P.LinearWeights.from_row_major(*real(gen, n, k, 0.05))
+    big = torch.empty((m, stride), dtype=torch.bfloat16, device="cuda")
+    x, res = big[:, :k], big[:, 1024:1024 + n]
+    x.copy_(torch.randn((m, k), generator=gen, device="cuda"))
+    res.copy_(torch.randn((m, n), generator=gen, device="cuda"))
+    want = P.mxfp8_linear(x.contiguous(), weights, residual=res.contiguous())
+    assert torch.equal(P.mxfp8_linear(x, weights, residual=res), want)
+    P.mxfp8_linear(x, weights, residual=res, out=res)
+    assert torch.equal(res, want)
+
+
+def test_codes_beyond_32_bits(P):
+    """Codes behind 2^31 bytes in, behind 2^32 bytes out: whole numbers, so that the rows of a smaller call have the same bits."""
+    gen = gen_of(14)
+    m, k, n = 1100000, 2080, 4096
+    x = torch.randint(-2, 3, (m, k), generator=gen, device="cuda", dtype=torch.int8)
+    codes = torch.empty((m, k), dtype=torch.uint8, device="cuda")
+    for part, to in zip(x.split(100000), codes.split(100000)):
+        to.copy_(part.to(torch.bfloat16).to(torch.float8_e4m3fn).view(torch.uint8))
+    scales = torch.randint(126, 129, (m, k // 32), generator=gen, device="cuda", dtype=torch.uint8)
+    weights = P.LinearWeights.from_row_major(*whole(gen, n, k))
+    got = P.mxfp8_linear((codes, scales), weights, activation="relu", mxfp8_out=True)
+    for at in (0, 524200, 1048500, m - 300):  # (2^31 / n and 2^32 / n are 524288 and 1048576)
+        want = P.mxfp8_linear((codes[at:at + 300], scales[at:at + 300]), weights, activation="relu", mxfp8_out=True)
+        assert torch.equal(got[0][at:at + 300], want[0]) and torch.equal(got[1][at:at + 300], want[1])
+
+
 def test_the_shared_expert_is_two_such_products(P):
     """The same weights through the shared expert: the norm's rows, a gated product to MXFP8, a product to bf16. The first product's
     sums may be ordered differently, so that a code may fall to the other side of a border: the results agree as two roundings do."""

@@ -153,3 +153,20 @@ def test_weights_refuse_bad_tensors():
 
 def test_output_columns():
     assert weights(gated=True).n == 32 and weights().n == 64 and L.MAX_DIM == 1 << 20
+
+
+@pytest.mark.parametrize("inter", [768, 1536])
+def test_c_abi_refuses_overlaps_with_all_that_is_read(inter):
+    """bf16 rows at every size (whether a launch in front quantises them or not), weights and bias; and rows of one stride side by side
+    that reach into one another."""
+    lib = _lib.load(inter)
+    X = 6 << 20
+    for m in (4, 64, 65, 300):
+        for bad in (dict(o=X), dict(o=X + 96 * 2 * m - 16), dict(xs=160, os=160, o=X + 2 * 88), dict(xs=160, os=160, o=X - 2 * 56), dict(xs=0, o=X)):
+            assert linear_call(lib, m=m, x=X, c=8 << 20, s=9 << 20, **bad) == _lib.E_ARG, (m, bad)
+    assert linear_call(lib, o=256 + 16512) == _lib.E_ARG and linear_call(lib, bias=3 << 20) == _lib.E_ARG
+    assert linear_call(lib, o=3 << 20, os=128, r=(3 << 20) + 112, rs=128) == _lib.E_ARG
+    assert linear_call(lib, o=(3 << 20) + 144, os=128, r=3 << 20, rs=128) == _lib.E_ARG  # its end reaches the next row's begin
+    quant = lambda x, st, c, s: lib.b200moe_quant_mxfp8(at(x), st, 4, 96, at(c), at(s), None)  # noqa: E731
+    assert quant(X, 96, X + 96 * 8 - 8, 8 << 20) == _lib.E_ARG and quant(X, 96, 8 << 20, X + 5) == _lib.E_ARG and quant(X, 96, 8 << 20, (8 << 20) + 300) == _lib.E_ARG
+    assert quant(X, 0, X + 96, 8 << 20) == _lib.E_ARG
