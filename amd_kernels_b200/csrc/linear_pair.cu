@@ -3,8 +3,8 @@
 // weight rows. No multicast.
 //
 // Unit = (pair of token blocks) x (pair of weight tiles). Two rings: 5 stages of codes, and 2 slots of the scales of four K-tiles that travel
-// ahead of them, so that the MMA warp waits for codes and, once in four K-tiles, for scales. The token scales come row-major, as every producer of this package writes them: the scale
-// warp turns them into atoms on the way, so no launch in front of the product re-lays them.
+// ahead of them, so that the MMA warp waits for codes and, once in four K-tiles, for scales. The token scales come row-major, as every
+// producer of this package writes them: the scale warp turns them into atoms on the way, so no launch in front of the product re-lays them.
 //
 //   warp 0      code producer (both CTAs): TMA of the CTA's 128 token rows and of its weight rows, counted on the leader's barrier
 //   warp 1      tensor memory (both CTAs); in the leader it issues the MMAs for both, the whole warp around one elected lane
@@ -66,14 +66,17 @@ __device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t
   return ok != 0;
 }
 
-// The units in groups of 8 pairs of token blocks: a group sweeps the weights once, tile by tile, so that its tokens (2048 rows) and the
-// few tiles in work stay in L2 whatever the size of the weights.
+// The units in groups of 16 pairs of token blocks: a group sweeps the weights once, tile by tile, so that its tokens (4096 rows) and the
+// few tiles in work stay in L2 whatever the size of the weights. What the SMs read of L2 (64 bytes a cycle each) comes near what it gives
+// them, more where neighbours read the same. Measured back to back, us, groups of 8 / 12 / 16 / 24 / 32: 4095 x 6144 -> 8192
+// 178 / 177 / 173 / 172 / 172, 8192 x 6144 -> 4096 gated 343 / 343 / 335 / 336 / 341, 16384 x 6144 -> 6144 548 / 539 / 538 / 547 / 575.
 struct LinearUnits {
+  static constexpr int kGroup = 16;
   int pairs, steps_n;  // pairs of token blocks, units along N
   __device__ __forceinline__ int total() const { return pairs * steps_n; }
   __device__ __forceinline__ void at(int u, int& pair, int& step) const {
-    const int group = u / (8 * steps_n), first = group * 8, rest = u - group * 8 * steps_n;
-    const int rows = pairs - first < 8 ? pairs - first : 8;
+    const int group = u / (kGroup * steps_n), first = group * kGroup, rest = u - group * kGroup * steps_n;
+    const int rows = pairs - first < kGroup ? pairs - first : kGroup;
     step = rest / rows;
     pair = first + rest % rows;
   }
