@@ -80,8 +80,8 @@ static int launch_quant(const uint4* x, int64_t x_stride, int64_t rows, int vect
   const int wide = vectors < V * 512 ? vectors : V * 512;
   const int threads = ((wide + V - 1) / V + 31) / 32 * 32, rows_per_cta = threads >= 128 ? 1 : 256 / threads;
   const int64_t grid = (rows + rows_per_cta - 1) / rows_per_cta;
-  B200MOE_LAUNCH(quant_mxfp8_kernel<V>, dim3(static_cast<unsigned>(grid), (vectors + V * threads - 1) / (V * threads)), dim3(threads, rows_per_cta), 0, stream, x, x_stride, rows,
-                 vectors, codes, scales);
+  B200MOE_LAUNCH(quant_mxfp8_kernel<V>, dim3(static_cast<unsigned>(grid), (vectors + V * threads - 1) / (V * threads)),
+                 dim3(threads, rows_per_cta), 0, stream, x, x_stride, rows, vectors, codes, scales);
   return 0;
 }
 
@@ -123,8 +123,9 @@ int set_wait_limit_linear(unsigned long long ns) {
 }
 
 // CTAs along K for `units` (weight tile, token block): the most of 1, 2 and 4 whose clusters are all resident at once (a second round of
-// clusters costs more than any split gives: 6144 -> 6144, one row, 10.4 us with 4, 16 with 6), and 8 where they do not fill the SMs
-// once (4096 -> 2048: 5.2 against 6.3 with 4; 6144 -> 4096, 256 CTAs of 8: 8.5 against 8.8 for a row, 16.1 against 14.7 for 128). 0: no one round.
+// clusters costs more than any split gives: 6144 -> 6144, one row, 10.0 us with 4, 14.3 with 8), and 8 where they do not fill the SMs
+// once (4096 -> 2048: 5.3 against 6.3 with 4; where they do, 6144 -> 4096 in 256 CTAs, 8.8 against 8.5 for a row, 16.1 against 14.8 for 128).
+// 0: no one round.
 static int splits_for(const LinearArgs& a, int bm, int64_t units) {
   for (int log = 3; log >= 0; --log) {
     if ((1 << log) > a.tiles_k || (log == 3 && units * 8 > sm_count())) continue;
@@ -135,11 +136,11 @@ static int splits_for(const LinearArgs& a, int bm, int64_t units) {
 
 // The kernel, its token block and its split of K. Measured, us, 6144 -> 6144 (4096; 12288) unless said otherwise:
 //   up to 128 rows the smallest block that holds them, so that the weights stream once; but two blocks of half the rows where these
-//   still split K by 4 (33 to 64 rows: 10.7 / 11.4 at 4096, 14.1 / 13.1 at 6144 with a split of 2) or by 2 (65 to 128 rows: 12.2 / 14.7 at
-//   4096, 16.3 / 16.4 at 6144, 25.7 / 22.7 at 12288 without a split).
-//   More rows: blocks of 128 on one CTA while they split K by 2 in one round, else CTA pairs: 256 rows 21.1 / 25.4, 384 21.1 / 25.7, 512
-//   34.3 / 26.2; 1024 rows 6144 -> 2048 20.5 / 24.3, 1536 33.4 / 25.7. Without a split too where they need one round and the pairs two
-//   (384 rows at 12288: 35.7 / 42.1).
+//   still split K by 4 (33 to 64 rows: 10.6 / 11.2 at 4096; 13.7 / 13.1 at 6144 with a split of 2) or by 2 (65 to 128 rows: 12.4 / 14.8 at
+//   4096, 15.6 / 16.6 at 6144; 23.9 / 22.0 at 12288 without a split).
+//   More rows: blocks of 128 on one CTA while they split K by 2 in one round, else CTA pairs: 256 rows 20.2 / 24.9, 384 20.9 / 24.7, 512
+//   30.8 / 25.2; 1024 rows 6144 -> 2048 19.6 / 23.2, 1536 30.1 / 24.1. Without a split too where they need one round and the pairs two
+//   (384 rows at 12288: 33.7 / 40.7).
 static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   const int64_t blocks = (a.m + 127) / 128;
   int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;

@@ -12,11 +12,16 @@
 //   warp 3      scales (both CTAs): the CTA's token rows through registers, the atoms of the weight tiles by TMA
 //   warps 4-11  epilogue (both CTAs): thread = one token row, 128 columns. The sums are pulled into registers and the accumulator
 //               is handed back; then bias, activation, residual and one rounding, 32 columns at a time. bf16 rows go through a strip of
-//               shared memory per warp, pieces of 32 rows x 32 columns: the residual arrives by TMA, two pieces ahead, the result leaves by TMA. (A
-//               thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the operands of
-//               the MMAs wait: with them a residual made 16384 x 6144 -> 6144 28 % slower.)
+//               shared memory per warp, pieces of 32 rows x 32 columns: the residual arrives by TMA, two pieces ahead, the result
+//               leaves by TMA. (A thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the
+//               operands of the MMAs wait: with them a residual made 16384 x 6144 -> 6144 28 % slower.)
 // 12 warps start with 168 registers; the issuing warpgroup drops to 88, the epilogue's rise to 208 (4 x 88 + 8 x 208 = 12 x 168: the
 // exchange must balance inside what the CTA was given at launch).
+//
+// What bounds it: the tensor pipe for long sums and many rows (4095 x 6144 -> 8192: busy 77 % of the cycles; the rest are the start, the ends
+// of units and waits for L2, 14 TB/s of operands) and the power limit: back to back the clock falls from 1.9 to 1.3 GHz, where
+// 16384 x 6144 -> 6144 takes 538 us (2.3 PFLOP/s; 445 us in a short burst, 2.8). A call of few K-tiles is bound by its epilogue and by
+// what starting and ending it costs, 11 us in all.
 #include "linear.cuh"
 #include "tc_pair.cuh"
 
@@ -51,7 +56,7 @@ __device__ __forceinline__ void tc_mma_mxf8_two(uint32_t d, uint32_t a_lo, uint3
 
 // Arrival on a barrier of another CTA of the cluster that orders what this thread has seen before it, and the wait that sees it. The
 // arrival waits for everything that its thread has in flight, so a thread without loads does it for the scale warp, whose own arrival is
-// local: with the scale warp arriving itself a group of K-tiles took 3400 cycles instead of 2300 (8192 rows 256 -> 219 us).
+// local: with the scale warp arriving itself a group of four K-tiles took 3400 cycles instead of 2300.
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -410,8 +415,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty_leader);
       // A loop of one piece: unrolled, the code of a unit does not stay in the instruction cache. The piece is picked from the accumulator's
-      // registers, or they move up behind it (GELU, gated); an activation takes 16 columns at a time. Measured, 2048 x 800 -> 5984: SiLU
-      // 27.4 us in this order, 32.5 with the registers moving up and pair behind pair; GELU 30.6, 31.7 picked and 16 columns at a time.
+      // registers, or they move up behind it (GELU, gated); an activation takes 16 columns at a time, GELU 4. 2048 x 800 -> 5984: SiLU 26.2 us
+      // (19 % more with the registers moving up and pair behind pair), GELU 27.8 (4 % more picked and 16 columns at a time).
       uint32_t scale_bytes = 0;
       bool ok = true;
 #pragma unroll 1

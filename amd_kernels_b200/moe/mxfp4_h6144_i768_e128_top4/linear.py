@@ -90,7 +90,8 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
     (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart.
     Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.
     ``out``: where the result goes, a bf16 tensor or a pair (``mxfp8_out`` is then not read); a bf16 ``out`` may be the residual
-    itself, and nothing else that the call reads. The sums of one call repeat bit for bit; between calls of different M they may be split along K in another way."""
+    itself, and nothing else that the call reads. The sums of one call repeat bit for bit; between calls of different M they may be
+    split along K in another way."""
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
