@@ -9,7 +9,7 @@ from dataclasses import dataclass
 import torch
 
 from ... import _lib
-from .add_rmsnorm import check_mxfp8, check_rows, launch_on, row_stride
+from .add_rmsnorm import check_mxfp8, check_rows, launch_on, new_rows, row_stride
 from .chain import status_word
 
 MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
@@ -73,7 +73,7 @@ def mxfp8_quant(x: torch.Tensor, *, out=None):
         raise ValueError(f"rows of {k} columns (needs a multiple of 32, up to {MAX_DIM}; up to {MAX_ROWS} rows)")
     stride = k if x.is_contiguous() else row_stride("x", x, m, k, True)
     if out is None:
-        out = torch.empty((m, k), dtype=torch.uint8, device=x.device), torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
+        out = new_rows(m, k, torch.uint8, x), new_rows(m, k // 32, torch.uint8, x)
     else:
         check_mxfp8("out", *out, m, k, device)
     launch_on(device, _lib.load().b200moe_quant_mxfp8, x.data_ptr(), stride, m, k, out[0].data_ptr(), out[1].data_ptr())
@@ -108,7 +108,7 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
         xs, x_at = k if x.is_contiguous() else row_stride("x", x, m, k, True), x.data_ptr()
         c_at = s_at = 0
         if m > ROWS_INSIDE:
-            quantised = torch.empty(m * (k + k // 32), dtype=torch.uint8, device=x.device)
+            quantised = tiles.new_empty(m * (k + k // 32))
             c_at = quantised.data_ptr()
             s_at = c_at + m * k
     elif isinstance(x, (tuple, list)) and len(x) == 2 and x[0] is not None:
@@ -122,10 +122,14 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
         rs, r_at = check_rows("residual", residual, (m, n), device), residual.data_ptr()
     if out is None:
         if mxfp8_out:
-            out = torch.empty((m, n), dtype=torch.uint8, device=tiles.device), torch.empty((m, n // 32), dtype=torch.uint8, device=tiles.device)
+            if n % 32:
+                raise ValueError(f"MXFP8 output of {n} columns (needs a multiple of 32)")
+            out = new_rows(m, n, torch.uint8, tiles), new_rows(m, n // 32, torch.uint8, tiles)
+            oc_at, os_at = out[0].data_ptr(), out[1].data_ptr()
         else:
-            out = torch.empty((m, n), dtype=torch.bfloat16, device=tiles.device)
-    if isinstance(out, torch.Tensor):
+            out = new_rows(m, n, torch.bfloat16, tiles)
+            y_at = out.data_ptr()
+    elif isinstance(out, torch.Tensor):
         ys, y_at = check_rows("out", out, (m, n), device), out.data_ptr()
     else:
         if n % 32:
