@@ -29,6 +29,7 @@ namespace b200moe {
 
 struct LinearPairCfg {
   static constexpr int kStages = 5;                // code ring (6 stages and no strips were 0 to 1 % faster, 4 were 5 % slower)
+  static constexpr int kAhead = 8;                 // K-tiles between a weight tile's way into L2 and into the ring
   static constexpr int kSfSlots = 2;               // groups of scales in shared memory
   static constexpr int kWOff = 128 * 128;          // the CTA's weight tile, behind its 128 token rows
   static constexpr int kStageBytes = 2 * 128 * 128;
@@ -164,7 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
   }
   if (cluster < total && (warp == 0 || warp == 3)) {
     units.at(cluster, pair, step);
-    const int row = pair * 256 + static_cast<int>(rank) * 128, tile = 2 * step + static_cast<int>(rank), n = tiles_k < 8 ? tiles_k : 8;
+    const int row = pair * 256 + static_cast<int>(rank) * 128, tile = 2 * step + static_cast<int>(rank), n = tiles_k < C::kAhead ? tiles_k : C::kAhead;
     if (warp == 3) {
       RowScales(args.scales, args.m, args.k).prefetch<4>(row + lane, 0);
     } else if (lane == 0) {
@@ -190,6 +191,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
     if (warp == 0) {
       // ---------------------------------------------------------------- code producer (both CTAs)
       pdl_wait();
+      launder(a.tiles);
       if (cluster < total) scales_first_wait();
       if (lane == 0) {
         const uint32_t full0 = map_to_cta(smem_u32(&bar_full[0]), 0);  // the leader's barriers, as seen from this CTA
@@ -199,6 +201,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
           units.at(u, pair, step);
           const int row = pair * 256 + static_cast<int>(rank) * 128;
           int rec = (2 * step + static_cast<int>(rank)) * tiles_k * 128;  // the images seen as rows of 128 bytes
+          // Few clusters read a weight tile and wait for HBM with it: one of them asks for it ahead of the ring. (512 x 8192 -> 4096 29.7 -> 28.6
+          // us, 777 x 6144 -> 6144 39.8 -> 38.9; with 16 that read it 4095 x 6144 -> 8192 150.7 -> 152.8.)
+          const int ahead_end = units.pairs <= 4 && pair == 0 && 2 * step + static_cast<int>(rank) < a.tiles_n ? tiles_k - C::kAhead : 0;
           for (int kt = 0; kt < tiles_k; ++kt, ++it, rec += 128) {
             if (!mbar_wait(smem_u32(&bar_empty[s]), ph, abort_v, status)) { ok = false; break; }
             const uint32_t full = full0 + 8u * s, base = tiles + s * C::kStageBytes;
@@ -206,6 +211,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LinearPairCfg::kThre
             // rows beyond the last token or the last weight tile are read as zeros and count all the same
             tma_load_2d_pair(base, &map_x, kt * 128, row, full);
             tma_load_2d_pair(base + C::kWOff, &map_wc, 0, rec, full);
+            if (kt < ahead_end)
+              l2_prefetch_bulk(a.tiles + (static_cast<int64_t>(rec) + C::kAhead * 128) * 128, kLinearImageBytes);
             if (++s == C::kStages) { s = 0; ph ^= 1u; }
           }
         }
