@@ -138,9 +138,9 @@ static int splits_for(const LinearArgs& a, int bm, int64_t units) {
 //   up to 128 rows the smallest block that holds them, so that the weights stream once; but two blocks of half the rows where these
 //   still split K by 4 (33 to 64 rows: 10.6 / 11.2 at 4096; 13.7 / 13.1 at 6144 with a split of 2) or by 2 (65 to 128 rows: 12.4 / 14.8 at
 //   4096, 15.6 / 16.6 at 6144; 23.9 / 22.0 at 12288 without a split).
-//   More rows: blocks of 128 on one CTA while they split K by 2 in one round, else CTA pairs: 256 rows 20.2 / 24.9, 384 20.9 / 24.7, 512
-//   30.8 / 25.2; 1024 rows 6144 -> 2048 19.6 / 23.2, 1536 30.1 / 24.1. Without a split too where they need one round and the pairs two
-//   (384 rows at 12288: 33.7 / 40.7).
+//   More rows: blocks of 128 on one CTA while they split K by 2 in one round, else CTA pairs: 256 rows 20.2 / 23.9, 384 20.8 / 24.1, 512
+//   30.6 / 24.4; 1024 rows 6144 -> 2048 19.6 / 22.7, 1536 29.9 / 24.0. Without a split too where they need one round and the pairs two
+//   (384 rows at 12288: 33.3 / 39.7).
 static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   const int64_t blocks = (a.m + 127) / 128;
   int bm = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
