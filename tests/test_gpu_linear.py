@@ -154,6 +154,28 @@ def test_gated_against_the_formula(P, m, k, n, act):
     assert bool(((got - y).abs() <= 2.0 ** -8 * y.abs() + 1.01 * slack).all())
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 800, 96), (37, 544, 160), (200, 288, 640), (1000, 160, 416), (2200, 288, 4160)])
+@pytest.mark.parametrize("act", [None, "silu", "gelu", "swiglu", "swiglu_oai"])
+def test_mxfp8_result_with_a_residual(P, m, k, n, act):
+    """The block's scale is that of the sum with the residual; codes that begin at 16 bytes of a sector, scales at any byte."""
+    gen = gen_of(m, k, n, act, "mx")
+    gated = act is not None and act.startswith("swiglu")
+    rows = 2 * n if gated else n
+    x, w = real(gen, m, k), real(gen, rows, k, 1.5 / math.sqrt(k))
+    bias = 0.5 * torch.randn(rows, generator=gen, device="cuda")
+    res = (3 * torch.randn((m, n), generator=gen, device="cuda")).bfloat16()
+    weights = P.LinearWeights.from_row_major(*w, bias, gated=gated)
+    y, slack = formula(x, w, bias, act, res)
+    codes, scales = P.mxfp8_linear(x, weights, activation=act, residual=res, mxfp8_out=True)
+    check_codes(codes, scales, y, 1, 0.0, slack)
+    room, sroom = (torch.full((size + 48,), 93, dtype=torch.uint8, device="cuda") for size in (m * n, m * (n // 32)))
+    out = room[16:m * n + 16].view(m, n), sroom[3:m * (n // 32) + 3].view(m, n // 32)
+    P.mxfp8_linear(x, weights, activation=act, residual=res, out=out)
+    assert torch.equal(out[0], codes) and torch.equal(out[1], scales)
+    assert bool((room[:16] == 93).all()) and bool((room[m * n + 16:] == 93).all())
+    assert bool((sroom[:3] == 93).all()) and bool((sroom[m * (n // 32) + 3:] == 93).all())
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 96, 40), (2, 6144, 1024), (13, 800, 136), (31, 1056, 640), (60, 2048, 264), (64, 512, 4096), (65, 512, 96), (300, 544, 136), (1300, 160, 520)])
 def test_bf16_rows_strides_and_in_place(P, m, k, n):
     gen = gen_of(m, k, n)
