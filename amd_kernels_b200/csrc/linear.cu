@@ -87,7 +87,7 @@ static int launch_quant(const uint4* x, int64_t x_stride, int64_t rows, int vect
 
 // ------------------------------------------------------------------------------------------------ the call
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream);  // linear_tc.cu
-int linear_tc_resident(int bm, int log_splits);
+const int* linear_tc_resident(int bm);
 int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_pair.cu
 int linear_pair_resident();
 int set_wait_limit_linear_tc(unsigned long long ns);
@@ -122,16 +122,23 @@ int set_wait_limit_linear(unsigned long long ns) {
   return r ? r : set_wait_limit_linear_pair(ns);
 }
 
-// CTAs along K for `units` (weight tile, token block): the most of 1, 2 and 4 whose clusters are all resident at once (a second round of
-// clusters costs more than any split gives: 6144 -> 6144, one row, 10.0 us with 4, 14.3 with 8), and 8 where they do not fill the SMs
-// once (4096 -> 2048: 5.3 against 6.3 with 4; where they do, 6144 -> 4096 in 256 CTAs, 8.8 against 8.5 for a row, 16.1 against 14.8 for 128).
-// 0: no one round.
+// CTAs along K for `units` (weight tile, token block). All clusters have to be resident at once: a second round of them costs more than any
+// split gives (6144 -> 6144, one row, 10.2 us with 4, 15.8 with 6). Of 4, 6 and 8 the one whose longest part has the fewest groups of
+// four K-tiles; of equals the smallest, the largest up to 8 units: one row 6144 -> 2560 with 4 / 6 / 8 8.1 / 7.1 / 7.3 (3 / 2 / 2 groups),
+// 4096 -> 1024 6.1 / 5.7 / 5.1 (2 / 2 / 1), 6144 -> 1024 7.3 / 6.3 / 5.8, 1536 -> 2048 4.6 each (1); 64 rows 6144 -> 5120 13.0 / 12.0.
+// With more than 32 rows a block 6 and 8 only where their parts are whole groups: 100 rows 8192 -> 2048 11.9 / 12.6. (Where 4 put a CTA on
+// each SM, 6 can lose: 16 rows 6144 -> 4096 8.9 / 9.3; one row 8.5 / 8.3.) Else 2 or 1. 0: no one round.
 static int splits_for(const LinearArgs& a, int bm, int64_t units) {
-  for (int log = 3; log >= 0; --log) {
-    if ((1 << log) > a.tiles_k || (log == 3 && units * 8 > sm_count())) continue;
-    if (units <= linear_tc_resident(bm, log)) return 1 << log;
+  const int* resident = linear_tc_resident(bm);
+  int best = 0, best_groups = 0;
+  for (int splits : {4, 6, 8, 2, 1}) {
+    if (units <= 8 && splits >= 4) splits = 12 - splits;
+    if (splits > a.tiles_k || (splits < 4 && best) || units > resident[splits]) continue;
+    if (splits > 4 && bm > 32 && a.tiles_k % (splits * kSfGroup)) continue;
+    const int groups = ((a.tiles_k + splits - 1) / splits + kSfGroup - 1) / kSfGroup;
+    if (!best || groups < best_groups) best = splits, best_groups = groups;
   }
-  return 0;
+  return best;
 }
 
 // The kernel, its token block and its split of K. Measured, us, 6144 -> 6144 (4096; 12288) unless said otherwise:
@@ -147,7 +154,7 @@ static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t st
   int splits = splits_for(a, bm, blocks * a.tiles_n);
   if (blocks == 1 && bm >= 64) {
     const int half = splits_for(a, bm / 2, 2 * static_cast<int64_t>(a.tiles_n));
-    if (half >= (bm == 64 ? 4 : 2)) bm /= 2, splits = half;
+    if (half >= (bm == 64 ? 4 : 2) && 2 * half >= splits) bm /= 2, splits = half;
   }
   if (blocks > 1) {
     const int64_t pairs = (a.m + 255) / 256 * ((a.tiles_n + 1) / 2);

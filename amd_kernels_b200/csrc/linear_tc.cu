@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(256, LinearCfg<BM>::kCtasPerSm)
     if (splits == 4) finish_rows<C::kSumRow, 4>(a, row0, rows, first, tile, parts, lane);
     else if (splits == 2) finish_rows<C::kSumRow, 2>(a, row0, rows, first, tile, parts, lane);
     else if (splits == 1) finish_rows<C::kSumRow, 1>(a, row0, rows, first, tile, parts, lane);
+    else if (splits == 6) finish_rows<C::kSumRow, 6>(a, row0, rows, first, tile, parts, lane);
     else finish_rows<C::kSumRow, 8>(a, row0, rows, first, tile, parts, lane);
   }
   __syncwarp();
@@ -484,36 +485,38 @@ static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cu
   return static_cast<int>(cudaLaunchKernelEx(&cfg, linear_tc_kernel<BM, QUANT>, mx, a, splits, static_cast<int>(n_blocks), status));
 }
 
-// Clusters of `1 << log_splits` CTAs that run at once on the current device; asked once per device. The occupancy calculation counts one CTA
+// Clusters of [splits] CTAs that run at once on the current device; asked once per device. The occupancy calculation counts one CTA
 // an SM for kernels that use tensor memory, whatever their shared memory (it says one at 60 KB too); two run (288 CTAs in clusters of two
 // take the time of 192), so its number is doubled.
 template <int BM>
-static int resident_clusters(int log_splits) {
+static const int* resident_clusters() {
   static std::mutex mu;
-  static int known[kMaxDevices][4] = {};  // 1 + the number
+  static bool known[kMaxDevices] = {};
+  static int clusters[kMaxDevices][9] = {};
+  static const int none[9] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || configure_linear_tc<BM, false>()) return 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return none;
   std::lock_guard<std::mutex> lock(mu);
-  int& n = known[dev][log_splits];
-  if (n == 0) {
-    int got = sm_count();
-    cudaLaunchAttribute attr[2];
-    const cudaLaunchConfig_t cfg = linear_tc_config<BM, false>(sm_count(), 1 << log_splits, attr, nullptr);
-    if (log_splits > 0 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM, false>, &cfg) != cudaSuccess) got = 0;
-    (void)cudaGetLastError();
-    n = 1 + LinearCfg<BM>::kCtasPerSm * got;
+  if (!known[dev]) {
+    if (configure_linear_tc<BM, false>()) return none;
+    for (const int splits : {1, 2, 4, 6, 8}) {
+      int got = sm_count();
+      cudaLaunchAttribute attr[2];
+      const cudaLaunchConfig_t cfg = linear_tc_config<BM, false>(sm_count(), splits, attr, nullptr);
+      if (splits > 1 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM, false>, &cfg) != cudaSuccess) got = 0;
+      (void)cudaGetLastError();
+      clusters[dev][splits] = LinearCfg<BM>::kCtasPerSm * got;
+    }
+    known[dev] = true;
   }
-  return n - 1;
+  return clusters[dev];
 }
 
-int linear_tc_resident(int bm, int log_splits) {
-  return bm == 16   ? resident_clusters<16>(log_splits)
-         : bm == 32 ? resident_clusters<32>(log_splits)
-         : bm == 64 ? resident_clusters<64>(log_splits)
-                    : resident_clusters<128>(log_splits);
+const int* linear_tc_resident(int bm) {
+  return bm == 16 ? resident_clusters<16>() : bm == 32 ? resident_clusters<32>() : bm == 64 ? resident_clusters<64>() : resident_clusters<128>();
 }
 
-// bm: 16, 32, 64 or 128 token rows a block (a.x given: 16, 32 or 64); splits: 1, 2, 4 or 8 CTAs along K, at most the K-tiles
+// bm: 16, 32, 64 or 128 token rows a block (a.x given: 16, 32 or 64); splits: 1, 2, 4, 6 or 8 CTAs along K, at most the K-tiles
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream) {
   switch (bm) {
     case 16: return a.x ? launch_linear_tc<16, true>(a, splits, status, stream) : launch_linear_tc<16, false>(a, splits, status, stream);
