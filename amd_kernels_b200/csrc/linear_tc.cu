@@ -1,7 +1,7 @@
 // The MXFP8 product for few rows: tcgen05.mma kind::mxf8f6f4 block-scaled with the weight tile as the 128-row M operand and a block of
 // BM token rows as N, so that one pass over the weights serves the whole block.
 //
-// What bounds it: the weight stream (HBM; one row 6144 -> 4096 takes 8.5 us, 4.0 at the copy rate; a call without work takes 4.3). One CTA =
+// What bounds it: the weight stream (HBM; one row 6144 -> 4096 takes 8.3 us, 4.0 at the copy rate; a call without work takes 3 to 4). One CTA =
 // (weight tile, token block, part of K). K is split over the CTAs of a cluster until there are enough of them to keep every SM loading;
 // each adds its part in tensor memory and writes it to its shared memory; after a cluster barrier the CTAs share out the block's
 // rows: the parts of a row are fetched and added in the order of K, then bias, activation, residual and the only rounding. No workspace, no atomics, one launch, sums in a fixed order. What bounds the end of a call is distributed
