@@ -234,6 +234,10 @@ static int linear_args(LinearArgs& a, const b200moe_linear_call* call, const int
     if (!in_place && rows_overlap(o, residual)) return B200MOE_E_ARG;
   }
   if (rows_overlap(outs[1], outs[2])) return B200MOE_E_ARG;
+  if (c.x && !inside) {  // the quantiser in front writes these two (and compares them with x): nothing else that the product reads
+    for (const RowSpan& scratch : {ins[1], ins[2]})
+      if (rows_overlap(scratch, residual) || rows_overlap(scratch, ins[3]) || rows_overlap(scratch, ins[4])) return B200MOE_E_ARG;
+  }
   a.tiles = w->tiles;
   a.bias = w->bias;
   a.x = inside ? static_cast<const __nv_bfloat16*>(c.x) : nullptr;

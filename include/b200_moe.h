@@ -478,8 +478,8 @@ typedef struct b200moe_linear_weights {
  * B200MOE_LINEAR_ROWS_INSIDE rows inside the product (codes8 and scales8 are not used), more of them into codes8 and scales8 by a launch
  * in front (b200moe_quant_mxfp8). residual, out and x are bf16 rows (16-byte aligned; strides in elements, multiples of 8; a stride of 0
  * of x is one row for all). Either out, or out_codes8 [m][n] (16-byte aligned) and out_scales8 [m][n/32]. out may be the
- * residual (same address and stride); any other overlap of an output with what the call reads is B200MOE_E_ARG (column ranges of one
- * tensor do not overlap). m may be 0. */
+ * residual (same address and stride); any other overlap of an output, or of codes8 and scales8 where the call writes them, with what
+ * the call reads is B200MOE_E_ARG (column ranges of one tensor do not overlap). m may be 0. */
 typedef struct b200moe_linear_call {
   b200moe_linear_weights w;
   const void* x; /* or null */

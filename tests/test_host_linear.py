@@ -170,3 +170,19 @@ def test_c_abi_refuses_overlaps_with_all_that_is_read(inter):
     quant = lambda x, st, c, s: lib.b200moe_quant_mxfp8(at(x), st, 4, 96, at(c), at(s), None)  # noqa: E731
     assert quant(X, 96, X + 96 * 8 - 8, 8 << 20) == _lib.E_ARG and quant(X, 96, 8 << 20, X + 5) == _lib.E_ARG and quant(X, 96, 8 << 20, (8 << 20) + 300) == _lib.E_ARG
     assert quant(X, 0, X + 96, 8 << 20) == _lib.E_ARG
+
+
+@pytest.mark.parametrize("inter", [768, 1536])
+def test_c_abi_refuses_a_scratch_over_what_the_product_reads(inter):
+    """More than 64 bf16 rows are quantised into codes8 and scales8 in front of the product: neither may reach into what it reads then."""
+    lib = _lib.load(inter)
+    X, C, S, R, W, B = 6 << 20, 8 << 20, 9 << 20, 10 << 20, 11 << 20, 12 << 20
+    for m in (65, 300):
+        for over, end in ((R, 2 * 64 * m), (W, 16896), (B, 4 * 64), (X, 2 * 96 * m)):
+            for bad in (dict(c=over), dict(s=over), dict(c=over + end - 16), dict(s=over + end - 1), dict(c=over - 96 * m + 16), dict(s=over - 3 * m + 1)):
+                call = dict(m=m, x=X, c=C, s=S, r=R, tiles=W, bias=B)
+                call.update(bad)
+                assert linear_call(lib, **call) == _lib.E_ARG, (m, bad)
+        assert linear_call(lib, m=m, x=X, c=C, s=C + 96 * m - 1, r=R, tiles=W, bias=B) == _lib.E_ARG
+    # a residual of rows that are wider apart: the scratch may not lie in its gaps either (their strides differ)
+    assert linear_call(lib, m=300, x=X, c=R + 160, s=S, r=R, rs=512, tiles=W, bias=B) == _lib.E_ARG
