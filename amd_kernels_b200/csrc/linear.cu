@@ -89,7 +89,7 @@ static int launch_quant(const uint4* x, int64_t x_stride, int64_t rows, int vect
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream);  // linear_tc.cu
 const int* linear_tc_resident(int bm);
 int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_pair.cu
-int linear_pair_resident();
+int linear_pair_resident(const LinearArgs& a);
 int set_wait_limit_linear_tc(unsigned long long ns);
 int set_wait_limit_linear_pair(unsigned long long ns);
 
@@ -156,9 +156,10 @@ static int dispatch_linear(const LinearArgs& a, int32_t* status, cudaStream_t st
     const int half = splits_for(a, bm / 2, 2 * static_cast<int64_t>(a.tiles_n));
     if (half >= (bm == 64 ? 4 : 2) && 2 * half >= splits) bm /= 2, splits = half;
   }
-  if (blocks > 1) {
+  if (blocks > 1) {  // (no pair resident: the one-CTA kernel, which needs no cluster without a split, takes any size)
     const int64_t pairs = (a.m + 255) / 256 * ((a.tiles_n + 1) / 2);
-    if (splits == 0 || (splits == 1 && pairs <= linear_pair_resident())) return linear_pair(a, status, stream);
+    const int resident = linear_pair_resident(a);
+    if (resident > 0 && (splits == 0 || (splits == 1 && pairs <= resident))) return linear_pair(a, status, stream);
   }
   return linear_tc(a, bm, splits ? splits : 1, status, stream);
 }

@@ -636,8 +636,15 @@ int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream) {
   return linear_pair_out<kGated>(a, status, stream);
 }
 
-// Pairs that are resident at once (the kinds do not differ in what they hold)
-int linear_pair_resident() { return linear_pairs<kLinear, false>(); }
+// Pairs of the call's kernel that are resident at once (0: cluster launch unavailable)
+int linear_pair_resident(const LinearArgs& a) {
+  switch (a.act.kind) {
+    case kLinear: return a.out ? linear_pairs<kLinear, false>() : linear_pairs<kLinear, true>();
+    case kSigmoid: return a.out ? linear_pairs<kSigmoid, false>() : linear_pairs<kSigmoid, true>();
+    case kGelu: return a.out ? linear_pairs<kGelu, false>() : linear_pairs<kGelu, true>();
+  }
+  return a.out ? linear_pairs<kGated, false>() : linear_pairs<kGated, true>();
+}
 
 int set_wait_limit_linear_pair(unsigned long long ns) { return set_wait_limit_here(ns); }
 

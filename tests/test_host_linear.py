@@ -186,3 +186,14 @@ def test_c_abi_refuses_a_scratch_over_what_the_product_reads(inter):
         assert linear_call(lib, m=m, x=X, c=C, s=C + 96 * m - 1, r=R, tiles=W, bias=B) == _lib.E_ARG
     # a residual of rows that are wider apart: the scratch may not lie in its gaps either (their strides differ)
     assert linear_call(lib, m=300, x=X, c=R + 160, s=S, r=R, rs=512, tiles=W, bias=B) == _lib.E_ARG
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="stands for a device on which no CTA pair can be resident")
+@pytest.mark.parametrize("inter", [768, 1536])
+def test_without_resident_pairs_the_one_cta_kernel_takes_many_rows(inter):
+    """The one-CTA kernel takes any size. Here its launch fails for want of a device; the pair kernel would have said E_DRIVER."""
+    lib = _lib.load(inter)
+    for call in (dict(m=300, c=8 << 20, s=9 << 20), dict(m=300, c=8 << 20, s=9 << 20, act=3), dict(m=300, c=8 << 20, s=9 << 20, gated=1, act=5),
+                 dict(m=5000, c=8 << 20, s=9 << 20, o=None, oc=16 << 20, osc=12 << 20)):
+        one_row = linear_call(lib, **{**call, "m": 1})
+        assert one_row > 0 and linear_call(lib, **call) == one_row  # a CUDA error code, the same for one row
