@@ -719,10 +719,8 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 // ------------------------------------------------------------------------------------------------ host side
 // CTA pairs that can be resident at once on the current device (0: cluster launch unavailable)
 static int resident_pairs() {
-  static std::mutex mu;
-  static int pairs[kMaxDevices] = {};
-  static bool known[kMaxDevices] = {};
-  return resident_pairs_of(gemm1_pair_kernel, PairCfg::kThreads, PairCfg::kSmemBytes, mu, known, pairs);
+  static PerDeviceAnswer<int> count;
+  return resident_pairs_of(gemm1_pair_kernel, PairCfg::kThreads, PairCfg::kSmemBytes, count);
 }
 
 int set_wait_limit_pair(unsigned long long ns) { return set_wait_limit_here(ns); }

@@ -87,7 +87,7 @@ static int launch_quant(const uint4* x, int64_t x_stride, int64_t rows, int vect
 
 // ------------------------------------------------------------------------------------------------ the call
 int linear_tc(const LinearArgs& a, int bm, int splits, int32_t* status, cudaStream_t stream);  // linear_tc.cu
-const int* linear_tc_resident(int bm);
+LinearResident linear_tc_resident(int bm);
 int linear_pair(const LinearArgs& a, int32_t* status, cudaStream_t stream);  // linear_pair.cu
 int linear_pair_resident(const LinearArgs& a);
 int set_wait_limit_linear_tc(unsigned long long ns);
@@ -129,11 +129,11 @@ int set_wait_limit_linear(unsigned long long ns) {
 // With more than 32 rows a block 6 and 8 only where their parts are whole groups: 100 rows 8192 -> 2048 11.9 / 12.6. (Where 4 put a CTA on
 // each SM, 6 can lose: 16 rows 6144 -> 4096 8.9 / 9.3; one row 8.5 / 8.3.) Else 2 or 1. 0: no one round.
 static int splits_for(const LinearArgs& a, int bm, int64_t units) {
-  const int* resident = linear_tc_resident(bm);
+  const LinearResident resident = linear_tc_resident(bm);
   int best = 0, best_groups = 0;
   for (int splits : {4, 6, 8, 2, 1}) {
     if (units <= 8 && splits >= 4) splits = 12 - splits;
-    if (splits > a.tiles_k || (splits < 4 && best) || units > resident[splits]) continue;
+    if (splits > a.tiles_k || (splits < 4 && best) || units > resident.of[splits]) continue;
     if (splits > 4 && bm > 32 && a.tiles_k % (splits * kSfGroup)) continue;
     const int groups = ((a.tiles_k + splits - 1) / splits + kSfGroup - 1) / kSfGroup;
     if (!best || groups < best_groups) best = splits, best_groups = groups;

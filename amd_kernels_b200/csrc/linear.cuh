@@ -44,6 +44,11 @@ struct LinearArgs {
   LinearAct act;
 };
 
+// of[splits]: clusters of so many CTAs of the one-CTA kernel that are resident at once
+struct LinearResident {
+  int of[9];
+};
+
 // Two fp32 values an instruction (add, mul and fma of f32x2, each half rounded as the scalar one): the epilogues of wide products are
 // bound by instructions, and by fetching them.
 struct F2 {

@@ -597,10 +597,8 @@ static int make_rows_map(CUtensorMap* map, const void* base, int64_t n, int64_t 
 
 template <int KIND, bool MX>
 static int linear_pairs() {
-  static std::mutex mu;
-  static int pairs[kMaxDevices] = {};
-  static bool known[kMaxDevices] = {};
-  return resident_pairs_of(linear_pair_kernel<KIND, MX>, LinearPairCfg::kThreads, LinearPairCfg::kSmemBytes, mu, known, pairs);
+  static PerDeviceAnswer<int> count;
+  return resident_pairs_of(linear_pair_kernel<KIND, MX>, LinearPairCfg::kThreads, LinearPairCfg::kSmemBytes, count);
 }
 
 template <int KIND, bool MX>

@@ -489,30 +489,25 @@ static int launch_linear_tc(const LinearArgs& a, int splits, int32_t* status, cu
 // an SM for kernels that use tensor memory, whatever their shared memory (it says one at 60 KB too); two run (288 CTAs in clusters of two
 // take the time of 192), so its number is doubled.
 template <int BM>
-static const int* resident_clusters() {
-  static std::mutex mu;
-  static bool known[kMaxDevices] = {};
-  static int clusters[kMaxDevices][9] = {};
-  static const int none[9] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return none;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!known[dev]) {
-    if (configure_linear_tc<BM, false>()) return none;
+static LinearResident resident_clusters() {
+  static PerDeviceAnswer<LinearResident> answer;
+  return answer.get([](LinearResident& clusters) {
+    if (configure_linear_tc<BM, false>()) return false;
+    bool all = true;
     for (const int splits : {1, 2, 4, 6, 8}) {
       int got = sm_count();
       cudaLaunchAttribute attr[2];
       const cudaLaunchConfig_t cfg = linear_tc_config<BM, false>(sm_count(), splits, attr, nullptr);
-      if (splits > 1 && cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM, false>, &cfg) != cudaSuccess) got = 0;
+      const bool ok = splits == 1 || cudaOccupancyMaxActiveClusters(&got, linear_tc_kernel<BM, false>, &cfg) == cudaSuccess;
       (void)cudaGetLastError();
-      clusters[dev][splits] = LinearCfg<BM>::kCtasPerSm * got;
+      clusters.of[splits] = ok ? LinearCfg<BM>::kCtasPerSm * got : 0;
+      all = all && ok;
     }
-    known[dev] = true;
-  }
-  return clusters[dev];
+    return all;
+  });
 }
 
-const int* linear_tc_resident(int bm) {
+LinearResident linear_tc_resident(int bm) {
   return bm == 16 ? resident_clusters<16>() : bm == 32 ? resident_clusters<32>() : bm == 64 ? resident_clusters<64>() : resident_clusters<128>();
 }
 

@@ -406,11 +406,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SharedPairCfg<MODE>:
 // ------------------------------------------------------------------------------------------------ host side
 template <int MODE>
 static int shared_pairs() {
-  static std::mutex mu;
-  static int pairs[kMaxDevices] = {};
-  static bool known[kMaxDevices] = {};
-  return resident_pairs_of(shared_pair_kernel<MODE>, SharedPairCfg<MODE>::kThreads, SharedPairCfg<MODE>::kSmemBytes, mu, known,
-                           pairs);
+  static PerDeviceAnswer<int> count;
+  return resident_pairs_of(shared_pair_kernel<MODE>, SharedPairCfg<MODE>::kThreads, SharedPairCfg<MODE>::kSmemBytes, count);
 }
 
 template <int MODE>

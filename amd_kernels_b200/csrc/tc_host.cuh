@@ -74,6 +74,27 @@ struct PerDeviceOnce {
   }
 };
 
+// What is asked of a device once (how many clusters of a kernel it holds), with that device current, under a lock. `ask(t)` fills t and
+// says whether all of it was answered: an answer is remembered, a query that failed is asked again by the next call.
+template <typename T>
+struct PerDeviceAnswer {
+  std::mutex mu;
+  bool known[kMaxDevices] = {};
+  T value[kMaxDevices] = {};
+  template <typename F>
+  T get(F&& ask) {
+    T t = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return t;
+    std::lock_guard<std::mutex> lock(mu);
+    if (known[dev]) return value[dev];
+    if (ask(t)) {
+      value[dev] = t;
+      known[dev] = true;
+    }
+    return t;
+  }
+};
 
 static inline bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 

@@ -69,34 +69,28 @@ static inline int make_flat_map(CUtensorMap* map, const void* base, uint64_t row
   return r == CUDA_SUCCESS ? 0 : B200MOE_E_DRIVER;
 }
 
-// Pairs of `kernel` that can be resident at once on the current device (0: cluster launch unavailable); asked once per device
-// and kernel (`known` and `pairs` are the kernel's own arrays of kMaxDevices, `mu` their lock).
+// Pairs of `kernel` that can be resident at once on the current device (0: cluster launch unavailable, or it cannot be asked now); `count`
+// is the kernel's own.
 template <typename K>
-static inline int resident_pairs_of(K kernel, int threads, int smem, std::mutex& mu, bool* known, int* pairs) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!known[dev]) {
-    int n = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(2 * sm_count());
-      cfg.blockDim = dim3(threads);
-      cfg.dynamicSmemBytes = smem;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
-    }
+static inline int resident_pairs_of(K kernel, int threads, int smem, PerDeviceAnswer<int>& count) {
+  return count.get([&](int& n) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * sm_count());
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess;
     (void)cudaGetLastError();
-    pairs[dev] = n;
-    known[dev] = true;
-  }
-  return pairs[dev];
+    if (!ok) n = 0;
+    return ok;
+  });
 }
 
 // Launches `clusters` CTA pairs with programmatic stream serialisation.
