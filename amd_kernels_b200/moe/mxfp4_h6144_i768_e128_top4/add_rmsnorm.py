@@ -10,6 +10,7 @@ from .tail import TailOutput
 
 MAX_H = 32768
 _BF16, _U8 = torch.bfloat16, torch.uint8
+CODE_DTYPES, SCALE_DTYPES = (torch.uint8, torch.float8_e4m3fn), (torch.uint8, torch.float8_e8m0fnu)
 
 
 def row_stride(name, t, m, h, one_row=False):
@@ -30,14 +31,14 @@ def check_rows(name, t, shape, device):
 
 
 def check_mxfp8(name, codes, scales, m, width, device):
-    """Contiguous [m, width] and [m, width / 32] of one byte each (uint8, or float8 of the two formats)."""
+    """Contiguous [m, width] and [m, width / 32], uint8 or float8 of the two formats (E4M3FN, E8M0: a byte of another means another value)."""
     if codes is None or scales is None:
         raise ValueError(f"{name}: codes and scales come together")
-    if ((codes.dtype is not _U8 and codes.element_size() != 1) or codes.shape != (m, width) or not codes.is_contiguous()
-            or (scales.dtype is not _U8 and scales.element_size() != 1) or scales.shape != (m, width // 32)
+    if (codes.dtype not in CODE_DTYPES or codes.shape != (m, width) or not codes.is_contiguous()
+            or scales.dtype not in SCALE_DTYPES or scales.shape != (m, width // 32)
             or not scales.is_contiguous() or codes.get_device() != device or scales.get_device() != device):
-        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] and scales [{m}, {width // 32}] of one byte each on "
-                         f"device {device}")
+        raise ValueError(f"{name}: expected contiguous codes [{m}, {width}] (uint8 or float8_e4m3fn) and scales [{m}, {width // 32}] "
+                         f"(uint8 or float8_e8m0fnu) on device {device}")
 
 
 def new_rows(m, width, dtype, like):

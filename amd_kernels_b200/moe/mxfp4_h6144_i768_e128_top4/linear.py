@@ -9,7 +9,7 @@ from dataclasses import dataclass
 import torch
 
 from ... import _lib
-from .add_rmsnorm import check_mxfp8, check_rows, launch_on, new_rows, row_stride
+from .add_rmsnorm import CODE_DTYPES, SCALE_DTYPES, check_mxfp8, check_rows, launch_on, new_rows, row_stride
 from .chain import status_word
 
 MAX_DIM, MAX_ROWS = 1 << 20, 1 << 24
@@ -34,11 +34,11 @@ class LinearWeights:
 
     @classmethod
     def from_row_major(cls, w, scale, bias=None, *, gated: bool = False):
-        """From row-major E4M3 codes [rows, K] and E8M0 scales [rows, K / 32] (one byte an element, any dtype of that size) and a bias
+        """From row-major E4M3 codes [rows, K] (uint8 or float8_e4m3fn), E8M0 scales [rows, K / 32] (uint8 or float8_e8m0fnu) and a bias
         [rows] of any floating type. K a multiple of 32, rows a multiple of 8. ``gated``: the first half of the rows are the gate,
         the second half the up projection (each a multiple of 32); the activation of the call is then a gated one."""
-        if w.ndim != 2 or w.element_size() != 1 or scale.element_size() != 1:
-            raise ValueError("expected codes [rows, K] and scales [rows, K / 32] of one byte each")
+        if w.ndim != 2 or w.dtype not in CODE_DTYPES or scale.dtype not in SCALE_DTYPES:
+            raise ValueError("expected E4M3 codes [rows, K] (uint8 or float8_e4m3fn) and E8M0 scales [rows, K / 32] (uint8 or float8_e8m0fnu)")
         rows, k = w.shape
         if not w.is_cuda or scale.device != w.device or (bias is not None and bias.device != w.device):
             raise ValueError("weights must be CUDA tensors of one device")

@@ -197,3 +197,43 @@ def test_without_resident_pairs_the_one_cta_kernel_takes_many_rows(inter):
                  dict(m=5000, c=8 << 20, s=9 << 20, o=None, oc=16 << 20, osc=12 << 20)):
         one_row = linear_call(lib, **{**call, "m": 1})
         assert one_row > 0 and linear_call(lib, **call) == one_row  # a CUDA error code, the same for one row
+
+
+OTHER_BYTES = [torch.int8, torch.bool, torch.float8_e5m2, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz]
+
+
+@pytest.mark.parametrize("dtype", OTHER_BYTES + [torch.float8_e8m0fnu])
+def test_codes_of_another_format_are_refused(dtype):
+    """The same byte stands for another value in the other formats (E4M3FNUZ: half of it)."""
+    u8 = lambda *s: torch.zeros(s, dtype=U8)  # noqa: E731
+    w, bad = weights(), u8(4, 96).view(dtype)
+    refused(P.mxfp8_linear, (bad, u8(4, 3)), w)
+    refused(P.mxfp8_linear, (u8(4, 96), u8(4, 3)), w, out=(u8(4, 64).view(dtype), u8(4, 2)))
+    refused(P.mxfp8_quant, torch.zeros((4, 96), dtype=BF16), out=(bad, u8(4, 3)))
+    x, r, nw = norm_inputs()
+    refused(P.add_rmsnorm_mxfp8, x, r, nw, out=P.TailOutput(None, u8(4, 64).view(dtype), u8(4, 2), None))
+    with pytest.raises(ValueError, match="E4M3"):
+        P.LinearWeights.from_row_major(u8(64, 96).view(dtype), u8(64, 3))
+
+
+@pytest.mark.parametrize("dtype", OTHER_BYTES + [torch.float8_e4m3fn])
+def test_scales_of_another_format_are_refused(dtype):
+    u8 = lambda *s: torch.zeros(s, dtype=U8)  # noqa: E731
+    refused(P.mxfp8_linear, (u8(4, 96), u8(4, 3).view(dtype)), weights())
+    refused(P.mxfp8_linear, (u8(4, 96), u8(4, 3)), weights(), out=(u8(4, 64), u8(4, 2).view(dtype)))
+    refused(P.mxfp8_quant, torch.zeros((4, 96), dtype=BF16), out=(u8(4, 96), u8(4, 3).view(dtype)))
+    x, r, nw = norm_inputs()
+    refused(P.add_rmsnorm_mxfp8, x, r, nw, out=P.TailOutput(None, u8(4, 64), u8(4, 2).view(dtype), None))
+    with pytest.raises(ValueError, match="E8M0"):
+        P.LinearWeights.from_row_major(u8(64, 96), u8(64, 3).view(dtype))
+
+
+def test_bytes_and_their_own_formats_are_taken():
+    u8 = lambda *s: torch.zeros(s, dtype=U8)  # noqa: E731
+    own = lambda c, s: (c.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu))  # noqa: E731
+    x = u8(4, 96), u8(4, 3)
+    refused(P.mxfp8_linear, own(*x), weights(), out=own(u8(4, 64), u8(4, 2)), why="nothing is launched")
+    refused(P.mxfp8_linear, x, weights(), out=(u8(4, 64), u8(4, 2)), why="nothing is launched")
+    refused(P.mxfp8_quant, torch.zeros((4, 96), dtype=BF16), out=own(*x), why="nothing is launched")
+    n, r, nw = norm_inputs()
+    refused(P.add_rmsnorm_mxfp8, n, r, nw, out=P.TailOutput(None, *own(u8(4, 64), u8(4, 2)), None), why="nothing is launched")
