@@ -10,8 +10,9 @@
 // One pass: a row stays in registers between its sum of squares and its outputs. Every thread adds its own squares in rising column
 // order, then a warp tree, then the warp sums in order: the bits of a row depend on its width alone, never on the other rows.
 //
-// Bound: HBM. 16384 x 6144 with a residual and all outputs, 909 MB, takes 143 us (0.97 of the copy rate); one row 2.6 us, what a launch and two
-// trips to memory take.
+// Bound: HBM. 16384 x 6144 with a residual and all outputs, 909 MB, takes 145 us (0.96 of the copy rate); one row 2.6 us, what a launch and two
+// trips to memory take. Wide rows keep fewer bytes in flight an SM (16384 columns: one CTA of 512 threads with 74 registers; above, the weights
+// come behind the sum): 4096 x 8192 48 us (0.96 of the copy rate), 4096 x 16384 123 (0.75), 2048 x 32768 145 (0.64); one row of 32768 8.2.
 #include "add_rmsnorm.cuh"
 #include "tc_host.cuh"
 

@@ -7,7 +7,7 @@ namespace b200moe {
 
 // Weights: first the codes, [row tile][K-tile] images of 128 weight rows x 128 K-elements, 16384 bytes of E4M3 as the 128-byte swizzle
 // lays them in shared memory; behind them the scales, [row tile][K-tile] atoms of 512 bytes, so that those of several K-tiles are one
-// copy. Rows and columns beyond the matrix are zeros. Gated weights (gate rows, then up rows) are interleaved in groups of 32,
+// copy. Rows and columns beyond the matrix are zero codes with scale byte 127. Gated weights (gate rows, then up rows) are interleaved in groups of 32,
 // [gate 32 | up 32 | gate 32 | up 32], so that a tile holds 64 output columns with both halves.
 constexpr int kLinearImageBytes = 128 * 128;
 constexpr int kLinearTileBytes = kLinearImageBytes + kAtomBytes;

@@ -16,10 +16,11 @@
 //               leaves by TMA. (A thread's own 16- or 32-byte pieces of its row cost the shared memory a cycle each, cycles in which the
 //               operands of the MMAs wait: with them a residual made 16384 x 6144 -> 6144 28 % slower.)
 // 12 warps start with 168 registers; the issuing warpgroup drops to 88, the epilogue's rise to 208 (4 x 88 + 8 x 208 = 12 x 168: the
-// exchange must balance inside what the CTA was given at launch).
+// exchange must balance inside what the CTA was given at launch). What does not fit the 168 at the start spills: up to 44 bytes stored and 200
+// loaded a thread, in all forms.
 //
-// What bounds it: the tensor pipe for long sums and many rows (4095 x 6144 -> 8192: busy 77 % of the cycles; the rest are the start, the ends
-// of units and waits for L2, 14 TB/s of operands) and the power limit: back to back the clock falls from 1.9 to 1.3 GHz, where
+// What bounds it: the tensor pipe for long sums and many rows (4095 x 6144 -> 8192: busy 75 % of the cycles; the rest are the start, the ends
+// of units and waits for L2, 1.8 GB of operands at 12.5 TB/s) and the power limit: back to back the clock falls from 1.9 to 1.3 GHz, where
 // 16384 x 6144 -> 6144 takes 538 us (2.3 PFLOP/s; 445 us in a short burst, 2.8). A call of few K-tiles is bound by its epilogue and by
 // what starting and ending it costs, 11 us in all.
 #include "linear.cuh"

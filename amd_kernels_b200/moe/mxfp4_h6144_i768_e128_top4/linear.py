@@ -85,7 +85,9 @@ def mxfp8_linear(x, w: LinearWeights, *, activation: str | None = None, residual
     """``y = activation(x @ w.T + bias) + residual``, fp32 until one rounding at the end.
 
     ``x``: MXFP8 rows as a pair (codes [M, K], scales [M, K / 32]), or bf16 [M, K], quantised as by
-    ``mxfp8_quant`` (up to 64 rows inside the product's launch, more in one in front of it; the same bits). M may be 0.
+    ``mxfp8_quant`` (up to 64 rows inside the product's launch, more in one in front of it; the same bits). M may be 0. Rows
+    for weights wider than some 6144 x 6144, rows that several products read, and most captured calls are faster quantised once
+    with ``mxfp8_quant``.
     ``activation``: None, "relu", "silu", "gelu" (exact), "gelu_tanh"; for gated weights "swiglu" (silu(gate) * up) or "swiglu_oai"
     (the MoE layer's: clamped, alpha 1.702, up + 1). ``residual`` bf16 [M, N], rows any multiple of 8 elements apart.
     Returns bf16 [M, N], or with ``mxfp8_out`` the pair (codes [M, N], scales [M, N / 32]) that the next product reads.

@@ -458,7 +458,8 @@ int b200moe_add_rmsnorm_quant(const b200moe_norm_call* call, void* stream);
 
 /* Weights: row-major E4M3 codes [rows][k] (16-byte aligned) and E8M0 scales [rows][k/32] -> tiles, b200moe_linear_weight_bytes bytes
  * (0: a shape that is not taken), 128-byte aligned. Layout: [row tile of 128][K-tile of 128] images of 16384 bytes of codes (128-byte
- * swizzle), then [row tile][K-tile] scale atoms; what is beyond the matrix is zero; gated rows interleaved [gate 32 | up 32] twice a tile. */
+ * swizzle), then [row tile][K-tile] scale atoms; what is beyond the matrix are zero codes with
+ * scale byte 127; gated rows interleaved [gate 32 | up 32] twice a tile. */
 size_t b200moe_linear_weight_bytes(int64_t rows, int64_t k, int gated);
 int b200moe_preshuffle_linear(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int gated, uint8_t* tiles,
                               void* stream);
