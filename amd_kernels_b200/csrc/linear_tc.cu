@@ -16,10 +16,11 @@
 // QUANT, for a few bf16 rows: there is no launch that quantises them. Warps 4-7, idle until the sum is there, quantise the block's rows
 // K-tile by K-tile into the stage, codes and scale atom, while the weights stream; every CTA does it again for its weight tile (the
 // rows are a few hundred KB in L2). A stage is then one barrier: image, weight atom and tokens. It saves a launch, which counts where the host
-// is the bound (two eager calls 15 us, the one 9.2 to 16 to 4096 columns, 17.7 to 50 to 12288); on the device the repeated work mostly costs more
-// than a launch in front. K = 6144, captured, us inside / quantised in front / from MXFP8 rows: 16 rows to 4096 columns 8.8 / 9.3 / 7.7, to 12288 17.6 / 14.1 / 12.7; 64 rows 16.1 / 11.6 / 9.8 and
-// 49.6 / 16.6 / 16.8; one row 10.5 / 8.4 / 7.2 and 24.6 / 13.5 / 12.9 (a zero takes the slow way through the scale's division, so rows of
-// zeros and the empty ones of a block cost most: 16 rows to 12288 17.3, 27.7 with 15 of them zero).
+// is the bound (two eager calls 15 us, the one 9.2 to 16 to 4096 columns, 17.7 to 50 to 12288); on the device the repeated work mostly costs
+// more than a launch in front. K = 6144, captured, us inside / quantised in front / from MXFP8 rows: 16 rows to 4096 columns 8.8 / 9.3 / 7.7,
+// to 12288 17.6 / 14.1 / 12.7; 64 rows 16.1 / 11.6 / 9.8 and 49.6 / 16.6 / 16.8; one row 10.5 / 8.4 / 7.2 and 24.6 / 13.5 / 12.9 (a zero takes
+// the slow way through the scale's division, so rows of zeros and the empty ones of a block cost most: 16 rows to 12288 17.3, 27.7 with 15
+// of them zero).
 //
 // Weights of more tiles than CTAs run at once (37888 rows) go without a split, in rounds: one row 6144 -> 131072 120 us (127 at the copy rate), 64
 // rows 133, 128 rows 159; just above the limit a round of few tiles is the price: one row -> 37888 39.6, -> 38016 48.4.
